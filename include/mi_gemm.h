@@ -366,6 +366,149 @@ int mi_rmsnorm_bwd(void* stream, const void* dy, const void* x, const void* weig
                    void* workspace, size_t workspace_bytes);
 
 /*
+ * Rotary positions.  At position p, pair i < rot_dim / 2 of a head turns by the angle
+ * p * inv_freq[i]:
+ *   a' = scale (a cos - b sin),  b' = scale (b cos + a sin)
+ * with (a, b) = (x[i], x[i + rot_dim/2]) or, interleaved, (x[2i], x[2i+1]); components
+ * rot_dim .. head_dim-1 are copied.  inv_freq is device memory, fp32 [rot_dim/2]; the angle
+ * is the product in 64 bits, so far positions lose nothing.  A schedule for longer contexts
+ * is another inv_freq (and, where it says so, a scale other than 1).
+ */
+typedef struct mi_rotary {
+  const float* inv_freq;    /* device, [rot_dim / 2]                                        */
+  int64_t rot_dim;          /* even, 0 < rot_dim <= head_dim                                */
+  int32_t interleaved;      /* 0: halves of the rotated part, 1: neighbouring components    */
+  float scale;              /* factor of the rotated components, finite                     */
+  const int32_t* positions; /* device, one per token (row pitch positions_ld between the
+                               sequences, 0 shares one row), or NULL: mi_rope takes
+                               pos0 + t, mi_kv_append the token's place in its sequence     */
+  int64_t positions_ld;
+  int64_t pos0;
+} mi_rotary;
+
+/* One tensor of an mi_rope call: element c of head h of token t of sequence b is at
+ * src[b*src_b + t*src_t + h*src_h + c] and goes to dst[b*dst_b + t*dst_t + h*dst_h + c]
+ * (strides in elements, components contiguous). */
+typedef struct mi_rope_part {
+  const void* src;
+  void* dst;
+  int64_t heads;
+  int64_t src_b, src_t, src_h;
+  int64_t dst_b, dst_t, dst_h;
+  int32_t rotate;   /* 0: copied as it is (V beside Q and K) */
+  int32_t reserved; /* 0 */
+} mi_rope_part;
+
+/*
+ * Rotates up to four tensors of the same tokens in one launch, for instance the Q, K and V
+ * columns of a fused QKV product into the [B, heads, T, d] operands of mi_flash_attn_fwd.
+ * inverse != 0 turns by the negated angle (same scale): the transposed map, so the backward
+ * takes dQ, dK, dV as src and the product's gradient as dst.  dtype MI_BF16 or MI_F32 for
+ * all parts; rotated in fp32 and rounded once.  dst may be src itself with the same strides;
+ * otherwise no dst may overlap any other memory of the call, and the strides of a dst must
+ * not map two elements to one place.  Any strides and alignments of whole elements; rows
+ * that are whole 16-byte vectors are fastest.  The engine rotates between its QKV product
+ * and its attention (rope_forward, rope_backward, MetalBridge.mm:2097).
+ */
+int mi_rope(void* stream, const mi_rope_part* parts, int64_t n_parts, int64_t batch, int64_t seq_len,
+            int64_t head_dim, const mi_rotary* rotary, int32_t inverse, int32_t dtype);
+
+/*
+ * A cache of K and V in pages of page_size tokens: element c of head h of slot i of page p is
+ * at k[p*page_stride + h*head_stride + i*slot_stride + c], and v alike (bf16, strides in
+ * elements).  Strides are multiples of 8 and k and v are 16-byte aligned.
+ */
+typedef struct mi_paged_cache {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t page_size; /* a power of two */
+  int64_t n_kv, head_dim;
+  int64_t page_stride, head_stride, slot_stride;
+} mi_paged_cache;
+
+/*
+ * The sequences of one call, in device memory.  New tokens are rows 0 .. total_q-1 of the
+ * call's tensors: sequence s has rows q_start[s] .. q_start[s+1]-1, and they are the last
+ * tokens of its kv_len[s], so the first of them is at position kv_len[s] - (q_start[s+1] -
+ * q_start[s]).  Position p lies in page pages[s*pages_ld + p / page_size], slot p % page_size.
+ * Sequences may have no new token, and rows behind the last sequence are left as they are.
+ * Positions below zero or past max_pages pages, and pages outside [0, num_pages), hold
+ * nothing: they are not written, and their keys are not seen.
+ */
+typedef struct mi_paged_seqs {
+  int64_t n_seqs, total_q;
+  const int32_t* q_start; /* [n_seqs + 1], starting at 0 and not decreasing; NULL: one new token
+                             for each sequence (total_q = n_seqs)                           */
+  const int32_t* kv_len;  /* [n_seqs] tokens with the new ones                               */
+  const int32_t* pages;   /* [n_seqs, pages_ld], max_pages entries of each row used          */
+  int64_t max_pages, pages_ld;
+} mi_paged_seqs;
+
+/*
+ * New tokens enter the cache: K [total_q, n_kv, head_dim] is rotated into its pages, V copied
+ * into its pages, and Q [total_q, n_heads, head_dim] rotated into q_out (q may be NULL: cache
+ * only; q_out may be q with the same strides).  All bf16; row strides (k_t: between tokens,
+ * k_h: between heads) in elements.  rotary NULL: nothing is rotated.  Two new tokens must not
+ * share a slot.  Without rotary->positions a token's angle is that of its place in its
+ * sequence.
+ */
+int mi_kv_append(void* stream, const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h,
+                 int64_t n_heads, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h,
+                 const mi_paged_cache* cache, const mi_paged_seqs* seqs, const mi_rotary* rotary);
+
+/*
+ * Attention of each sequence's new tokens over its cached ones (mi_kv_append has put the new
+ * ones there before): row r, head h of a sequence with n keys at position p
+ *   O[r, h] = softmax(scale * q K^T, keys 0 .. p (causal) or 0 .. n-1) V
+ * with the keys of head h / (n_heads / n_kv).  Q and O [total_q, n_heads, head_dim] bf16, row
+ * strides in elements and multiples of 8, 16-byte aligned; head_dim a multiple of 8 up to 128;
+ * O may be Q with the same strides.  lse (optional, fp32 [total_q, n_heads]) receives
+ * the natural-log log-sum-exp.  A row without a key gets zeros and -inf.  max_q_len and
+ * max_kv_len are the host's bounds on the new and cached tokens of a sequence, from which the
+ * launch is shaped: max_q_len must not be exceeded (rows past it are not computed), a
+ * sequence longer than max_kv_len is right but slower.  Long sequences with few rows are
+ * split over workgroups whose parts a second kernel joins in a fixed order; their fp32 parts
+ * lie in the workspace (16-byte aligned, mi_paged_attn_workspace_size bytes, or less: fewer
+ * parts, NULL: no split).  Results do not depend on timing.
+ */
+int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h, float* lse,
+                  int64_t n_heads, const mi_paged_cache* cache, const mi_paged_seqs* seqs, int64_t max_q_len,
+                  int64_t max_kv_len, int32_t causal, float scale, void* workspace, size_t workspace_bytes);
+
+size_t mi_paged_attn_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t n_seqs, int64_t total_q,
+                                    int64_t max_q_len, int64_t max_kv_len);
+
+/*
+ * How mi_sample picks.  A device pointer gives every row its own value ([rows]); where it is
+ * NULL the value beside it holds for all rows.
+ */
+typedef struct mi_sampling {
+  const float* temperature; /* <= 0: the largest logit                                       */
+  const int32_t* top_k;     /* <= 0: off                                                     */
+  const float* top_p;       /* >= 1: off                                                     */
+  const float* min_p;       /* <= 0: off                                                     */
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+} mi_sampling;
+
+/*
+ * One token for each row of logits [rows, ld] (MI_BF16 or MI_F32).  Tokens are ordered by
+ * logit, equal ones by index, lowest first, and weighted w = exp((x - max x) / temperature).
+ * Kept are, in this order: the first top_k; of those the shortest run from the front whose
+ * weight reaches top_p of theirs (at least one token); of those the ones with w >= min_p.
+ * tokens[r] is the lowest index at which the kept weights, summed in index order, exceed
+ * u[r] times their total (u fp32 in [0, 1), given by the caller), probs[r] (optional, fp32)
+ * its share of the total.  Weights are computed in 64 bits and summed as whole multiples of
+ * 2^-(62 - b), b the bits of vocab - 1 (2^-46 for 65536 entries), so sums do not depend on their
+ * order and a token of less than half of that is never drawn.  NaN logits weigh nothing; a +inf logit takes all; a row without a
+ * logit above -inf gets token -1 and share 0.  vocab at most 2^24.
+ */
+int mi_sample(void* stream, const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t vocab,
+              const mi_sampling* how, const float* u, int32_t* tokens, float* probs);
+
+/*
  * Weight conversion for checkpoint loading: rows [row0, row0 + rows) x columns
  * [0, cols) of a row-major source matrix (leading dimension src_ld, dtype MI_F32,
  * MI_BF16 or MI_F16) into dst (MI_F32, or MI_BF16 rounded to nearest even):

@@ -24,6 +24,7 @@
 #include "mi_norm.hpp"
 #include "mi_convert.hpp"
 #include "mi_gemm_kernels.hpp"
+#include "mi_host.hpp"
 #include "mi_skinny.hpp"
 
 using namespace mig;
@@ -108,6 +109,16 @@ int current_cus() {
   if (hipGetDevice(&d) != hipSuccess) return 256;
   return (d >= 0 && d < 64 && g_dev[d].ok) ? g_dev[d].cus : 256;
 }
+
+}  // namespace
+
+namespace mig {
+int host_error(int code, const char* text) { return fail(code, "%s", text); }
+int host_device() { return init_devices(); }
+int host_cus() { return current_cus(); }
+}  // namespace mig
+
+namespace {
 
 // ---- kernel table ------------------------------------------------------------
 

@@ -39,7 +39,8 @@ C_SYMBOLS = (
     "mi_profiler_begin_step", "mi_profiler_count", "mi_profiler_record", "mi_profiler_totals",
     "mi_profiler_reset", "mi_gemm_noalloc", "mi_flash_attn_fwd_scaled", "mi_flash_attn_bwd_scaled",
     "mi_convert_matrices", "mi_rmsnorm_fold_weight", "mi_lm_head_xent",
-    "mi_lm_head_xent_workspace_size",
+    "mi_lm_head_xent_workspace_size", "mi_rope", "mi_kv_append", "mi_paged_attn",
+    "mi_paged_attn_workspace_size", "mi_sample",
 )
 MI_ATTN_O_BHTD, MI_ATTN_O_BTHD = 0, 1
 
@@ -80,6 +81,47 @@ class MiConvertJob(ctypes.Structure):
         ("src_ld", ctypes.c_int64), ("row0", ctypes.c_int64), ("rows", ctypes.c_int64),
         ("cols", ctypes.c_int64), ("dst", ctypes.c_void_p), ("dst_dtype", ctypes.c_int32),
         ("reserved", ctypes.c_int32), ("dst_ld", ctypes.c_int64),
+    ]
+
+
+class MiRotary(ctypes.Structure):
+    _fields_ = [
+        ("inv_freq", ctypes.c_void_p), ("rot_dim", ctypes.c_int64), ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("positions", ctypes.c_void_p), ("positions_ld", ctypes.c_int64),
+        ("pos0", ctypes.c_int64),
+    ]
+
+
+class MiRopePart(ctypes.Structure):
+    _fields_ = [
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("heads", ctypes.c_int64),
+        ("src_b", ctypes.c_int64), ("src_t", ctypes.c_int64), ("src_h", ctypes.c_int64),
+        ("dst_b", ctypes.c_int64), ("dst_t", ctypes.c_int64), ("dst_h", ctypes.c_int64),
+        ("rotate", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class MiPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64), ("n_kv", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64),
+    ]
+
+
+class MiPagedSeqs(ctypes.Structure):
+    _fields_ = [
+        ("n_seqs", ctypes.c_int64), ("total_q", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("max_pages", ctypes.c_int64),
+        ("pages_ld", ctypes.c_int64),
+    ]
+
+
+class MiSampling(ctypes.Structure):
+    _fields_ = [
+        ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+        ("min_p", ctypes.c_void_p), ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int32),
+        ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float),
     ]
 
 
@@ -170,6 +212,20 @@ def load_library():
     L.mi_convert_matrix.argtypes = [vp, vp, i32, i64, i64, i64, i64, i32, vp, i32, i64]
     L.mi_convert_matrices.restype = ctypes.c_int
     L.mi_convert_matrices.argtypes = [vp, ctypes.POINTER(MiConvertJob), i64]
+    L.mi_rope.restype = ctypes.c_int
+    L.mi_rope.argtypes = [vp, ctypes.POINTER(MiRopePart), i64, i64, i64, i64, ctypes.POINTER(MiRotary),
+                          i32, i32]
+    L.mi_kv_append.restype = ctypes.c_int
+    L.mi_kv_append.argtypes = [vp, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, vp, i64, i64,
+                               ctypes.POINTER(MiPagedCache), ctypes.POINTER(MiPagedSeqs),
+                               ctypes.POINTER(MiRotary)]
+    L.mi_paged_attn.restype = ctypes.c_int
+    L.mi_paged_attn.argtypes = [vp, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.POINTER(MiPagedCache),
+                                ctypes.POINTER(MiPagedSeqs), i64, i64, i32, f32, vp, ctypes.c_size_t]
+    L.mi_paged_attn_workspace_size.restype = ctypes.c_size_t
+    L.mi_paged_attn_workspace_size.argtypes = [i64] * 7
+    L.mi_sample.restype = ctypes.c_int
+    L.mi_sample.argtypes = [vp, vp, i32, i64, i64, i64, ctypes.POINTER(MiSampling), vp, vp, vp]
     L.mi_profiler_enable.restype = ctypes.c_int
     L.mi_profiler_enable.argtypes = [ctypes.c_int]
     L.mi_profiler_begin_step.restype = ctypes.c_int
@@ -1015,6 +1071,328 @@ class RMSNorm:
         dx, _ = rms_norm_backward(grad_output, input, self.weight, self.eps, dw=grad_weight,
                                   dw_beta=1.0)
         return dx
+
+
+# ---- rotary positions -------------------------------------------------------------
+
+def _on_device(**tensors):
+    """The tensors (None entries aside) are on the current GPU, whose stream a call goes to."""
+    torch = _torch()
+    for name, t in tensors.items():
+        if t is not None and (t.device.type != "cuda" or t.device.index != torch.cuda.current_device()):
+            raise ValueError(f"{name} is on {t.device}: a tensor on the current GPU is needed")
+
+
+def _done(fn, st, sync):
+    (_finish if sync is None else _check)(fn, st)
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
+    """(inv_freq fp32 [rot_dim / 2] on device, scale) of rotary positions: f_i = base^(-2i / rot_dim).
+    scaling, for contexts `factor` times as long as the trained ones:
+      ("linear", factor)   positions shrink: f_i / factor
+      ("base", factor)     base * factor^(rot_dim / (rot_dim - 2)): the slowest pair slows by the
+                           factor, the fastest stays
+      ("bands", factor, low, high, length)   by how often a pair turns over the trained length,
+                           r_i = length f_i / 2 pi: f_i where r_i >= high, f_i / factor where
+                           r_i <= low, in between (1 - g) f_i / factor + g f_i with
+                           g = (r_i - low) / (high - low)
+      ("bands", factor, low, high, length, scale)   and that scale of the rotated components."""
+    torch = _torch()
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim}: an even number is needed")
+    kind = scaling[0] if scaling else None
+    if kind not in (None, "linear", "base", "bands"):
+        raise ValueError(f"unknown scaling {kind!r}")
+    if scaling and len(scaling) not in ((2,) if kind != "bands" else (5, 6)):
+        raise ValueError(f"{kind} scaling takes {'factor' if kind != 'bands' else 'factor, low, high, length[, scale]'}")
+    if scaling and not scaling[1] > 0:
+        raise ValueError("the factor must be positive")
+    if kind == "base":
+        if rot_dim == 2:
+            raise ValueError("base scaling needs two pairs")
+        base = base * scaling[1] ** (rot_dim / (rot_dim - 2))
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rot_dim)
+    if kind == "linear":
+        f = f / scaling[1]
+    elif kind == "bands":
+        factor, low, high, length = scaling[1:5]
+        if not high > low:
+            raise ValueError("bands scaling needs low < high")
+        g = ((length * f / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f / factor * (1.0 - g) + f * g
+    return f.to(torch.float32).to(device), float(scaling[5]) if kind == "bands" and len(scaling) == 6 else 1.0
+
+
+def _rotary(inv_freq, positions, positions_shape, pos0, interleaved, scale):
+    torch = _torch()
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous fp32 vector")
+    r = MiRotary()
+    r.inv_freq, r.rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
+    r.interleaved, r.scale, r.pos0 = int(bool(interleaved)), float(scale), int(pos0)
+    if positions is not None:
+        if positions.dtype != torch.int32:
+            raise ValueError("positions must be int32")
+        shape = tuple(positions.shape)
+        if shape not in (positions_shape, positions_shape[-1:]):
+            raise ValueError(f"positions {shape} for tokens {positions_shape}")
+        if positions.numel() > 1 and shape[-1] > 1 and positions.stride(-1) != 1:
+            raise ValueError("positions must have a contiguous last dimension")
+        r.positions = positions.data_ptr()
+        r.positions_ld = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
+    return r
+
+
+def _rope_part(src, dst, rotate=True):
+    """Views [B, T, heads, d] of src and dst as a part of an mi_rope call."""
+    a = MiRopePart()
+    a.src, a.dst, a.heads, a.rotate = src.data_ptr(), dst.data_ptr(), src.shape[2], int(rotate)
+    a.src_b, a.src_t, a.src_h, _ = src.stride()
+    a.dst_b, a.dst_t, a.dst_h, _ = dst.stride()
+    return a
+
+
+def _rope_call(parts, views, inv_freq, positions, pos0, inverse, interleaved, scale, sync):
+    x = views[0]
+    for v in views:
+        if v.dtype != x.dtype or (v.shape[0], v.shape[1], v.shape[3]) != (x.shape[0], x.shape[1], x.shape[3]):
+            raise ValueError("the tensors must share dtype, batch, tokens and head dimension")
+        if v.stride(-1) != 1 and v.shape[-1] > 1:
+            raise ValueError("components must be contiguous")
+    _on_device(x=x, inv_freq=inv_freq, positions=positions)
+    B, T, _, d = x.shape
+    r = _rotary(inv_freq, positions, (B, T), pos0, interleaved, scale)
+    arr = (MiRopePart * len(parts))(*parts)
+    _done("mi_rope", load_library().mi_rope(_stream(), arr, len(parts), B, T, d, ctypes.byref(r),
+                                            int(bool(inverse)), _dt(x)), sync)
+
+
+def rope(x, inv_freq, positions=None, pos0=0, layout="bthd", inverse=False, interleaved=False, scale=1.0,
+         out=None, sync=None):
+    """Rotary positions of one tensor (mi_rope), x [B,T,H,d] (layout "bthd") or [B,H,T,d] ("bhtd"),
+    bf16 or fp32, components contiguous: the first 2 * len(inv_freq) components of every head turn
+    pair by pair, halves apart or, interleaved, neighbours, by position * inv_freq; the rest is
+    copied. positions: int32 [B,T] or [T]; pos0 + t without. inverse: the backward (the gradient's
+    map). out: a tensor of x's shape, x itself for in place. Returns out."""
+    torch = _torch()
+    if layout not in ("bthd", "bhtd") or x.dim() != 4:
+        raise ValueError("x is [B,T,H,d] (bthd) or [B,H,T,d] (bhtd)")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must match x's shape and dtype")
+    a, b = (x, out) if layout == "bthd" else (x.transpose(1, 2), out.transpose(1, 2))
+    _on_device(out=out)
+    _rope_call([_rope_part(a, b)], [a, b], inv_freq, positions, pos0, inverse, interleaved, scale, sync)
+    return out
+
+
+def _split_heads(qkv, n_heads, n_kv):
+    """The Q, K and V parts of [B, T, (nH + 2 nKV) d] as [B, T, heads, d] views."""
+    B, T, n = qkv.shape
+    heads = n_heads + 2 * n_kv
+    if heads < 1 or n % heads:
+        raise ValueError(f"{n} columns are no {n_heads} + 2 * {n_kv} heads")
+    return qkv.unflatten(2, (heads, n // heads)).split((n_heads, n_kv, n_kv), dim=2)
+
+
+def rope_qkv(qkv, n_heads, n_kv, inv_freq, positions=None, pos0=0, interleaved=False, scale=1.0, sync=None):
+    """From the fused QKV product's rows to the operands of flash_attn_fwd in one launch: qkv
+    [B, T, (nH + 2 nKV) d], bf16 or fp32 -> Q [B,nH,T,d], K, V [B,nKV,T,d], contiguous, Q and K with
+    their rotary positions (Attention.cpp:68-100 splits and rotates in separate passes)."""
+    torch = _torch()
+    if qkv.dim() != 3:
+        raise ValueError("qkv is [B, T, columns]")
+    src = _split_heads(qkv, n_heads, n_kv)
+    B, T, _, d = src[0].shape
+    out = [torch.empty((B, s.shape[2], T, d), dtype=qkv.dtype, device=qkv.device) for s in src]
+    dst = [o.transpose(1, 2) for o in out]
+    parts = [_rope_part(s, t, i < 2) for i, (s, t) in enumerate(zip(src, dst))]
+    _rope_call(parts, [*src, *dst], inv_freq, positions, pos0, False, interleaved, scale, sync)
+    return tuple(out)
+
+
+def rope_qkv_backward(dQ4, dK4, dV4, inv_freq, positions=None, pos0=0, interleaved=False, scale=1.0, out=None,
+                      sync=None):
+    """Backward of rope_qkv: dQ [B,nH,T,d], dK, dV [B,nKV,T,d] (flash_attn_bwd's) -> the gradient of
+    the QKV product, [B, T, (nH + 2 nKV) d], dQ and dK turned back, in one launch."""
+    torch = _torch()
+    if dQ4.dim() != 4 or dK4.shape != dV4.shape:
+        raise ValueError("dQ is [B,nH,T,d], dK and dV [B,nKV,T,d]")
+    src = [t.transpose(1, 2) for t in (dQ4, dK4, dV4)]
+    B, T, nH, d = src[0].shape
+    nKV = src[1].shape[2]
+    shape = (B, T, (nH + 2 * nKV) * d)
+    if out is None:
+        out = torch.empty(shape, dtype=dQ4.dtype, device=dQ4.device)
+    if tuple(out.shape) != shape or (out.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError(f"out must be {shape} with a contiguous last dimension")
+    dst = _split_heads(out, nH, nKV)
+    parts = [_rope_part(s, t, i < 2) for i, (s, t) in enumerate(zip(src, dst))]
+    _on_device(dK=dK4, dV=dV4, out=out)
+    _rope_call(parts, [*src, *dst], inv_freq, positions, pos0, True, interleaved, scale, sync)
+    return out
+
+
+# ---- paged cache ------------------------------------------------------------------
+
+def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
+    """mi_paged_cache and mi_paged_seqs of caches [pages, nKV, page size, d] (any strides with
+    contiguous components) and int32 device tables."""
+    torch = _torch()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError("k_cache and v_cache are [pages, nKV, page size, d] of one shape and strides")
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16 or (k_cache.stride(3) != 1 and k_cache.shape[3] > 1):
+        raise ValueError("the caches must be bf16 with contiguous components")
+    for name, t, dim in (("pages", pages, 2), ("kv_len", kv_len, 1), ("q_start", q_start, 1)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != dim or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name} must be int32, {dim}-D, with a contiguous last dimension")
+    n = kv_len.shape[0]
+    if pages.shape[0] != n or (q_start is not None and q_start.shape[0] != n + 1):
+        raise ValueError(f"pages needs {n} rows and q_start {n + 1} entries, as kv_len has {n}")
+    if q_start is None and rows != n:
+        raise ValueError(f"{rows} rows for {n} sequences: q_start is needed")
+    _on_device(k_cache=k_cache, v_cache=v_cache, pages=pages, kv_len=kv_len, q_start=q_start)
+    c = MiPagedCache()
+    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
+    c.num_pages, c.n_kv, c.page_size, c.head_dim = k_cache.shape
+    c.page_stride, c.head_stride, c.slot_stride = k_cache.stride()[:3]
+    s = MiPagedSeqs()
+    s.n_seqs, s.total_q = n, rows
+    s.q_start = None if q_start is None else q_start.data_ptr()
+    s.kv_len, s.pages = kv_len.data_ptr(), pages.data_ptr()
+    s.max_pages = pages.shape[1]
+    s.pages_ld = pages.stride(0) if n > 1 else pages.shape[1]
+    return c, s
+
+
+def _heads_of(name, t, rows, heads, d):
+    """Strides of a bf16 [rows, heads, d] tensor."""
+    if t.dtype != _torch().bfloat16 or tuple(t.shape) != (rows, heads, d) or (t.stride(2) != 1 and d > 1):
+        raise ValueError(f"{name} must be bf16 [{rows}, {heads}, {d}] with contiguous components")
+    _on_device(**{name: t})
+    return t.stride(0), t.stride(1)
+
+
+def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out=None, inv_freq=None,
+              positions=None, interleaved=False, scale=1.0, sync=None):
+    """New tokens enter a paged cache (mi_kv_append): k, v [N, nKV, d] bf16 (views of the QKV product's
+    rows, for instance), k rotated, go to the places that pages [S, n], kv_len [S] (with the new
+    tokens) and q_start [S + 1] (int32; None: one token for each sequence) name in k_cache, v_cache
+    [pages, nKV, page size, d]. q [N, nH, d], if given, is rotated into q_out (allocated when None;
+    q itself for in place), which is returned. inv_freq None: nothing is rotated. positions: int32
+    [N], where they are not the tokens' places."""
+    torch = _torch()
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v are [tokens, nKV, d]")
+    N, nKV, d = k.shape
+    c, s = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
+    if (c.n_kv, c.head_dim) != (nKV, d):
+        raise ValueError(f"the cache has {c.n_kv} heads of {c.head_dim}, k has {nKV} of {d}")
+    ks, vs = _heads_of("k", k, N, nKV, d), _heads_of("v", v, N, nKV, d)
+    nH, qs, os_ = 0, (0, 0), (0, 0)
+    if q is not None:
+        nH = q.shape[1] if q.dim() == 3 else 0
+        qs = _heads_of("q", q, N, nH, d)
+        if q_out is None:
+            q_out = torch.empty((N, nH, d), dtype=q.dtype, device=q.device)
+        os_ = _heads_of("q_out", q_out, N, nH, d)
+    r = None
+    if inv_freq is not None:
+        _on_device(inv_freq=inv_freq, positions=positions)
+        r = ctypes.byref(_rotary(inv_freq, positions, (N,), 0, interleaved, scale))
+    elif positions is not None:
+        raise ValueError("positions without inv_freq")
+    st = load_library().mi_kv_append(_stream(), _ptr(q), *qs, _ptr(q_out) if q is not None else None, *os_, nH,
+                                     _ptr(k), *ks, _ptr(v), *vs, ctypes.byref(c), ctypes.byref(s), r)
+    _done("mi_kv_append", st, sync)
+    return q_out if q is not None else None
+
+
+def paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len) -> int:
+    """Bytes of workspace paged_attn uses (mi_paged_attn_workspace_size)."""
+    return int(load_library().mi_paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len,
+                                                           max_kv_len))
+
+
+def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None, max_kv_len=None, out=None,
+               lse=None, causal=True, scale=None, workspace="auto", sync=None):
+    """Attention of each sequence's new tokens over its pages (mi_paged_attn): q [N, nH, d] bf16, the
+    cache and tables as in kv_append, which has put the new tokens in before. Row i of a sequence's
+    n new rows sees its keys up to kv_len - n + i, or all of them (causal False). Returns out
+    [N, nH, d]; a row without keys gets zeros. lse: optional fp32 [N, nH] for the log-sum-exp of the
+    scaled scores. max_q_len: most new tokens of a sequence (N when not given; 1 without q_start);
+    max_kv_len: most cached tokens, as far as the host knows (else what the page table holds).
+    workspace: "auto" allocates it, None never splits a sequence, or a device tensor of
+    paged_attn_workspace_size bytes, which calls that may overlap must not share."""
+    torch = _torch()
+    if q.dim() != 3:
+        raise ValueError("q is [tokens, nH, d]")
+    N, nH, d = q.shape
+    c, s = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
+    if d != c.head_dim:
+        raise ValueError(f"the cache has heads of {c.head_dim}, q of {d}")
+    qs = _heads_of("q", q, N, nH, d)
+    if out is None:
+        out = torch.empty((N, nH, d), dtype=q.dtype, device=q.device)
+    os_ = _heads_of("out", out, N, nH, d)
+    if lse is not None:
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (N, nH) or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous fp32 [{N}, {nH}] tensor")
+        _on_device(lse=lse)
+    mq = 1 if q_start is None else N if max_q_len is None else int(max_q_len)
+    mk = c.page_size * s.max_pages if max_kv_len is None else int(max_kv_len)
+    if isinstance(workspace, str):
+        n = paged_attn_workspace_size(nH, c.n_kv, d, s.n_seqs, N, mq, mk)
+        workspace = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
+    elif workspace is not None:
+        _on_device(workspace=workspace)
+    wsb = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    st = load_library().mi_paged_attn(_stream(), _ptr(q), *qs, _ptr(out), *os_, _ptr(lse), nH, ctypes.byref(c),
+                                      ctypes.byref(s), mq, mk, int(bool(causal)),
+                                      1.0 / math.sqrt(d) if scale is None else float(scale), _ptr(workspace), wsb)
+    _done("mi_paged_attn", st, sync)
+    return out
+
+
+# ---- sampling ---------------------------------------------------------------------
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, prob=None, sync=None):
+    """One token for each row of logits [rows, V] (bf16 or fp32, any row stride; mi_sample) from the
+    uniform numbers u (fp32 [rows], in [0, 1)). temperature, top_k, top_p, min_p: a number for all
+    rows or a tensor [rows] (fp32, top_k int32); temperature <= 0 takes the largest logit, top_k <= 0,
+    top_p >= 1 and min_p <= 0 are off. Filters apply in the order top-k, top-p of what is left,
+    min-p; equal logits go by index, lowest first. Returns tokens (int32 [rows], into `out` if
+    given; -1 for a row without a logit above -inf); prob: optional fp32 [rows] for the picked
+    token's probability among the kept ones."""
+    torch = _torch()
+    if logits.dim() != 2:
+        raise ValueError("logits is [rows, V]")
+    rows, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("logits must have a contiguous last dimension")
+    h = MiSampling()
+    for name, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            if v.dtype != dt or tuple(v.shape) != (rows,) or not v.is_contiguous():
+                raise ValueError(f"{name} must be a number or a contiguous {dt} [{rows}] tensor")
+            _on_device(**{name: v})
+            setattr(h, name, v.data_ptr())
+        else:
+            setattr(h, name + "_all", int(v) if dt == torch.int32 else float(v))
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    for name, t, dt in (("u", u, torch.float32), ("out", out, torch.int32), ("prob", prob, torch.float32)):
+        if t is not None and (t.dtype != dt or tuple(t.shape) != (rows,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dt} [{rows}] tensor")
+    _on_device(logits=logits, u=u, out=out, prob=prob)
+    st = load_library().mi_sample(_stream(), _ptr(logits), _dt(logits), logits.stride(0) if rows > 1 else V, rows, V,
+                                  ctypes.byref(h), _ptr(u), _ptr(out), _ptr(prob))
+    _done("mi_sample", st, sync)
+    return out
 
 
 # ---- checkpoint weights ---------------------------------------------------------
