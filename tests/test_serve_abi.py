@@ -182,6 +182,19 @@ def test_struct_layouts(mi, name, cls):
     assert [(n, t) for n, t in getattr(mi, cls)._fields_] == want
 
 
+def test_packed_structs_match_the_mirrors(mi):
+    import struct
+
+    for pack, cls in ((mi._PACK_PART, mi.MiRopePart), (mi._PACK_ROTARY, mi.MiRotary), (mi._PACK_CACHE, mi.MiPagedCache),
+                      (mi._PACK_SEQS, mi.MiPagedSeqs), (mi._PACK_SAMPLING, mi.MiSampling)):
+        kinds = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+        fmt = "@" + "".join(kinds[t] for _, t in cls._fields_)
+        assert pack.__self__.format == fmt and struct.calcsize(fmt) == ctypes.sizeof(cls)
+        raw = pack(*range(1, len(fmt)))
+        got = cls.from_buffer_copy(raw)
+        assert [getattr(got, n) for n, _ in cls._fields_] == list(range(1, len(fmt)))
+
+
 def test_python_refusals(mi):
     """The Python layer's own checks, on CPU tensors, which it refuses last."""
     import torch
