@@ -1,19 +1,29 @@
 // mi_sample.hip -- one token for each row of logits, by temperature, top-k, top-p and min-p, gfx950.
 //
 // With the tokens of a row ordered by (logit descending, index ascending), each of the three
-// filters keeps a run from the front, so what is kept is fixed by one border: a logit and how many
-// of the tokens equal to it.  A row needs no sort: the border is found digit by digit in the
-// logits' bits (an order-preserving integer key), by counting tokens above (top-k) or summing their
-// weights (top-p).
+// filters keeps a run from the front, so what is kept is fixed by one border: a logit, and how many
+// of the tokens equal to it.  No sort is needed to find it:
+//   1. a histogram over the distance from the row's maximum, SMP_BINS bins evenly over the distances
+//      that can weigh anything, counts tokens (top-k) or sums weights (top-p);
+//   2. a scan over the bins finds the one in which the border lies;
+//   3. that bin's tokens (1/1000 of the row) go to LDS, where each finds its rank among them.
+// A bin that holds more than SMP_LIST of them (a row of few distinct logits) is halved by its logits'
+// bits instead, over the row, until one value is left.
 //
-// Weights w = exp((x - max) / T) are computed in 64 bits and held as integers, w * 2^shift, so every
-// sum is exact: it is the same whatever order atomics and waves add in, and a border is never moved
-// by rounding.  A weight below half of 2^-shift counts as nothing: u = 0, one of 2^24 numbers, then does
-// not draw a token whose chance is 1e-20.
+// Weights w = 2^y, y = (x - max) log2(e) / T, are computed in 64 bits and held as integers, w * 2^shift,
+// so every sum is exact: it is the same whatever order atomics and waves add in, and a border is never
+// moved by rounding.  A weight below half of 2^-shift counts as nothing: u = 0, one of 2^24 numbers,
+// then does not draw a token whose chance is 1e-20.  64 bits cost no more than 32 here (a 64-lane
+// instruction takes four cycles either way); 2^y is a table of 16 steps in LDS, a polynomial of degree 6
+// on what is left, and an addition that leaves the rounded integer in the low bits.
 //
-// One workgroup a row.
+// One workgroup a row, each wave a run of it.  A pass reads the row again, from the caches: held in
+// registers it would need every pass unrolled over them, more code than the instruction cache holds.
+// Bound by the passes' instructions, 0.2 us for each one an element at 32000 logits on a CU.
 #include <hip/hip_runtime.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "mi_gemm_device.hpp"
 #include "mi_host.hpp"
@@ -23,22 +33,23 @@ namespace {
 
 constexpr int SMP_THREADS = 1024;
 constexpr int SMP_WAVES = SMP_THREADS / 64;
-constexpr uint32_t SMP_KEY_NEG_INF = 0x007fffffu;  // key of -inf: nothing below it is a token
+constexpr int SMP_BINS = 1024;        // one for each thread in the scan
+constexpr int SMP_LIST = 1024;        // tokens of a bin that are ranked in LDS
 
 struct SampleParams {
   const void* logits;
   int64_t ld;
   int vocab, shift;
+  int layers;  // 16-byte vectors of a lane
   const float* u;
   int32_t* tokens;
   float* probs;
   mi_sampling how;
 };
 
-// Keys order as the logits do; both zeros have one key, NaN the lowest.
+// Keys order as finite floats do (halving a range of values by their bits).
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0;
-  const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
+  const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
@@ -46,9 +57,29 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ float logit_at(const void* row, int i) {
-  if constexpr (BF16) return bf16_bits_to_f32(((const uint16_t*)row)[i]);
-  else return ((const float*)row)[i];
+__device__ __forceinline__ float smp_elem(const u32x4_t& v, int e) {
+  if constexpr (BF16) return (e & 1) ? __uint_as_float(v[e >> 1] & 0xffff0000u) : bf16_bits_to_f32(v[e >> 1]);
+  else return __uint_as_float(v[e]);
+}
+
+// Elements j .. of a row of V as one vector; past the row's end -inf.
+template <bool BF16, bool ALIGNED>
+__device__ __forceinline__ u32x4_t smp_load(const void* row, int j, int V) {
+  constexpr int EV = BF16 ? 8 : 4;
+  const uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
+  u32x4_t v = {none, none, none, none};
+  if (ALIGNED && j + EV <= V) return *(const u32x4_t*)((const char*)row + (int64_t)j * (BF16 ? 2 : 4));
+#pragma unroll
+  for (int e = 0; e < EV; ++e) {
+    if (j + e >= V) continue;
+    if constexpr (BF16) {
+      const uint32_t h = ((const uint16_t*)row)[j + e];
+      v[e >> 1] = (e & 1) ? (v[e >> 1] & 0xffffu) | h << 16 : (v[e >> 1] & 0xffff0000u) | h;
+    } else {
+      v[e] = ((const uint32_t*)row)[j + e];
+    }
+  }
+  return v;
 }
 
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
@@ -57,196 +88,329 @@ __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
   return v;
 }
 
-struct RowWeights {
-  float mx;
-  double inv_t, one;  // 1 / T, 2^shift
-  __device__ __forceinline__ uint64_t of(float x) const {
-    if (x == mx) return (uint64_t)one;
-    if (!(x > -INFINITY) || mx == INFINITY) return 0;
-    return (uint64_t)rint(exp(((double)x - (double)mx) * inv_t) * one);
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
   }
+  return v;
+}
+
+struct SampleShared {
+  uint64_t bins[SMP_BINS];
+  uint64_t weights[SMP_LIST];
+  float list[SMP_LIST];
+  double pow16[16];  // 2^(j/16)
+  uint64_t wave_sum[SMP_WAVES];
+  uint32_t wave_cnt[SMP_WAVES];
+  float wave_mx[SMP_WAVES], wave_mn[SMP_WAVES];
+  uint64_t above;
+  uint32_t n_list, bin;
+  float border;
+  uint32_t ties;
 };
 
-template <bool BF16>
+template <bool BF16, bool ALIGNED>
 __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(SampleParams p) {
-  __shared__ uint32_t cnt[256];
-  __shared__ uint64_t mass[256];
-  __shared__ uint64_t wave_mass[SMP_WAVES];
-  __shared__ uint32_t wave_cnt[SMP_WAVES];
-  __shared__ uint32_t s_key, s_left;
-  __shared__ uint64_t s_mass;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int V = p.vocab;
+  constexpr int EV = BF16 ? 8 : 4;
+  __shared__ SampleShared sh;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int V = p.vocab, layers = p.layers;
   const void* x = (const char*)p.logits + (int64_t)row * p.ld * (BF16 ? 2 : 4);
+  // this wave's run of the row: layer i holds elements first + (64 i + lane) EV ..; a whole number of
+  // layers covers it, so runs of the last waves may lie past its end (the sum stays below 2^25)
+  const int first = wave * layers * 64 * EV + lane * EV;
+  auto layer = [&](int i) __attribute__((always_inline)) {
+    return smp_load<BF16, ALIGNED>(x, first + 64 * EV * i, V);
+  };
+  // f(i, vector) over this lane's vectors, the next one on its way; f returns whether to go on (the
+  // same in all lanes)
+  auto each_vector = [&](auto f) __attribute__((always_inline)) {
+    u32x4_t v = layer(0);
+    for (int i = 0; i < layers; ++i) {
+      const u32x4_t next = layer(i + 1);
+      if (!f(i, v)) break;
+      v = next;
+    }
+  };
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    each_vector([&](int, const u32x4_t& v) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e) f(smp_elem<BF16>(v, e));
+      return true;
+    });
+  };
 
   float T = p.how.temperature ? p.how.temperature[row] : p.how.temperature_all;
-  int top_k = p.how.top_k ? p.how.top_k[row] : p.how.top_k_all;
+  const int top_k = p.how.top_k ? p.how.top_k[row] : p.how.top_k_all;
   const float top_p = p.how.top_p ? p.how.top_p[row] : p.how.top_p_all;
   const float min_p = p.how.min_p ? p.how.min_p[row] : p.how.min_p_all;
-  if (!(T > 0.0f)) {
-    T = 1.0f;
-    top_k = 1;
-  }
+  const float u = p.u[row];
+  const bool greedy = !(T > 0.0f) || top_k == 1;
+  if (tid < 16) sh.pow16[tid] = exp2(tid * 0.0625);
 
-  uint32_t mk = 0;
-  for (int i = tid; i < V; i += SMP_THREADS) mk = max(mk, key_of(logit_at<BF16>(x, i)));
+  // largest and smallest logit above -inf (NaN is neither)
+  float mx = -INFINITY, mn = INFINITY;
+  each([&](float v) __attribute__((always_inline)) {
+    mx = fmaxf(mx, v);
+    mn = fminf(mn, v > -INFINITY ? v : INFINITY);
+  });
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
-  if (lane == 0) wave_cnt[wave] = mk;
+  for (int o = 32; o > 0; o >>= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    mn = fminf(mn, __shfl_xor(mn, o, 64));
+  }
+  if (lane == 0) sh.wave_mx[wave] = mx, sh.wave_mn[wave] = mn;
   __syncthreads();
-  for (int w = 0; w < SMP_WAVES; ++w) mk = max(mk, wave_cnt[w]);
-  if (mk <= SMP_KEY_NEG_INF) {
+#pragma unroll
+  for (int w = 0; w < SMP_WAVES; ++w) {
+    mx = fmaxf(mx, sh.wave_mx[w]);
+    mn = fminf(mn, sh.wave_mn[w]);
+  }
+  if (mx == -INFINITY) {
     if (tid == 0) {
       p.tokens[row] = -1;
       if (p.probs) p.probs[row] = 0.0f;
     }
     return;
   }
-  const RowWeights W = {logit_of(mk), 1.0 / (double)T, (double)(uint64_t{1} << p.shift)};
 
-  // Kept so far: keys above `border`, and the first `ties` tokens that equal it.
-  uint32_t border = SMP_KEY_NEG_INF, ties = 0;
-
-  // Narrows the kept run to its first tokens, `want` of them (by_mass false), or as many as
-  // reach the weight `goal`.
-  auto narrow = [&](bool by_mass, uint32_t want, uint64_t goal) {
-    uint32_t prefix = 0, above = 0;  // digits found; tokens above them
-    uint64_t above_m = 0;
-    for (int sh = 24; sh >= 0; sh -= 8) {
-      __syncthreads();
-      if (tid < 256) cnt[tid] = 0, mass[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += SMP_THREADS) {
-        const float xi = logit_at<BF16>(x, i);
-        const uint32_t k = key_of(xi);
-        if (k <= border || (sh < 24 && (k ^ prefix) >> (sh + 8))) continue;
-        const int b = k >> sh & 255;
-        atomicAdd(&cnt[b], 1u);
-        if (by_mass) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)W.of(xi));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        // tokens that equal the old border stand in its bin, kept ones only
-        if (ties && (sh == 24 || !((border ^ prefix) >> (sh + 8)))) {
-          cnt[border >> sh & 255] += ties;
-          mass[border >> sh & 255] += ties * W.of(logit_of(border));
-        }
-        uint32_t c = above;
-        uint64_t m = above_m;
-        int b = 255;
-        for (; b > 0; --b) {
-          if (by_mass ? m + mass[b] >= goal : c + cnt[b] >= want) break;
-          c += cnt[b];
-          m += mass[b];
-        }
-        s_key = prefix | (uint32_t)b << sh;
-        s_left = c;
-        s_mass = m;
-      }
-      __syncthreads();
-      prefix = s_key;
-      above = s_left;
-      above_m = s_mass;
-    }
-    // all tokens above `prefix` are kept, and some that equal it
-    if (by_mass) {
-      const uint64_t w = W.of(logit_of(prefix));
-      uint64_t n = w ? (goal > above_m ? (goal - above_m + w - 1) / w : 0) : 0;
-      if (n > (uint64_t)V) n = V;
-      const uint32_t most = prefix == border ? ties : 0xffffffffu;
-      border = prefix;
-      ties = n < most ? (uint32_t)n : most;
-    } else {
-      const uint32_t n = want - above, most = prefix == border ? ties : 0xffffffffu;
-      border = prefix;
-      ties = n < most ? n : most;
-    }
+  // weights
+  const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)T;
+  const double one = (double)(uint64_t{1} << p.shift);
+  const double to_bits = 1.5 * (double)(uint64_t{1} << (52 - p.shift));  // w + this: w * 2^shift in the low bits
+  const double mxd = (double)mx;
+  auto weight_of = [&](float v) __attribute__((always_inline)) {  // as a 64-bit float
+    const double y = v == mx ? 0.0 : ((double)v - mxd) * c;
+    const double t = fma(y, 16.0, 6755399441055744.0);  // 1.5 * 2^52: 16 y, rounded, in the low bits
+    const int n = (int)(uint32_t)__double_as_longlong(t);
+    const double z = fma(t - 6755399441055744.0, -0.0625, y);  // |z| <= 1/32
+    // 2^z = sum (ln 2)^k / k! z^k, past k = 6 below 2^-51
+    double q = 1.5403530393381609e-04;
+    q = fma(q, z, 1.3333558146428443e-03);
+    q = fma(q, z, 9.6181291076284772e-03);
+    q = fma(q, z, 5.5504108664821580e-02);
+    q = fma(q, z, 2.4022650695910071e-01);
+    q = fma(q, z, 6.9314718055994531e-01);
+    q = fma(q, z, 1.0);
+    return y < -64.0 ? 0.0 : ldexp(q * sh.pow16[n & 15], n >> 4);
+  };
+  auto whole_of = [&](double w) __attribute__((always_inline)) {  // rounded to whole 2^-shift
+    return (uint64_t)(__double_as_longlong(w + to_bits) - __double_as_longlong(to_bits));
   };
 
-  // Weight of what is kept: this wave's share of the row, a run of whole 64s, in index order.
-  const int run = (V + SMP_WAVES * 64 - 1) / (SMP_WAVES * 64) * 64;
-  const int i0 = min(wave * run, V), i1 = min(i0 + run, V);
-  uint32_t floor_key = 0;  // min_p: keys below it are dropped
-  uint64_t total = 0, before = 0;
-  uint32_t ties_before = 0;
-  auto sum_kept = [&]() {
-    uint64_t m = 0;
-    uint32_t c = 0;
-    for (int i = i0 + lane; i < i1; i += 64) {
-      const float xi = logit_at<BF16>(x, i);
-      const uint32_t k = key_of(xi);
-      if (k > border && k >= floor_key) m += W.of(xi);
-      c += k == border;
+  // Kept: logits above `border`, and the first `ties` tokens that equal it.
+  float border = greedy ? mx : -INFINITY;
+  uint32_t ties = greedy ? 1 : 0;
+  if (mx == INFINITY && !greedy) border = 3.4028234663852886e38f;  // it takes all
+
+  // Bins, even in the distance from the maximum, over what weighs anything; halves of the values, whose
+  // difference cannot overflow.
+  const float reach = min((float)((0.5 * mxd - 0.5 * (double)mn) * c), 0.5f * (float)(p.shift + 2));
+  const float per =
+      c > 0.0 && reach > 0.0f ? (float)min((double)(SMP_BINS - 1) / (double)reach * c, 3e38) : 0.0f;
+  const float half_mx = 0.5f * mx;
+  auto bin_of = [&](float v) __attribute__((always_inline)) {
+    const float b = v == mx ? 0.0f : (half_mx - 0.5f * v) * per;
+    return (int)fminf(b, (float)SMP_BINS);  // SMP_BINS: weighs nothing
+  };
+
+  // Narrows what is kept to its first tokens: `want` of them, or (by weight) as many as reach the
+  // share `want` of all.  If there are not so many, all stay.
+  auto narrow = [&](auto by_weight, auto want) __attribute__((always_inline)) {
+    constexpr bool MASS = decltype(by_weight)::value;
+    sh.bins[tid] = 0;
+    if (tid == 0) sh.n_list = 0, sh.bin = SMP_BINS;
+    __syncthreads();
+    each([&](float v) __attribute__((always_inline)) {
+      if (v > border) {
+        const int b = bin_of(v);
+        if (b < SMP_BINS) {
+          if constexpr (MASS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)whole_of(weight_of(v)));
+          else atomicAdd((uint32_t*)&sh.bins[b], 1u);
+        }
+      }
+    });
+    __syncthreads();
+    // the bin in which the sum reaches the goal
+    const uint64_t mine = sh.bins[tid];
+    uint64_t sum = wave_scan_u64(mine), all = 0;
+    if (lane == 63) sh.wave_sum[wave] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SMP_WAVES; ++w) {
+      sum += w < wave ? sh.wave_sum[w] : 0;
+      all += sh.wave_sum[w];
     }
+    const uint64_t tie = MASS ? (ties ? whole_of(weight_of(border)) : 0) : 1;
+    uint64_t goal;
+    if constexpr (MASS) {
+      const double share = ceil((double)want * (double)(all + ties * tie));
+      goal = share >= 1.0 ? (uint64_t)share : 1;
+    } else {
+      goal = want;
+    }
+    if (sum >= goal && sum - mine < goal) sh.bin = tid, sh.above = sum - mine;
+    __syncthreads();
+    const int at = sh.bin;
+    const uint64_t above = sh.above;
+    if (at >= SMP_BINS) {
+      // among those that equal the old border, or nowhere
+      if (tie && ties) {
+        const uint64_t n = goal > all ? (goal - all + tie - 1) / tie : 0;
+        if (n < ties) ties = (uint32_t)n;
+      }
+      return;
+    }
+    each([&](float v) __attribute__((always_inline)) {
+      if (v > border && bin_of(v) == at) {
+        const uint32_t i = atomicAdd(&sh.n_list, 1u);
+        if (i < SMP_LIST) sh.list[i] = v;
+      }
+    });
+    __syncthreads();
+    const int n = (int)sh.n_list;
+    if (n <= SMP_LIST) {
+      if (MASS) {
+        if (tid < n) sh.weights[tid] = whole_of(weight_of(sh.list[tid]));
+        __syncthreads();
+      }
+      if (tid < n) {
+        const float v = sh.list[tid];
+        uint64_t more = above, same = 0;
+        for (int i = 0; i < n; ++i) {
+          const float o = sh.list[i];
+          const uint64_t w = MASS ? sh.weights[i] : 1;
+          more += o > v ? w : 0;
+          same += o == v ? w : 0;
+        }
+        if (more < goal && goal <= more + same) {
+          const uint64_t w = MASS ? sh.weights[tid] : 1;
+          sh.border = v;
+          sh.ties = (uint32_t)((goal - more + w - 1) / w);
+        }
+      }
+      __syncthreads();
+      border = sh.border;
+      ties = sh.ties;
+    } else {
+      // halve the values: the bin's tokens above `lo` reach the goal, those above `hi` do not
+      uint32_t lo = key_of(mn) - 1, hi = key_of(mx);
+      uint64_t over = 0;  // weight of the bin's tokens above `hi`
+      while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const float vm = logit_of(mid);
+        uint64_t s = 0;
+        each([&](float v) __attribute__((always_inline)) {
+          if (v > vm && v > border && bin_of(v) == at) s += MASS ? whole_of(weight_of(v)) : 1;
+        });
+        s = wave_sum_u64(s);
+        if (lane == 0) sh.wave_sum[wave] = s;
+        __syncthreads();
+        s = 0;
+#pragma unroll
+        for (int w = 0; w < SMP_WAVES; ++w) s += sh.wave_sum[w];
+        __syncthreads();
+        if (above + s >= goal) lo = mid;
+        else hi = mid, over = s;
+      }
+      const float v = logit_of(hi);
+      const uint64_t w = MASS ? whole_of(weight_of(v)) : 1;
+      border = v;
+      ties = (uint32_t)((goal - above - over + w - 1) / w);
+    }
+    __syncthreads();
+  };
+
+  // Weight of what is kept: of all, and of the waves before this one.
+  double low = 0.0;  // min_p: lighter tokens are dropped; the largest logit always stays
+  uint64_t total = 0, before = 0, tie_weight = 0;
+  uint32_t ties_before = 0;
+  auto sum_kept = [&]() __attribute__((always_inline)) {
+    uint64_t m = 0;
+    uint32_t n = 0;
+    each([&](float v) __attribute__((always_inline)) {
+      if (v > border) {
+        const double w = weight_of(v);
+        m += w >= low ? whole_of(w) : 0;
+      }
+      n += v == border;
+    });
     m = wave_sum_u64(m);
-    c = (uint32_t)wave_sum_u64(c);
+    n = (uint32_t)wave_sum_u64(n);
+    if (lane == 0) sh.wave_sum[wave] = m, sh.wave_cnt[wave] = n;
     __syncthreads();
-    if (lane == 0) wave_mass[wave] = m, wave_cnt[wave] = c;
-    __syncthreads();
-    const uint64_t wb = border >= floor_key ? W.of(logit_of(border)) : 0;
+    const double wb = ties ? weight_of(border) : 0.0;
+    tie_weight = wb >= low ? whole_of(wb) : 0;
     uint32_t seen = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < SMP_WAVES; ++w) {
       if (w == wave) before = total, ties_before = seen;
       const uint32_t left = ties > seen ? ties - seen : 0;
-      total += wave_mass[w] + wb * min(left, wave_cnt[w]);
-      seen += wave_cnt[w];
+      total += sh.wave_sum[w] + tie_weight * min(left, sh.wave_cnt[w]);
+      seen += sh.wave_cnt[w];
     }
   };
 
-  if (top_k > 0 && top_k < V) narrow(false, (uint32_t)top_k, 0);
-  if (top_p < 1.0f) {
-    sum_kept();
-    const double goal = ceil((double)top_p * (double)total);
-    narrow(true, 0, goal >= 1.0 ? (uint64_t)goal : 1);
-  }
-  if (min_p > 0.0f) {
-    // the lowest key whose weight reaches min_p; the largest logit always stays
-    const double low = (double)min_p * W.one;
-    uint32_t lo = SMP_KEY_NEG_INF, hi = mk;  // below(lo), not below(hi)
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      const float xm = logit_of(mid);
-      const double w = xm == W.mx ? W.one : exp(((double)xm - (double)W.mx) * W.inv_t) * W.one;
-      if (w >= low) hi = mid;
-      else lo = mid;
-    }
-    floor_key = hi;
+  if (!greedy) {
+    if (top_k > 0 && top_k < V) narrow(std::false_type{}, (uint64_t)top_k);
+    if (top_p < 1.0f) narrow(std::true_type{}, top_p);
+    if (min_p > 0.0f) low = min((double)min_p, 1.0);
   }
   sum_kept();
 
   // the token at which the kept weight passes u * total
-  const double t = (double)p.u[row] * (double)total;
+  const double t = (double)u * (double)total;
   uint64_t target = t > 0.0 ? (uint64_t)t : 0;
   if (target >= total) target = total - 1;
-  const uint64_t wb = border >= floor_key ? W.of(logit_of(border)) : 0;
   uint64_t acc = before;
   uint32_t seen = ties_before;
-  for (int j0 = i0; j0 < i1; j0 += 64) {
-    const int i = j0 + lane;
-    const float xi = i < i1 ? logit_at<BF16>(x, i) : -INFINITY;
-    const uint32_t k = i < i1 ? key_of(xi) : 0;
-    const bool tie = i < i1 && k == border;
-    const uint64_t tb = __ballot(tie);
-    const uint32_t rank = seen + (uint32_t)__popcll(tb & ((uint64_t{1} << lane) - 1));
-    uint64_t w = k > border && k >= floor_key ? W.of(xi) : tie && rank < ties ? wb : 0;
-    const uint64_t own_w = w;
+  each_vector([&](int i, const u32x4_t& vec) __attribute__((always_inline)) {
+    // ties of the lanes before this one
+    uint32_t n = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t y = __shfl_up(w, o, 64);
-      if (lane >= o) w += y;
+    for (int e = 0; e < EV; ++e) n += smp_elem<BF16>(vec, e) == border;
+    uint32_t rank = seen, all_ties = 0;
+    if (__any(n)) {
+      const uint32_t upto = (uint32_t)wave_scan_u64(n);
+      rank += upto - n;
+      all_ties = (uint32_t)__shfl((int)upto, 63, 64);
     }
-    const uint64_t hit = __ballot(acc + w > target && acc + w - own_w <= target);
-    if (hit) {
-      if (lane == (int)__ffsll((unsigned long long)hit) - 1) {
-        p.tokens[row] = i;
-        if (p.probs) p.probs[row] = (float)((double)own_w / (double)total);
+    uint64_t m = 0, w[EV];
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      const float v = smp_elem<BF16>(vec, e);
+      w[e] = 0;
+      if (v > border) {
+        const double d = weight_of(v);
+        w[e] = d >= low ? whole_of(d) : 0;
+      } else if (v == border) {
+        w[e] = rank < ties ? tie_weight : 0;
+        ++rank;
       }
-      break;
+      m += w[e];
     }
-    acc += __shfl(w, 63, 64);
-    seen += (uint32_t)__popcll(tb);
-  }
+    const uint64_t upto = acc + wave_scan_u64(m), from = upto - m;
+    if (from <= target && target < upto) {
+      uint64_t s = from;
+      bool open = true;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        s += w[e];
+        if (open && s > target) {
+          open = false;
+          p.tokens[row] = first + 64 * EV * i + e;
+          if (p.probs) p.probs[row] = (float)((double)w[e] / (double)total);
+        }
+      }
+    }
+    acc = __shfl(upto, 63, 64);
+    seen += all_ties;
+    return acc <= target;
+  });
 }
 
 }  // namespace
@@ -278,13 +442,18 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
   p.vocab = (int)vocab;
   int bits = 0;
   while ((int64_t{1} << bits) < vocab) ++bits;
-  p.shift = 62 - bits < 52 ? 62 - bits : 52;
+  p.shift = 62 - bits < 50 ? 62 - bits : 50;
   p.u = u;
   p.tokens = tokens;
   p.probs = probs;
   p.how = *how;
-  if (dtype == MI_BF16) sample_kernel<true><<<(unsigned)rows, SMP_THREADS, 0, (hipStream_t)stream>>>(p);
-  else sample_kernel<false><<<(unsigned)rows, SMP_THREADS, 0, (hipStream_t)stream>>>(p);
+  const bool bf16 = dtype == MI_BF16;
+  const int per_layer = SMP_THREADS * (bf16 ? 8 : 4);
+  p.layers = (int)((vocab + per_layer - 1) / per_layer);
+  const bool aligned = ((uintptr_t)logits & 15) == 0 && (rows == 1 || ld % (bf16 ? 8 : 4) == 0);
+  const auto kernel = bf16 ? (aligned ? sample_kernel<true, true> : sample_kernel<true, false>)
+                           : (aligned ? sample_kernel<false, true> : sample_kernel<false, false>);
+  kernel<<<(unsigned)rows, SMP_THREADS, 0, (hipStream_t)stream>>>(p);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MI_OK : host_fail(MI_ERR_HIP, "sample launch: %s", hipGetErrorString(e));
 }

@@ -1,5 +1,6 @@
 """Sampling (mi_sample) against the definition in 64 bits: tokens are equal, without tolerance. The
-definition counts weights in whole multiples of 2^-(62 - b), b the bits of V - 1, and so does the oracle.
+definition counts weights in whole multiples of 2^-(62 - b) (2^-50 at
+most), b the bits of V - 1, and so does the oracle.
 
 The picked token's share is a quotient of two sums of 64-bit weights, rounded once to fp32: 2^-24 of
 its value, with 2^-40 for the weights' own rounding.
@@ -25,7 +26,7 @@ def reference(x, u, T, k, p, low):
     y = x[order[:n]]
     with np.errstate(invalid="ignore"):
         w = np.where(y == top, 1.0, np.where(y == -np.inf, 0.0, np.exp((y - top) / T)))
-    unit = 2.0 ** min(52, 62 - int(x.size - 1).bit_length())
+    unit = 2.0 ** min(50, 62 - int(x.size - 1).bit_length())
     exact, w = w, np.rint(w * unit)
     if p < 1:
         mass = np.cumsum(w)
