@@ -6,7 +6,8 @@
 //   1. a histogram over the distance from the row's maximum, SMP_BINS bins evenly over the distances
 //      that can weigh anything, counts tokens (top-k) or sums weights (top-p);
 //   2. a scan over the bins finds the one in which the border lies;
-//   3. that bin's tokens (1/1000 of the row) go to LDS, where each finds its rank among them.
+//   3. that bin's tokens (1/1000 of the row) go to LDS, where each finds its rank among them; where a
+//      top-k keeps few, they all go there, and the row is not read again.
 // A bin that holds more than SMP_LIST of them (a row of few distinct logits) is halved by its logits'
 // bits instead, over the row, until one value is left.
 //
@@ -14,8 +15,10 @@
 // so every sum is exact: it is the same whatever order atomics and waves add in, and a border is never
 // moved by rounding.  A weight below half of 2^-shift counts as nothing: u = 0, one of 2^24 numbers,
 // then does not draw a token whose chance is 1e-20.  64 bits cost no more than 32 here (a 64-lane
-// instruction takes four cycles either way); 2^y is a table of 16 steps in LDS, a polynomial of degree 6
-// on what is left, and an addition that leaves the rounded integer in the low bits.
+// instruction takes four cycles either way); 2^y is a table of 32 steps in LDS, a polynomial of degree 5
+// on what is left, and an addition that leaves the rounded integer in the low bits.  Tokens that a
+// border has left are gathered 64 at a time before they are weighed: of a nucleus of 5 % of the
+// vocabulary nearly every 64 tokens hold one, and weighing costs more than the rest of a pass.
 //
 // One workgroup a row, each wave a run of it.  A pass reads the row again, from the caches: held in
 // registers it would need every pass unrolled over them, more code than the instruction cache holds.
@@ -35,6 +38,8 @@ constexpr int SMP_THREADS = 1024;
 constexpr int SMP_WAVES = SMP_THREADS / 64;
 constexpr int SMP_BINS = 1024;        // one for each thread in the scan
 constexpr int SMP_LIST = 1024;        // tokens of a bin that are ranked in LDS
+constexpr int SMP_FEW = 256;          // tokens that are handled in LDS altogether
+constexpr int SMP_GATHER = 4;         // logits that a lane weighs at a time: its waits for each overlap
 
 struct SampleParams {
   const void* logits;
@@ -102,11 +107,13 @@ struct SampleShared {
   uint64_t bins[SMP_BINS];
   uint64_t weights[SMP_LIST];
   float list[SMP_LIST];
-  double pow16[16];  // 2^(j/16)
+  int index[SMP_LIST];
+  double pow32[32];  // 2^(j/32)
+  float pending[SMP_WAVES][64 * (SMP_GATHER + 8)];
   uint64_t wave_sum[SMP_WAVES];
   uint32_t wave_cnt[SMP_WAVES];
   float wave_mx[SMP_WAVES], wave_mn[SMP_WAVES];
-  uint64_t above;
+  uint64_t above, upto;
   uint32_t n_list, bin;
   float border;
   uint32_t ties;
@@ -149,7 +156,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(SampleParams p) {
   const float min_p = p.how.min_p ? p.how.min_p[row] : p.how.min_p_all;
   const float u = p.u[row];
   const bool greedy = !(T > 0.0f) || top_k == 1;
-  if (tid < 16) sh.pow16[tid] = exp2(tid * 0.0625);
+  if (tid < 32) sh.pow32[tid] = exp2(tid * 0.03125);
 
   // largest and smallest logit above -inf (NaN is neither)
   float mx = -INFINITY, mn = INFINITY;
@@ -177,34 +184,89 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(SampleParams p) {
     return;
   }
 
-  // weights
+  // weights of logits up to a finite maximum
   const double c = greedy ? 0.0 : 1.4426950408889634074 / (double)T;
-  const double one = (double)(uint64_t{1} << p.shift);
+  const double c32 = 32.0 * c, mxd = (double)mx;
   const double to_bits = 1.5 * (double)(uint64_t{1} << (52 - p.shift));  // w + this: w * 2^shift in the low bits
-  const double mxd = (double)mx;
   auto weight_of = [&](float v) __attribute__((always_inline)) {  // as a 64-bit float
-    const double y = v == mx ? 0.0 : ((double)v - mxd) * c;
-    const double t = fma(y, 16.0, 6755399441055744.0);  // 1.5 * 2^52: 16 y, rounded, in the low bits
+    const double y = max(((double)v - mxd) * c32, -2048.0);  // 32 y; 2^-64 rounds to nothing
+    const double t = y + 6755399441055744.0;                 // 1.5 * 2^52: rounded, in the low bits
     const int n = (int)(uint32_t)__double_as_longlong(t);
-    const double z = fma(t - 6755399441055744.0, -0.0625, y);  // |z| <= 1/32
-    // 2^z = sum (ln 2)^k / k! z^k, past k = 6 below 2^-51
-    double q = 1.5403530393381609e-04;
-    q = fma(q, z, 1.3333558146428443e-03);
-    q = fma(q, z, 9.6181291076284772e-03);
-    q = fma(q, z, 5.5504108664821580e-02);
-    q = fma(q, z, 2.4022650695910071e-01);
-    q = fma(q, z, 6.9314718055994531e-01);
+    const double z = y - (t - 6755399441055744.0);           // |z| <= 1/2, of 1/32
+    // 2^(z/32) = sum (z ln 2 / 32)^k / k!, past k = 5 below 2^-48
+    double q = 3.9737099845494154e-11;
+    q = fma(q, z, 9.172562701824643e-09);
+    q = fma(q, z, 1.6938509724371819e-06);
+    q = fma(q, z, 2.3459619820224677e-04);
+    q = fma(q, z, 2.1660849392498290e-02);
     q = fma(q, z, 1.0);
-    return y < -64.0 ? 0.0 : ldexp(q * sh.pow16[n & 15], n >> 4);
+    q *= sh.pow32[n & 31];
+    return __hiloint2double(__double2hiint(q) + ((n >> 5) << 20), __double2loint(q));
   };
   auto whole_of = [&](double w) __attribute__((always_inline)) {  // rounded to whole 2^-shift
     return (uint64_t)(__double_as_longlong(w + to_bits) - __double_as_longlong(to_bits));
   };
 
-  // Kept: logits above `border`, and the first `ties` tokens that equal it.
+  // Kept: logits above `border`, and the first `ties` tokens that equal it, which weigh `tie` each.
   float border = greedy ? mx : -INFINITY;
   uint32_t ties = greedy ? 1 : 0;
-  if (mx == INFINITY && !greedy) border = 3.4028234663852886e38f;  // it takes all
+  double tie_w = greedy ? 1.0 : 0.0;
+  if (mx == INFINITY && !greedy) {
+    // it takes all: every +inf is a tie
+    border = mx;
+    tie_w = 1.0;
+    uint32_t n = 0;
+    each([&](float v) __attribute__((always_inline)) { n += v == mx; });
+    n = (uint32_t)wave_sum_u64(n);
+    if (lane == 0) sh.wave_cnt[wave] = n;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SMP_WAVES; ++w) ties += sh.wave_cnt[w];
+    __syncthreads();
+  }
+
+  // f(logit, is one) with the logits above the border for which take(logit, index) holds, in no order:
+  // as they stand where most are, else gathered
+  auto each_kept = [&](auto take, auto f) __attribute__((always_inline)) {
+    float* pend = &sh.pending[wave][0];
+    int n = 0;
+    each_vector([&](int i, const u32x4_t& vec) __attribute__((always_inline)) {
+      uint64_t mask[EV];
+      int more = 0;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const float v = smp_elem<BF16>(vec, e);
+        mask[e] = __ballot(v > border && take(v, first + 64 * EV * i + e));
+        more += (int)__popcll(mask[e]);
+      }
+      if (more > 32 * EV) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) f(smp_elem<BF16>(vec, e), (mask[e] >> lane) & 1);
+        return true;
+      }
+      if (more == 0) return true;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const int at = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask[e] >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo((uint32_t)mask[e], 0));
+        if ((mask[e] >> lane) & 1) pend[at] = smp_elem<BF16>(vec, e);
+        n += (int)__popcll(mask[e]);
+      }
+      asm volatile("" ::: "memory");  // a wave's LDS accesses are in order
+      while (n >= 64 * SMP_GATHER) {
+        n -= 64 * SMP_GATHER;
+        float v[SMP_GATHER];
+#pragma unroll
+        for (int k = 0; k < SMP_GATHER; ++k) v[k] = pend[n + 64 * k + lane];
+#pragma unroll
+        for (int k = 0; k < SMP_GATHER; ++k) f(v[k], true);
+      }
+      asm volatile("" ::: "memory");
+      return true;
+    });
+    for (; n > 0; n -= 64) f(pend[max(n - 64 + lane, 0)], n - 64 + lane >= 0);
+  };
+  auto all = [](float, int) { return true; };
 
   // Bins, even in the distance from the maximum, over what weighs anything; halves of the values, whose
   // difference cannot overflow.
@@ -213,159 +275,292 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(SampleParams p) {
       c > 0.0 && reach > 0.0f ? (float)min((double)(SMP_BINS - 1) / (double)reach * c, 3e38) : 0.0f;
   const float half_mx = 0.5f * mx;
   auto bin_of = [&](float v) __attribute__((always_inline)) {
-    const float b = v == mx ? 0.0f : (half_mx - 0.5f * v) * per;
-    return (int)fminf(b, (float)SMP_BINS);  // SMP_BINS: weighs nothing
+    return (int)fminf(fmaf(-0.5f, v, half_mx) * per, (float)SMP_BINS);  // SMP_BINS: weighs nothing
   };
 
-  // Narrows what is kept to its first tokens: `want` of them, or (by weight) as many as reach the
-  // share `want` of all.  If there are not so many, all stay.
-  auto narrow = [&](auto by_weight, auto want) __attribute__((always_inline)) {
-    constexpr bool MASS = decltype(by_weight)::value;
-    sh.bins[tid] = 0;
-    if (tid == 0) sh.n_list = 0, sh.bin = SMP_BINS;
-    __syncthreads();
-    each([&](float v) __attribute__((always_inline)) {
-      if (v > border) {
-        const int b = bin_of(v);
-        if (b < SMP_BINS) {
-          if constexpr (MASS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)whole_of(weight_of(v)));
-          else atomicAdd((uint32_t*)&sh.bins[b], 1u);
-        }
-      }
-    });
-    __syncthreads();
-    // the bin in which the sum reaches the goal
+  double low = 0.0;  // min_p: lighter tokens are dropped; the largest logit always stays
+  if (!greedy && min_p > 0.0f) low = min((double)min_p, 1.0);
+  // weight of what is kept: of all, of the waves before this one, and of this one
+  uint64_t total = 0, before = 0, own = 0, tie_weight = 0;
+  uint32_t ties_before = 0;
+  bool summed = false;  // sh.wave_sum and sh.wave_cnt hold the waves' sums above the border, and their ties
+
+  // The bin in which the sum of the bins reaches the goal, into sh.bin, what lies above it and up to its
+  // end; goal: of the sum of all.
+  auto scan_bins = [&](auto goal_of) __attribute__((always_inline)) {
     const uint64_t mine = sh.bins[tid];
-    uint64_t sum = wave_scan_u64(mine), all = 0;
+    uint64_t sum = wave_scan_u64(mine), sum_all = 0;
     if (lane == 63) sh.wave_sum[wave] = sum;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < SMP_WAVES; ++w) {
       sum += w < wave ? sh.wave_sum[w] : 0;
-      all += sh.wave_sum[w];
+      sum_all += sh.wave_sum[w];
     }
-    const uint64_t tie = MASS ? (ties ? whole_of(weight_of(border)) : 0) : 1;
-    uint64_t goal;
-    if constexpr (MASS) {
-      const double share = ceil((double)want * (double)(all + ties * tie));
-      goal = share >= 1.0 ? (uint64_t)share : 1;
-    } else {
-      goal = want;
-    }
-    if (sum >= goal && sum - mine < goal) sh.bin = tid, sh.above = sum - mine;
+    const uint64_t goal = goal_of(sum_all);
+    if (sum >= goal && sum - mine < goal) sh.bin = tid, sh.above = sum - mine, sh.upto = sum;
     __syncthreads();
-    const int at = sh.bin;
-    const uint64_t above = sh.above;
-    if (at >= SMP_BINS) {
-      // among those that equal the old border, or nowhere
-      if (tie && ties) {
-        const uint64_t n = goal > all ? (goal - all + tie - 1) / tie : 0;
-        if (n < ties) ties = (uint32_t)n;
-      }
-      return;
-    }
-    each([&](float v) __attribute__((always_inline)) {
-      if (v > border && bin_of(v) == at) {
-        const uint32_t i = atomicAdd(&sh.n_list, 1u);
-        if (i < SMP_LIST) sh.list[i] = v;
-      }
-    });
-    __syncthreads();
-    const int n = (int)sh.n_list;
-    if (n <= SMP_LIST) {
-      if (MASS) {
-        if (tid < n) sh.weights[tid] = whole_of(weight_of(sh.list[tid]));
-        __syncthreads();
-      }
-      if (tid < n) {
-        const float v = sh.list[tid];
-        uint64_t more = above, same = 0;
-        for (int i = 0; i < n; ++i) {
-          const float o = sh.list[i];
-          const uint64_t w = MASS ? sh.weights[i] : 1;
-          more += o > v ? w : 0;
-          same += o == v ? w : 0;
-        }
-        if (more < goal && goal <= more + same) {
-          const uint64_t w = MASS ? sh.weights[tid] : 1;
-          sh.border = v;
-          sh.ties = (uint32_t)((goal - more + w - 1) / w);
-        }
-      }
+    return goal;
+  };
+  // Where no bin has it: the goal lies among those that equal the old border, or nowhere.
+  auto cut_ties = [&](uint64_t sum_all, uint64_t goal, uint64_t tie) __attribute__((always_inline)) {
+    if (!tie || !ties) return;
+    const uint64_t n = goal > sum_all ? (goal - sum_all + tie - 1) / tie : 0;
+    if (n < ties) ties = (uint32_t)n;
+  };
+  // The border among the n tokens of the list, above which `above` lies.
+  auto rank_list = [&](int n, uint64_t above, uint64_t goal, auto by_weight) __attribute__((always_inline)) {
+    constexpr bool MASS = decltype(by_weight)::value;
+    if (MASS) {
+      if (tid < n) sh.weights[tid] = whole_of(weight_of(sh.list[tid]));
       __syncthreads();
-      border = sh.border;
-      ties = sh.ties;
-    } else {
-      // halve the values: the bin's tokens above `lo` reach the goal, those above `hi` do not
-      uint32_t lo = key_of(mn) - 1, hi = key_of(mx);
-      uint64_t over = 0;  // weight of the bin's tokens above `hi`
-      while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const float vm = logit_of(mid);
-        uint64_t s = 0;
-        each([&](float v) __attribute__((always_inline)) {
-          if (v > vm && v > border && bin_of(v) == at) s += MASS ? whole_of(weight_of(v)) : 1;
-        });
-        s = wave_sum_u64(s);
-        if (lane == 0) sh.wave_sum[wave] = s;
-        __syncthreads();
-        s = 0;
-#pragma unroll
-        for (int w = 0; w < SMP_WAVES; ++w) s += sh.wave_sum[w];
-        __syncthreads();
-        if (above + s >= goal) lo = mid;
-        else hi = mid, over = s;
-      }
-      const float v = logit_of(hi);
-      const uint64_t w = MASS ? whole_of(weight_of(v)) : 1;
-      border = v;
-      ties = (uint32_t)((goal - above - over + w - 1) / w);
     }
+    if (tid < n) {
+      const float v = sh.list[tid];
+      uint64_t more = above, same = 0;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float o = sh.list[i];
+        const uint64_t w = MASS ? sh.weights[i] : 1;
+        more += o > v ? w : 0;
+        same += o == v ? w : 0;
+      }
+      if (more < goal && goal <= more + same) {
+        const uint64_t w = MASS ? sh.weights[tid] : 1;
+        sh.border = v;
+        sh.ties = (uint32_t)((goal - more + w - 1) / w);
+      }
+    }
+    __syncthreads();
+    border = sh.border;
+    ties = sh.ties;
+    tie_w = weight_of(border);
+  };
+  // The same for a bin of more tokens, by halving the values: those above `lo` reach the goal, those
+  // above `hi` do not.
+  auto halve = [&](int at, uint64_t above, uint64_t goal, auto by_weight) __attribute__((always_inline)) {
+    constexpr bool MASS = decltype(by_weight)::value;
+    uint32_t lo = key_of(mn) - 1, hi = key_of(mx);
+    uint64_t over = 0;  // weight of the bin's tokens above `hi`
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const float vm = logit_of(mid);
+      uint64_t s = 0;
+      each([&](float v) __attribute__((always_inline)) {
+        if (v > vm && v > border && bin_of(v) == at) s += MASS ? whole_of(weight_of(v)) : 1;
+      });
+      s = wave_sum_u64(s);
+      __syncthreads();
+      if (lane == 0) sh.wave_sum[wave] = s;
+      __syncthreads();
+      s = 0;
+#pragma unroll
+      for (int w = 0; w < SMP_WAVES; ++w) s += sh.wave_sum[w];
+      if (above + s >= goal) lo = mid;
+      else hi = mid, over = s;
+    }
+    const float v = logit_of(hi);
+    const uint64_t w = MASS ? whole_of(weight_of(v)) : 1;
+    border = v;
+    tie_w = weight_of(v);
+    ties = (uint32_t)((goal - above - over + w - 1) / w);
+  };
+  auto clear = [&]() __attribute__((always_inline)) {
+    sh.bins[tid] = 0;
+    if (tid < SMP_WAVES) sh.wave_cnt[tid] = 0;
+    if (tid == 0) sh.n_list = 0, sh.bin = SMP_BINS;
     __syncthreads();
   };
 
-  // Weight of what is kept: of all, and of the waves before this one.
-  double low = 0.0;  // min_p: lighter tokens are dropped; the largest logit always stays
-  uint64_t total = 0, before = 0, tie_weight = 0;
-  uint32_t ties_before = 0;
-  auto sum_kept = [&]() __attribute__((always_inline)) {
+  if (!greedy && top_k > 0 && top_k < V) {
+    clear();
+    each([&](float v) __attribute__((always_inline)) {
+      const int b = bin_of(v);
+      if (v > border && b < SMP_BINS) atomicAdd((uint32_t*)&sh.bins[b], 1u);
+    });
+    __syncthreads();
+    uint64_t sum_all = 0;
+    const uint64_t goal = scan_bins([&](uint64_t t) { sum_all = t; return (uint64_t)top_k; });
+    const int at = sh.bin;
+    if (at >= SMP_BINS) {
+      cut_ties(sum_all, goal, 1);
+    } else {
+      const uint64_t above = sh.above, upto = sh.upto;
+      const int from = upto <= SMP_FEW ? 0 : at;  // few: all that may be kept
+      each_vector([&](int i, const u32x4_t& vec) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          const float v = smp_elem<BF16>(vec, e);
+          const int b = bin_of(v);
+          if (v > border && b >= from && b <= at) {
+            const uint32_t k = atomicAdd(&sh.n_list, 1u);
+            if (k < SMP_LIST) sh.list[k] = v, sh.index[k] = first + 64 * EV * i + e;
+          }
+        }
+        return true;
+      });
+      __syncthreads();
+      const int n = (int)sh.n_list;
+      if (from == 0 && n <= SMP_FEW) {
+        // in order of rank, in the bins: weights and, behind them, indexes
+        uint64_t* w_at = sh.bins;
+        int* i_at = (int*)(sh.bins + SMP_FEW);
+        if (tid < n) {
+          const float v = sh.list[tid];
+          const int idx = sh.index[tid];
+          int r = 0;
+#pragma unroll 8
+          for (int i = 0; i < n; ++i) r += sh.list[i] > v || (sh.list[i] == v && sh.index[i] < idx);
+          const double w = weight_of(v);
+          w_at[r] = whole_of(w);
+          i_at[r] = idx;
+          sh.pending[0][r] = w >= low ? 1.0f : 0.0f;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        // one wave, rank 64 j + lane
+        constexpr int J = SMP_FEW / 64;
+        const int m = min(n, top_k);
+        uint64_t w[J], lies[J], sum_k = 0;  // weight, and what lies before it in order of rank
+        int idx[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          w[j] = 0;
+          if (64 * j >= m) continue;
+          const int r = min(64 * j + lane, m - 1);
+          idx[j] = i_at[r];
+          w[j] = 64 * j + lane < m ? w_at[r] : 0;
+          const uint64_t to = wave_scan_u64(w[j]);
+          lies[j] = sum_k + to - w[j];
+          sum_k += __shfl(to, 63, 64);
+        }
+        uint64_t goal_p = sum_k;
+        if (top_p < 1.0f) {
+          const double share = ceil((double)top_p * (double)sum_k);
+          goal_p = share >= 1.0 ? (uint64_t)share : 1;
+        }
+        uint64_t kept = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (64 * j >= m) continue;
+          const int r = min(64 * j + lane, m - 1);
+          if (!(lies[j] < goal_p && sh.pending[0][r] != 0.0f)) w[j] = 0;
+          kept += w[j];
+          if (64 * j + lane < m) w_at[r] = w[j];
+        }
+        total = wave_sum_u64(kept);
+        const double t = (double)u * (double)total;
+        uint64_t target = t > 0.0 ? (uint64_t)t : 0;
+        if (target >= total) target = total - 1;
+        asm volatile("" ::: "memory");  // a wave's LDS accesses are in order
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (64 * j >= m) continue;
+          uint64_t ahead = 0;  // what lies before it in order of index
+#pragma unroll 8
+          for (int i = 0; i < m; ++i) ahead += i_at[i] < idx[j] ? w_at[i] : 0;
+          if (w[j] && ahead <= target && target < ahead + w[j]) {
+            p.tokens[row] = idx[j];
+            if (p.probs) p.probs[row] = (float)((double)w[j] / (double)total);
+          }
+        }
+        return;
+      }
+      if (n > SMP_LIST) halve(at, above, goal, std::false_type{});
+      else rank_list(n, above, goal, std::false_type{});
+    }
+    __syncthreads();
+  }
+  if (!greedy && top_p < 1.0f) {
+    clear();
+    each_kept(all, [&](float v, bool is) __attribute__((always_inline)) {
+      const int b = bin_of(v);
+      const uint64_t w = whole_of(weight_of(v));
+      if (is && b < SMP_BINS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)w);
+    });
+    __syncthreads();
+    const uint64_t tie = ties ? whole_of(tie_w) : 0;
+    uint64_t sum_all = 0;
+    const uint64_t goal = scan_bins([&](uint64_t t) {
+      sum_all = t;
+      const double share = ceil((double)top_p * (double)(t + ties * tie));
+      return share >= 1.0 ? (uint64_t)share : (uint64_t)1;
+    });
+    const int at = sh.bin;
+    const uint64_t above = sh.above;
+    if (at >= SMP_BINS) {
+      cut_ties(sum_all, goal, tie);
+    } else {
+      // the border's bin goes to the list; what lies above it is kept, and summed on the way
+      uint64_t m = 0;
+      each_kept(
+          [&](float v, int idx) __attribute__((always_inline)) {
+            const int b = bin_of(v);
+            if (b == at) {
+              const uint32_t k = atomicAdd(&sh.n_list, 1u);
+              if (k < SMP_LIST) sh.list[k] = v, sh.index[k] = idx;
+            }
+            return b < at;
+          },
+          [&](float v, bool is) __attribute__((always_inline)) {
+            const double w = weight_of(v);
+            const uint64_t whole = whole_of(w);
+            m += is && w >= low ? whole : 0;
+          });
+      m = wave_sum_u64(m);
+      __syncthreads();
+      const int n = (int)sh.n_list;
+      if (n <= SMP_LIST) {
+        rank_list(n, above, goal, std::true_type{});
+        if (lane == 0) sh.wave_sum[wave] = m;
+        __syncthreads();
+        if (tid < n) {
+          const float v = sh.list[tid];
+          const int w = sh.index[tid] / (layers * 64 * EV);
+          if (v > border && weight_of(v) >= low)
+            atomicAdd((unsigned long long*)&sh.wave_sum[w], (unsigned long long)sh.weights[tid]);
+          if (v == border) atomicAdd(&sh.wave_cnt[w], 1u);
+        }
+        summed = true;
+      } else {
+        halve(at, above, goal, std::true_type{});
+      }
+    }
+    __syncthreads();
+  }
+  if (!summed) {
     uint64_t m = 0;
     uint32_t n = 0;
-    each([&](float v) __attribute__((always_inline)) {
-      if (v > border) {
-        const double w = weight_of(v);
-        m += w >= low ? whole_of(w) : 0;
-      }
-      n += v == border;
+    each_kept(all, [&](float v, bool is) __attribute__((always_inline)) {
+      const double w = weight_of(v);
+      const uint64_t whole = whole_of(w);
+      m += is && w >= low ? whole : 0;
     });
+    if (ties) each([&](float v) __attribute__((always_inline)) { n += v == border; });
     m = wave_sum_u64(m);
     n = (uint32_t)wave_sum_u64(n);
     if (lane == 0) sh.wave_sum[wave] = m, sh.wave_cnt[wave] = n;
     __syncthreads();
-    const double wb = ties ? weight_of(border) : 0.0;
-    tie_weight = wb >= low ? whole_of(wb) : 0;
+  }
+  tie_weight = ties && tie_w >= low ? whole_of(tie_w) : 0;
+  {
     uint32_t seen = 0;
-    total = 0;
 #pragma unroll
     for (int w = 0; w < SMP_WAVES; ++w) {
       if (w == wave) before = total, ties_before = seen;
       const uint32_t left = ties > seen ? ties - seen : 0;
-      total += sh.wave_sum[w] + tie_weight * min(left, sh.wave_cnt[w]);
+      const uint64_t of_wave = sh.wave_sum[w] + tie_weight * min(left, sh.wave_cnt[w]);
+      if (w == wave) own = of_wave;
+      total += of_wave;
       seen += sh.wave_cnt[w];
     }
-  };
-
-  if (!greedy) {
-    if (top_k > 0 && top_k < V) narrow(std::false_type{}, (uint64_t)top_k);
-    if (top_p < 1.0f) narrow(std::true_type{}, top_p);
-    if (min_p > 0.0f) low = min((double)min_p, 1.0);
   }
-  sum_kept();
 
   // the token at which the kept weight passes u * total
   const double t = (double)u * (double)total;
   uint64_t target = t > 0.0 ? (uint64_t)t : 0;
   if (target >= total) target = total - 1;
+  if (target < before || target - before >= own) return;
   uint64_t acc = before;
   uint32_t seen = ties_before;
   each_vector([&](int i, const u32x4_t& vec) __attribute__((always_inline)) {
