@@ -433,8 +433,8 @@ typedef struct mi_paged_cache {
  * tokens of its kv_len[s], so the first of them is at position kv_len[s] - (q_start[s+1] -
  * q_start[s]).  Position p lies in page pages[s*pages_ld + p / page_size], slot p % page_size.
  * Sequences may have no new token, and rows behind the last sequence are left as they are.
- * Positions below zero or past max_pages pages, and pages outside [0, num_pages), hold
- * nothing: they are not written, and their keys are not seen.
+ * Positions below zero or past max_pages pages (at most 2^31 - 4096 tokens), and pages outside
+ * [0, num_pages), hold nothing: they are not written, and their keys are not seen.
  */
 typedef struct mi_paged_seqs {
   int64_t n_seqs, total_q;

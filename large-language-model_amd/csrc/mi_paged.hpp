@@ -70,6 +70,9 @@ inline int check_paged(const mi_paged_cache* c, const mi_paged_seqs* s) {
   if (!s->q_start && s->total_q != s->n_seqs)
     return host_fail(MI_ERR_SHAPE, "total_q=%lld for %lld sequences without q_start", (long long)s->total_q,
                      (long long)s->n_seqs);
+  if (s->max_pages * c->page_size > INT32_MAX - 4096)
+    return host_fail(MI_ERR_SHAPE, "max_pages * page_size = %lld exceeds 2^31 - 4096",
+                     (long long)(s->max_pages * c->page_size));
   if (s->pages_ld < s->max_pages)
     return host_fail(MI_ERR_LD, "pages_ld=%lld < max_pages=%lld", (long long)s->pages_ld, (long long)s->max_pages);
   if (s->n_seqs == 0 || s->total_q == 0) return MI_OK;
