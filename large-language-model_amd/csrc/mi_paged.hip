@@ -850,8 +850,8 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnParams p) {
   pa_join(p, row, head, n, [&](int i) { return i * pitch + at; });
 }
 
-// The same for up to four pieces: a wave a row, 32 lanes reading one piece's components and 32 another's.
-__global__ void __launch_bounds__(256) paged_attn_join4_kernel(AttnParams p) {
+// The same for up to eight pieces: a wave a row, 32 lanes reading one piece's components and 32 another's.
+__global__ void __launch_bounds__(256) paged_attn_join8_kernel(AttnParams p) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
   const int64_t at = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
   if (at >= (int64_t)p.pv.total_q * p.n_heads) return;
@@ -859,9 +859,9 @@ __global__ void __launch_bounds__(256) paged_attn_join4_kernel(AttnParams p) {
   const int n = pa_pieces_of(p, row, head);
   if (n < 2) return;
   const int64_t pitch = (int64_t)p.pv.total_q * p.n_heads;
-  float lse[4], mx = -INFINITY;
+  float lse[8], mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     lse[i] = i < n ? p.part_lse[i * pitch + at] : -INFINITY;
     mx = fmaxf(mx, lse[i]);
   }
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(256) paged_attn_join4_kernel(AttnParams p) {
   f32x4_t acc = {0, 0, 0, 0};
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float w = lse[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lse[i] - mx);
     sum += w;
     if ((i & 1) == half && i < n && c < p.d) acc += w * *(const f32x4_t*)(p.part_o + (i * pitch + at) * p.d + c);
@@ -902,7 +902,8 @@ struct PaPlan {
 // and a join 10.5); else a workgroup for each CU, of 128 keys at least (one sequence of 32768: 23.9 us,
 // in twice as many pieces 29); where those pieces are long and the sequences several, even shares (64 of
 // up to 8000: 115 us in pieces, 83 in shares; 64 of up to 1000: 19 and 24).
-// Many rows: pieces of 256 keys at least until there are two workgroups for each CU.
+// Many rows: pieces of 256 keys at least until there are three workgroups for each CU, of two that fit
+// (16 sequences of up to 333 rows over 2500 keys, 12 heads of 64: 43 us with two, 36 with three).
 PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t total_q, int64_t max_q, int64_t max_kv,
                bool one_each, int cus) {
   PaPlan pl;
@@ -912,7 +913,7 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   const int64_t rows = int64_t{1} << pl.tile_shift;
   pl.tiles = one_each ? n_seqs * ((g + rows - 1) / rows) : n_seqs + total_q * g / rows;
   const int64_t units = std::max<int64_t>(1, std::min(pl.tiles, n_seqs * ((q * g + rows - 1) / rows)) * n_kv);
-  const int64_t want = ((pl.few ? 1 : 2) * (int64_t)cus + units - 1) / units;
+  const int64_t want = ((pl.few ? 1 : 3) * (int64_t)cus + units - 1) / units;
   pl.min_piece = pl.few ? (max_kv <= 512 ? 512 : 128) : 256;
   const int64_t most = (max_kv + pl.min_piece - 1) / pl.min_piece;
   pl.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 256}));
@@ -1017,7 +1018,7 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   else paged_attn_kernel<128><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(p);
   e = hipGetLastError();
   if (e == hipSuccess && plan.pieces > 1) {
-    if (plan.pieces <= 4) paged_attn_join4_kernel<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, (hipStream_t)stream>>>(p);
+    if (plan.pieces <= 8) paged_attn_join8_kernel<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, (hipStream_t)stream>>>(p);
     else paged_attn_join_kernel<<<(unsigned)(rows * n_heads), 256, 0, (hipStream_t)stream>>>(p);
     e = hipGetLastError();
   }

@@ -134,7 +134,8 @@ def test_chunks(mi, dev, nH, nKV, d, causal):
 
 @pytest.mark.parametrize("order", ["phsd", "pshd"])
 @pytest.mark.parametrize("q,kv,nH,nKV,d", [([200], [1000], 8, 2, 128), ([129, 1, 64], [400, 700, 64], 4, 4, 64),
-                                           ([257], [257], 4, 1, 128)])
+                                           ([257], [257], 4, 1, 128), ([40, 3], [2600, 1900], 4, 2, 128),
+                                           ([33, 40], [700, 2048], 1, 1, 72)])
 def test_long_chunks(mi, dev, order, q, kv, nH, nKV, d):
     b = Batch(q, kv, 32, nH, nKV, d, seed=3, order=order)
     check(*run(mi, b), b.reference())
@@ -156,6 +157,37 @@ def test_long_context_split(mi, dev, n, d):
     check(*run(mi, b, max_kv_len=1 << 20), ref)  # and one far shorter
     a, c = run(mi, b), run(mi, b)
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+@pytest.mark.parametrize("S,nH,nKV,d,P", [(140, 4, 2, 64, 16), (70, 8, 4, 128, 1), (300, 1, 1, 40, 64), (1024, 2, 1, 8, 32)])
+def test_decode_many_uneven(mi, dev, S, nH, nKV, d, P):
+    """Sequences of very unequal length, some without a key, whose keys the workgroups share evenly; a row
+    that is cut is joined from its shares, and a share may run over many sequences."""
+    import torch
+
+    r = np.random.default_rng(S)
+    kv = [int(x) for x in np.exp(r.uniform(0, np.log(1500), S))]
+    kv[0], kv[S // 2], kv[S - 1], kv[3] = 2500, 2100, 0, 0
+    b = Batch([1] * S, kv, P, nH, nKV, d, seed=S, one_each=True)
+    ref = b.reference()
+    check(*run(mi, b), ref)
+    n = mi.paged_attn_workspace_size(nH, nKV, d, S, S, 1, max(kv))
+    ws = torch.full((n + 16,), 255, dtype=torch.uint8, device="cuda")
+    check(*run(mi, b, workspace=ws[:n]), ref)
+    assert (ws[n:] == 255).all()
+    check(*run(mi, b, workspace=ws[:n // 2 // 16 * 16]), ref)
+    a, c = run(mi, b), run(mi, b)
+    assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_page_tables(mi, dev, d):
+    """More pages in a workgroup's keys than it looks up at a time (pages of one token)."""
+    b = Batch([1, 1, 1], [5000, 1, 2999], 1, 2, 1, d, seed=d, one_each=True)
+    ref = b.reference()
+    check(*run(mi, b), ref)
+    check(*run(mi, b, workspace=None), ref)
+    check(*run(mi, b, max_kv_len=1), ref)
 
 
 def test_scale_and_large_scores(mi, dev):
