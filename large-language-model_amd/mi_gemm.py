@@ -20,6 +20,7 @@ is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import struct
@@ -252,9 +253,16 @@ def init():
 
 # ---- torch plumbing -----------------------------------------------------------
 
+_TORCH = None
+
+
 def _torch():
-    import torch
-    return torch
+    """torch, imported on first use (an import statement in each call costs 0.3 us)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
 
 
 def _dt(t) -> int:
@@ -1084,14 +1092,18 @@ _PACK_SEQS = struct.Struct("@qqPPPqq").pack         # mi_paged_seqs
 _PACK_SAMPLING = struct.Struct("@PPPPfiff").pack    # mi_sampling
 
 
-def _on_device(*tensors):
-    """The tensors (None aside) are on the current GPU, whose stream a call goes to."""
+def _stream_of(*tensors):
+    """The handle of the current stream, after a look at the tensors (None aside): all on the current GPU,
+    whose stream a call goes to."""
     here = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != here or here < 0):
             raise ValueError(f"a tensor is on {t.device}: all are needed on the current GPU")
-    if here != _torch().cuda.current_device():
+    C = _torch()._C
+    if here != C._cuda_getDevice():
         raise ValueError(f"the tensors are on cuda:{here}, which is not the current GPU")
+    raw = getattr(C, "_cuda_getCurrentRawStream", None)
+    return raw(here) if raw is not None else _torch().cuda.current_stream().cuda_stream
 
 
 def _done(fn, st, sync):
@@ -1153,8 +1165,8 @@ def _rotary(inv_freq, positions, B, T, pos0, interleaved, scale):
     return _PACK_ROTARY(inv_freq.data_ptr(), 2 * inv_freq.numel(), 1 if interleaved else 0, scale, at, ld, pos0)
 
 
-def _rope_call(parts, n, B, T, d, rotary, inverse, dtype, sync):
-    _done("mi_rope", load_library().mi_rope(_stream(), parts, n, B, T, d, rotary, 1 if inverse else 0, dtype), sync)
+def _rope_call(stream, parts, n, B, T, d, rotary, inverse, dtype, sync):
+    _done("mi_rope", load_library().mi_rope(stream, parts, n, B, T, d, rotary, 1 if inverse else 0, dtype), sync)
 
 
 def rope(x, inv_freq, positions=None, pos0=0, layout="bthd", inverse=False, interleaved=False, scale=1.0,
@@ -1172,12 +1184,12 @@ def rope(x, inv_freq, positions=None, pos0=0, layout="bthd", inverse=False, inte
         raise ValueError("out must match x's shape and dtype")
     if x.shape[3] > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
         raise ValueError("components must be contiguous")
-    _on_device(x, out, inv_freq, positions)
+    stream = _stream_of(x, out, inv_freq, positions)
     t, h = (1, 2) if layout == "bthd" else (2, 1)
     B, T, H = x.shape[0], x.shape[t], x.shape[h]
     part = _PACK_PART(x.data_ptr(), out.data_ptr(), H, x.stride(0), x.stride(t), x.stride(h),
                       out.stride(0), out.stride(t), out.stride(h), 1, 0)
-    _rope_call(part, 1, B, T, x.shape[3], _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), inverse,
+    _rope_call(stream, part, 1, B, T, x.shape[3], _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), inverse,
                _dt(x), sync)
     return out
 
@@ -1195,7 +1207,7 @@ def rope_qkv(qkv, n_heads, n_kv, inv_freq, positions=None, pos0=0, interleaved=F
     sb, st, sc = qkv.stride()
     if sc != 1 and n > 1:
         raise ValueError("components must be contiguous")
-    _on_device(qkv, inv_freq, positions)
+    stream = _stream_of(qkv, inv_freq, positions)
     dt, d = _dt(qkv), n // heads
     size = d * (4 if dt == MI_F32 else 2)
     Q, K, V = qkv.new_empty((B, n_heads, T, d)), qkv.new_empty((B, n_kv, T, d)), qkv.new_empty((B, n_kv, T, d))
@@ -1203,7 +1215,7 @@ def rope_qkv(qkv, n_heads, n_kv, inv_freq, positions=None, pos0=0, interleaved=F
     parts = (_PACK_PART(at, Q.data_ptr(), n_heads, sb, st, d, n_heads * row, d, row, 1, 0)
              + _PACK_PART(at + n_heads * size, K.data_ptr(), n_kv, sb, st, d, n_kv * row, d, row, 1, 0)
              + _PACK_PART(at + (n_heads + n_kv) * size, V.data_ptr(), n_kv, sb, st, d, n_kv * row, d, row, 0, 0))
-    _rope_call(parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), False, dt, sync)
+    _rope_call(stream, parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), False, dt, sync)
     return Q, K, V
 
 
@@ -1223,7 +1235,7 @@ def rope_qkv_backward(dQ4, dK4, dV4, inv_freq, positions=None, pos0=0, interleav
     ob, ot, oc = out.stride() if out.dim() == 3 else (0, 0, 0)
     if out.shape != (B, T, n) or out.dtype != dQ4.dtype or (oc != 1 and n > 1):
         raise ValueError(f"out must be {(B, T, n)} of dQ's dtype with a contiguous last dimension")
-    _on_device(dQ4, dK4, dV4, out, inv_freq, positions)
+    stream = _stream_of(dQ4, dK4, dV4, out, inv_freq, positions)
     dt = _dt(dQ4)
     at, size = out.data_ptr(), d * (4 if dt == MI_F32 else 2)
     parts = b""
@@ -1233,7 +1245,7 @@ def rope_qkv_backward(dQ4, dK4, dV4, inv_freq, positions=None, pos0=0, interleav
             raise ValueError("components must be contiguous")
         parts += _PACK_PART(t.data_ptr(), at, h, sb, st, sh, ob, ot, d, rotate, 0)
         at += h * size
-    _rope_call(parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), True, dt, sync)
+    _rope_call(stream, parts, 3, B, T, d, _rotary(inv_freq, positions, B, T, pos0, interleaved, scale), True, dt, sync)
     return out
 
 
@@ -1302,13 +1314,13 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
             q_out = q.new_empty((N, n_heads, d))
         o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
-    _on_device(k, v, k_cache, v_cache, pages, kv_len, q_start, q, q_out, inv_freq, positions)
+    stream = _stream_of(k, v, k_cache, v_cache, pages, kv_len, q_start, q, q_out, inv_freq, positions)
     rotary = None
     if inv_freq is not None:
         rotary = _rotary(inv_freq, positions, 1, N, 0, interleaved, scale)
     elif positions is not None:
         raise ValueError("positions without inv_freq")
-    st = load_library().mi_kv_append(_stream(), q_at, q_t, q_h, o_at, o_t, o_h, n_heads, k.data_ptr(), k_t, k_h,
+    st = load_library().mi_kv_append(stream, q_at, q_t, q_h, o_at, o_t, o_h, n_heads, k.data_ptr(), k_t, k_h,
                                      v.data_ptr(), v_t, v_h, cache, seqs, rotary)
     _done("mi_kv_append", st, sync)
     return q_out
@@ -1317,6 +1329,11 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
 def paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len) -> int:
     """Bytes of workspace paged_attn uses (mi_paged_attn_workspace_size)."""
     return load_library().mi_paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_bytes(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len, device):
+    return paged_attn_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len)
 
 
 def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None, max_kv_len=None, out=None,
@@ -1342,19 +1359,19 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
     o_t, o_h = _heads_of("out", out, N, n_heads, d)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, n_heads) or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 [{N}, {n_heads}] tensor")
-    _on_device(q, k_cache, v_cache, pages, kv_len, q_start, out, lse, None if isinstance(workspace, str) else workspace)
+    stream = _stream_of(q, k_cache, v_cache, pages, kv_len, q_start, out, lse,
+                        None if isinstance(workspace, str) else workspace)
     mq = 1 if q_start is None else N if max_q_len is None else int(max_q_len)
     mk = page * width if max_kv_len is None else int(max_kv_len)
-    L = load_library()
     at = size = 0
     if isinstance(workspace, str):
-        size = L.mi_paged_attn_workspace_size(n_heads, n_kv, d, n, N, mq, mk)
-        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
+        size = _attn_bytes(n_heads, n_kv, d, n, N, mq, mk, q.get_device())
+        workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     elif workspace is not None:
         size = workspace.numel() * workspace.element_size()
     if workspace is not None:
         at = workspace.data_ptr()
-    st = L.mi_paged_attn(_stream(), q.data_ptr(), q_t, q_h, out.data_ptr(), o_t, o_h,
+    st = load_library().mi_paged_attn(stream, q.data_ptr(), q_t, q_h, out.data_ptr(), o_t, o_h,
                          None if lse is None else lse.data_ptr(), n_heads, cache, seqs, mq, mk, 1 if causal else 0,
                          1.0 / math.sqrt(d) if scale is None else scale, at, size)
     _done("mi_paged_attn", st, sync)
@@ -1396,9 +1413,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         else:
             at.append(0)
             values.append(v)
-    _on_device(*tensors)
+    stream = _stream_of(*tensors)
     how = _PACK_SAMPLING(*at[:4], values[0], int(values[1]), values[2], values[3])
-    st = load_library().mi_sample(_stream(), logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V, how, *at[4:])
+    st = load_library().mi_sample(stream, logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V, how, *at[4:])
     _done("mi_sample", st, sync)
     return out
 
