@@ -107,6 +107,7 @@ def test_ties(mi, dev, dtype, how):
         x = x.to(torch.bfloat16 if dtype == "bf16" else torch.float32)
         u = torch.tensor([0.0, 0.25, 0.5, 0.7501, 0.999, 1 - 2.0 ** -24], device="cuda")
         check(mi, x, u, **how)
+        check(mi, x.repeat(50, 1), u.repeat(50), **how)  # more rows than CUs
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -122,6 +123,7 @@ def test_infinities_and_nan(mi, dev, dtype, how):
     x = torch.tensor(rows, device="cuda").to(torch.bfloat16 if dtype == "bf16" else torch.float32)
     for a in (0.0, 0.4, 0.99):
         check(mi, x, torch.full((8,), a, device="cuda"), **how)
+        check(mi, x.repeat(40, 1), torch.full((320,), a, device="cuda"), **how)
 
 
 def test_extreme_settings(mi, dev):
@@ -144,6 +146,20 @@ def test_extreme_settings(mi, dev):
     odd = torch.tensor([-1.0, 1.0, inf, float("nan")], device="cuda")
     got, order = mi.sample(x, odd, top_k=3).tolist(), x.argsort(1, descending=True)[:, :3].sort(1).values.tolist()
     assert got == [order[0][0], order[1][2], order[2][2], order[3][0]]
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("how", [dict(k=100), dict(k=160, p=0.9), dict(k=161, p=0.5), dict(k=255), dict(k=2000, p=0.99),
+                                 dict(p=0.9), dict(p=0.999, low=1e-4), dict(k=30, p=0.8, low=0.03, T=0.5)])
+def test_peaked_and_flat_rows(mi, dev, rows, how):
+    """Rows whose top tokens lie together in one lane's run, rows that are nearly flat, and rows with a tail."""
+    import torch
+
+    x, u = make(rows, 9001, "f32", rows)
+    x[::3, 500:700] += 30.0
+    x[1::3] *= 1e-3
+    check(mi, x, u, **how)
+    check(mi, x.bfloat16(), u, **how)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
