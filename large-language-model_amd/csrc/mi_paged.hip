@@ -136,8 +136,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int h32 = lane >> 5, l32 = lane & 31;
 
-  const int x = uniform(blockIdx.x % p.tiles), rest = uniform(blockIdx.x / p.tiles);
-  const int kvh = uniform(rest % p.n_kv), piece = uniform(rest / p.n_kv);
+  // Workgroup b runs on XCD b mod 8.  With the KV heads innermost an XCD's L2 holds the keys of few of
+  // them, which the row tiles of a sequence read at about the same time; the last tiles, which see the
+  // most keys, come first.
+  const int rest = uniform(blockIdx.x / p.n_kv), kvh = uniform(blockIdx.x - rest * p.n_kv);
+  const int piece = uniform(rest / p.tiles), x = uniform(p.tiles - 1 - (rest - piece * p.tiles));
   const PaTile t = pa_tile(p, x);
   if (t.s < 0) return;
   const int end = t.end(p), plen = pa_piece(p, end);
@@ -170,31 +173,48 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   const uint16_t* kbase = p.k + (int64_t)kvh * p.pv.head_stride;
   const uint16_t* vbase = p.v + (int64_t)kvh * p.pv.head_stride;
   int page_next = -1;   // page of key `lane` of the next block to be issued, read a block ahead of its use
-  int64_t row_off = 0;  // element offset of key `lane` of the block issued last, -1: none
-  uint64_t seen_next = 0;  // that block's keys that exist
+  uint64_t seen_next = 0;  // keys of the block issued last that exist
   auto look_up = [&](int base) __attribute__((always_inline)) {
     const int pos = base + lane;
     page_next = pos < k_end ? p.pv.pages[(int64_t)t.s * p.pv.pages_ld + (pos >> p.pv.page_shift)] : -1;
   };
-  auto resolve = [&](int base) __attribute__((always_inline)) {
-    const bool there = (uint32_t)page_next < (uint32_t)p.pv.num_pages;
-    const int slot = (base + lane) & ((1 << p.pv.page_shift) - 1);
-    row_off = there ? page_next * p.pv.page_stride + slot * p.pv.slot_stride : -1;
-    seen_next = __ballot(there);
+  // The wave's 16 rows lie in one page where pages are of 16 tokens or more: a scalar base and these offsets.
+  const bool even = p.pv.page_shift >= 4 && p.d == D && p.pv.slot_stride <= (1 << 24);
+  uint32_t k_off[L::NU], v_off[L::NU];
+#pragma unroll
+  for (int u = 0; u < L::NU; ++u) {
+    const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
+    k_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::k_pos(r, at));
+    v_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::v_pos(r, at));
+  }
+  auto to_lds = [&](const uint16_t* src, uint32_t dst) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(uintptr_t)src,
+                                     (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0, 0);
   };
-  auto issue = [&](int stage) __attribute__((always_inline)) {
+  // asks for the block at `base`, whose pages have been looked up
+  auto issue = [&](int base, int stage) __attribute__((always_inline)) {
+    const bool there = (uint32_t)page_next < (uint32_t)p.pv.num_pages;
+    const int mask = (1 << p.pv.page_shift) - 1;
+    const uint32_t dst = lds0 + (uint32_t)(stage * STAGE + wave * L::NU * 1024);
+    seen_next = __ballot(there);
+    if (even && seen_next == ~uint64_t{0}) {
+      const int64_t at = __builtin_amdgcn_readlane(page_next, 16 * wave) * p.pv.page_stride +
+                         ((base + 16 * wave) & mask) * p.pv.slot_stride;
+#pragma unroll
+      for (int u = 0; u < L::NU; ++u) {
+        to_lds(kbase + at + k_off[u], dst + u * 1024);
+        to_lds(vbase + at + v_off[u], dst + u * 1024 + L::BYTES);
+      }
+      return;
+    }
+    const int64_t row_off = there ? page_next * p.pv.page_stride + ((base + lane) & mask) * p.pv.slot_stride : -1;
 #pragma unroll
     for (int u = 0; u < L::NU; ++u) {
       const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
       const int64_t off = __shfl(row_off, r, 64);
       const int kc = 8 * L::k_pos(r, at), vc = 8 * L::v_pos(r, at);
-      const void* ks = off >= 0 && kc < p.d ? (const void*)(kbase + off + kc) : (const void*)pa_zero;
-      const void* vs = off >= 0 && vc < p.d ? (const void*)(vbase + off + vc) : (const void*)pa_zero;
-      const uint32_t dst = lds0 + (uint32_t)(stage * STAGE + (wave * L::NU + u) * 1024);
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(uintptr_t)ks,
-                                       (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(uintptr_t)vs,
-                                       (__attribute__((address_space(3))) void*)(uintptr_t)(dst + L::BYTES), 16, 0, 0);
+      to_lds(off >= 0 && kc < p.d ? kbase + off + kc : (const uint16_t*)pa_zero, dst + u * 1024);
+      to_lds(off >= 0 && vc < p.d ? vbase + off + vc : (const uint16_t*)pa_zero, dst + u * 1024 + L::BYTES);
     }
   };
 
@@ -220,8 +240,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   float m_run = -INFINITY, l_run = 0.0f;
   const float sl2 = p.scale_log2;
 
-  auto block = [&](uint32_t st, uint64_t seen, auto masked) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(masked)::value;
+  // One 64-key block; `seen`: the keys that this lane's row sees, of which none is missing in any row of the
+  // wave unless `masked`.
+  auto block = [&](uint32_t st, uint64_t seen, bool masked) __attribute__((always_inline)) {
     f32x16_t sc[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -241,19 +262,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf[s][kb]),
                                                         __builtin_bit_cast(bf16x8_t, qf[s]), sc[kb], 0, 0, 0);
     // sc[kb][4q + e] is key 32kb + 8*h32 + 16(q>>1) + 4(q&1) + e
-    float mx = -INFINITY;
+    if (masked) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const uint32_t bits = (uint32_t)(seen >> (32 * kb)) >> (8 * h32);
+      for (int kb = 0; kb < 2; ++kb) {
+        const uint32_t bits = (uint32_t)(seen >> (32 * kb)) >> (8 * h32);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (MASK) {
+        for (int i = 0; i < 16; ++i) {
           const int at = 16 * ((i >> 2) >> 1) + 4 * ((i >> 2) & 1) + (i & 3);
           sc[kb][i] = (bits >> at) & 1 ? sc[kb][i] : -INFINITY;
         }
-        mx = fmaxf(mx, sc[kb][i]);
       }
     }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     // a row keeps its reference maximum until a block raises it by more than PA_TAU
     const float m_old = m_run;
@@ -314,8 +338,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
   const int n_blocks = uniform((k_end - k_begin + PA_KEYS - 1) / PA_KEYS);
   if (n_blocks > 0) {
     look_up(k_begin);
-    resolve(k_begin);
-    issue(0);
+    issue(k_begin, 0);
     look_up(k_begin + PA_KEYS);
   }
   for (int j = 0; j < n_blocks; ++j) {
@@ -324,18 +347,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     wait_vmcnt<0>();     // this wave's share of block j has landed, and the pages of block j + 1
     lds_ring_barrier();  // and everyone's; and block j - 1 has been read
     if (j + 1 < n_blocks) {
-      resolve(base + PA_KEYS);
-      issue((j + 1) & 1);
+      issue(base + PA_KEYS, (j + 1) & 1);
       look_up(base + 2 * PA_KEYS);
     }
     const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
     if (!wave_has_rows || base >= lim_hi) continue;
-    if (base + PA_KEYS <= lim_lo && seen == ~uint64_t{0}) {
-      block(st, seen, std::false_type{});
-    } else {
-      const int room = lim - base;
-      block(st, room >= 64 ? seen : room <= 0 ? 0 : seen & ((uint64_t{1} << room) - 1), std::true_type{});
-    }
+    const bool masked = base + PA_KEYS > lim_lo || seen != ~uint64_t{0};
+    const int room = lim - base;
+    block(st, room >= 64 ? seen : room <= 0 ? 0 : seen & ((uint64_t{1} << room) - 1), masked);
   }
 
   if (!wave_has_rows || 32 * wave + l32 >= n_packed) return;
@@ -681,19 +700,24 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
                 [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
 }
 
-// Pieces of the keys of a row's tile; a row that no sequence has counts as whole.
-__device__ __forceinline__ int pa_pieces_of(const AttnParams& p, int row, int head) {
+// The sequence of a row (s < 0: none), and the pieces of the keys of one of its heads' tile.
+__device__ __forceinline__ PaTile pa_row_tile(const AttnParams& p, int row) {
   PaTile t;
   t.s = row;
   t.q0 = row;
   t.n = 1;
   if (p.pv.q_start) {
     t.s = wave_first_false(p.pv.n_seqs, [&](int k) { return p.pv.q_start[k + 1] <= row; });
-    if (t.s >= p.pv.n_seqs) return 1;
-    seq_rows(p.pv, t.s, t.q0, t.n);
-    if (row < t.q0 || row >= t.q0 + t.n) return 1;
+    if (t.s < p.pv.n_seqs) seq_rows(p.pv, t.s, t.q0, t.n);
+    if (t.s >= p.pv.n_seqs || row < t.q0 || row >= t.q0 + t.n) {
+      t.s = -1;
+      return t;
+    }
   }
   t.len = p.pv.kv_len[t.s];
+  return t;
+}
+__device__ __forceinline__ int pa_pieces_of(const AttnParams& p, PaTile t, int row, int head) {
   const int packed = (row - t.q0) * p.group + head % p.group;
   t.first = packed >> p.tile_shift << p.tile_shift;
   const int end = t.end(p), plen = pa_piece(p, end);
@@ -844,43 +868,47 @@ __global__ void __launch_bounds__(256) paged_attn_share_join_kernel(AttnParams p
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnParams p) {
   const int64_t at = blockIdx.x;
   const int row = (int)(at / p.n_heads), head = (int)(at - (int64_t)row * p.n_heads);
-  const int n = pa_pieces_of(p, row, head);
+  const PaTile t = pa_row_tile(p, row);
+  if (t.s < 0) return;
+  const int n = pa_pieces_of(p, t, row, head);
   if (n < 2) return;
   const int64_t pitch = (int64_t)p.pv.total_q * p.n_heads;
   pa_join(p, row, head, n, [&](int i) { return i * pitch + at; });
 }
 
-// The same for up to eight pieces: a wave a row, 32 lanes reading one piece's components and 32 another's.
+// The same for up to eight pieces of many rows: a workgroup a token, 32 lanes a head, all pieces' loads in flight.
 __global__ void __launch_bounds__(256) paged_attn_join8_kernel(AttnParams p) {
-  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-  const int64_t at = (int64_t)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
-  if (at >= (int64_t)p.pv.total_q * p.n_heads) return;
-  const int row = (int)(at / p.n_heads), head = (int)(at - (int64_t)row * p.n_heads);
-  const int n = pa_pieces_of(p, row, head);
-  if (n < 2) return;
+  const int l32 = threadIdx.x & 31, c = 4 * l32, row = blockIdx.x;
+  const PaTile t = pa_row_tile(p, row);
+  if (t.s < 0) return;
   const int64_t pitch = (int64_t)p.pv.total_q * p.n_heads;
-  float lse[8], mx = -INFINITY;
+  for (int head = threadIdx.x >> 5; head < p.n_heads; head += 8) {
+    const int n = pa_pieces_of(p, t, row, head);
+    if (n < 2) continue;
+    const int64_t at = (int64_t)row * p.n_heads + head;
+    float lse[8];
+    f32x4_t x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lse[i] = i < n ? p.part_lse[i * pitch + at] : -INFINITY;
-    mx = fmaxf(mx, lse[i]);
+    for (int i = 0; i < 8; ++i) {
+      lse[i] = i < n ? p.part_lse[i * pitch + at] : -INFINITY;
+      x[i] = i < n && c < p.d ? *(const f32x4_t*)(p.part_o + (i * pitch + at) * p.d + c) : f32x4_t{0, 0, 0, 0};
+    }
+    float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, lse[i]);
+    f32x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = lse[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lse[i] - mx);
+      sum += w;
+      acc += w * x[i];
+    }
+    acc *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (c < p.d)
+      *(u32x2_t*)(p.o + (int64_t)row * p.o_t + (int64_t)head * p.o_h + c) =
+          u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    if (p.lse && l32 == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
   }
-  const int c = 4 * l32;
-  f32x4_t acc = {0, 0, 0, 0};
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float w = lse[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lse[i] - mx);
-    sum += w;
-    if ((i & 1) == half && i < n && c < p.d) acc += w * *(const f32x4_t*)(p.part_o + (i * pitch + at) * p.d + c);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], 32, 64);
-  acc *= sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (half == 0 && c < p.d)
-    *(u32x2_t*)(p.o + (int64_t)row * p.o_t + (int64_t)head * p.o_h + c) =
-        u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
-  if (p.lse && lane == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
 }
 
 // How a launch is laid out: tiles of rows, pieces of a tile's keys, and keys of a piece at least.
@@ -1018,7 +1046,7 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   else paged_attn_kernel<128><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(p);
   e = hipGetLastError();
   if (e == hipSuccess && plan.pieces > 1) {
-    if (plan.pieces <= 8) paged_attn_join8_kernel<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, (hipStream_t)stream>>>(p);
+    if (plan.pieces <= 8 && !plan.few) paged_attn_join8_kernel<<<(unsigned)rows, 256, 0, (hipStream_t)stream>>>(p);
     else paged_attn_join_kernel<<<(unsigned)(rows * n_heads), 256, 0, (hipStream_t)stream>>>(p);
     e = hipGetLastError();
   }
