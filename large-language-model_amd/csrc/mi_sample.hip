@@ -37,6 +37,7 @@ namespace {
 constexpr int SMP_BINS = 1024;
 constexpr int SMP_LIST = 1024;        // tokens of a bin that are ranked in LDS
 constexpr int SMP_FEW = 256;          // tokens that are handled in LDS altogether
+constexpr int SMP_FEW_K = SMP_FEW * 5 / 8;  // the largest top-k for which that is tried
 constexpr int SMP_GATHER = 4;         // logits that a lane weighs at a time: its waits for each overlap
 
 struct SampleParams {
@@ -101,6 +102,33 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {  // inclusive
   return v;
 }
 
+// Weights of logits up to a finite maximum.
+struct SampleWeights {
+  double mx, c32, to_bits;  // w + to_bits: w * 2^shift, rounded, in the low bits
+  const double* pow32;      // LDS, 2^(j/32)
+  __device__ __forceinline__ SampleWeights(float mx_, float T, int shift, const double* pow32_)
+      : mx((double)mx_), c32(32.0 * (1.4426950408889634074 / (double)T)),
+        to_bits(1.5 * (double)(uint64_t{1} << (52 - shift))), pow32(pow32_) {}
+  __device__ __forceinline__ double of(float v) const {  // as a 64-bit float
+    const double y = max(((double)v - mx) * c32, -2048.0);  // 32 y; 2^-64 rounds to nothing
+    const double t = y + 6755399441055744.0;                // 1.5 * 2^52: rounded, in the low bits
+    const int n = (int)(uint32_t)__double_as_longlong(t);
+    const double z = y - (t - 6755399441055744.0);          // |z| <= 1/2, of 1/32
+    // 2^(z/32) = sum (z ln 2 / 32)^k / k!, past k = 5 below 2^-48
+    double q = 3.9737099845494154e-11;
+    q = fma(q, z, 9.172562701824643e-09);
+    q = fma(q, z, 1.6938509724371819e-06);
+    q = fma(q, z, 2.3459619820224677e-04);
+    q = fma(q, z, 2.1660849392498290e-02);
+    q = fma(q, z, 1.0);
+    q *= pow32[n & 31];
+    return __hiloint2double(__double2hiint(q) + ((n >> 5) << 20), __double2loint(q));
+  }
+  __device__ __forceinline__ uint64_t whole(double w) const {  // rounded to whole 2^-shift
+    return (uint64_t)(__double_as_longlong(w + to_bits) - __double_as_longlong(to_bits));
+  }
+};
+
 template <int WAVES>
 struct SampleShared {
   uint64_t bins[SMP_BINS];
@@ -119,10 +147,9 @@ struct SampleShared {
 };
 
 template <int TH, bool BF16, bool ALIGNED>
-__global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
+__device__ __forceinline__ void sample_row(const SampleParams& p, int row, SampleShared<TH / 64>& sh) {
   constexpr int EV = BF16 ? 8 : 4, WAVES = TH / 64;
-  __shared__ SampleShared<WAVES> sh;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int V = p.vocab, layers = p.layers;
   const void* x = (const char*)p.logits + (int64_t)row * p.ld * (BF16 ? 2 : 4);
   // this wave's run of the row: layer i holds elements first + (64 i + lane) EV ..; a whole number of
@@ -200,28 +227,10 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
     return;
   }
 
-  // weights of logits up to a finite maximum
-  const double c = 1.4426950408889634074 / (double)T;
-  const double c32 = 32.0 * c, mxd = (double)mx;
-  const double to_bits = 1.5 * (double)(uint64_t{1} << (52 - p.shift));  // w + this: w * 2^shift in the low bits
-  auto weight_of = [&](float v) __attribute__((always_inline)) {  // as a 64-bit float
-    const double y = max(((double)v - mxd) * c32, -2048.0);  // 32 y; 2^-64 rounds to nothing
-    const double t = y + 6755399441055744.0;                 // 1.5 * 2^52: rounded, in the low bits
-    const int n = (int)(uint32_t)__double_as_longlong(t);
-    const double z = y - (t - 6755399441055744.0);           // |z| <= 1/2, of 1/32
-    // 2^(z/32) = sum (z ln 2 / 32)^k / k!, past k = 5 below 2^-48
-    double q = 3.9737099845494154e-11;
-    q = fma(q, z, 9.172562701824643e-09);
-    q = fma(q, z, 1.6938509724371819e-06);
-    q = fma(q, z, 2.3459619820224677e-04);
-    q = fma(q, z, 2.1660849392498290e-02);
-    q = fma(q, z, 1.0);
-    q *= sh.pow32[n & 31];
-    return __hiloint2double(__double2hiint(q) + ((n >> 5) << 20), __double2loint(q));
-  };
-  auto whole_of = [&](double w) __attribute__((always_inline)) {  // rounded to whole 2^-shift
-    return (uint64_t)(__double_as_longlong(w + to_bits) - __double_as_longlong(to_bits));
-  };
+  const SampleWeights W(mx, T, p.shift, sh.pow32);
+  const double c = W.c32 * 0.03125, mxd = W.mx;
+  auto weight_of = [&](float v) __attribute__((always_inline)) { return W.of(v); };
+  auto whole_of = [&](double w) __attribute__((always_inline)) { return W.whole(w); };
 
   // Kept: logits above `border`, and the first `ties` tokens that equal it, which weigh `tie` each.
   float border = -INFINITY;
@@ -414,7 +423,7 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
   };
   if (top_k > 0 && top_k < V) {
     int few = 0;  // tokens in the list, among them all that may be kept
-    if (top_k <= SMP_FEW * 5 / 8) {
+    if (top_k <= SMP_FEW_K) {
       // The top_k-th of the lanes' own maxima bounds the row's from below: a bin for each lane instead of
       // one for each token, and what lies above it is seldom much more than top_k tokens.
       clear();
@@ -660,6 +669,385 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
   });
 }
 
+template <int TH, bool BF16, bool ALIGNED>
+__global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
+  __shared__ SampleShared<TH / 64> sh;
+  sample_row<TH, BF16, ALIGNED>(p, blockIdx.x, sh);
+}
+
+// Long rows of bf16 logits hold few distinct ones (32000 normal ones about 2200): they are counted by
+// their bits, 32768 counters of 16 bits in LDS, and listed in order with their counts, so only the
+// distinct ones are weighed and all three borders lie in running sums over the list.  The second pass
+// takes each token's weight from LDS by its bits.  The answers are those of the kernel above, to the bit.
+// Normal logits, top-p 0.9, without / with it (us):
+//             8192       16384      32000 logits
+//    64 rows  16.6/15.7  22.7/17.8  35.4/23.6
+//   512 rows  22.7/19.4  34.0/25.4  60.0/38.5   (4096 logits: 15.4/16.5)
+// LDS and vector instructions bound it: of a row's 17 us alone 4 go to the counting, 4 to the second
+// pass, 7 to the list and its sums.  80 KB of LDS leave room for two blocks of 512 threads on a CU.
+constexpr int SMC_LIST = 3584;          // distinct logits of a row
+constexpr int SMC_KEPT = SMC_LIST / 2;  // of them above the border: their 64-bit weights fill the list
+constexpr int SMC_FROM = 8192;          // logits of a row from which it pays to clear and read the counters
+
+template <int WAVES>
+struct SampleCounts {
+  uint32_t count[16384];  // two 16-bit counters each; then the kept logits' places in the list
+  union {
+    uint32_t list[SMC_LIST];     // place << 16 | count, from the largest
+    uint64_t weights[SMC_KEPT];  // of the kept ones
+  };
+  uint16_t chunk[256] __attribute__((aligned(16)));  // distinct logits of 128 places
+  double pow32[32];
+  uint64_t wave_sum[WAVES];
+  uint32_t wave_cnt[WAVES];
+  uint64_t above, weight;
+  uint32_t entry, place, ties, other;
+};
+
+// Finite logits have places in order if they are 0 or their absolute value lies in [2^-64, 2^64), the
+// uppermost two of that left out: zeros 0x4000, the others from there by their absolute bits.  -inf has
+// one below 0; the rest (`other`) is left to the general kernel.
+constexpr int SMC_ZERO = 0x4000, SMC_FIRST = 63 << 7;  // exponent -64
+__device__ __forceinline__ int place_of(uint32_t h) {
+  const int a = (int)(h & 0x7fffu), d = a ? a - (SMC_FIRST - 1) : 0;
+  return SMC_ZERO + ((h & 0x8000u) ? -d : d);
+}
+__device__ __forceinline__ bool has_place(uint32_t h) {
+  const uint32_t a = h & 0x7fffu;
+  return a == 0 || a - SMC_FIRST < (uint32_t)SMC_ZERO - 1;
+}
+// The places of two logits at once, of those that have one; -inf below all of them.
+typedef int16_t s16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ s16x2_t places_of(uint32_t hh) {
+  const s16x2_t a = __builtin_bit_cast(s16x2_t, hh & 0x7fff7fffu), sign = __builtin_bit_cast(s16x2_t, hh) >> 15;
+  const s16x2_t d = __builtin_elementwise_max(a - (int16_t)(SMC_FIRST - 1), s16x2_t{0, 0});
+  return (d ^ sign) - sign + (int16_t)SMC_ZERO;
+}
+__device__ __forceinline__ float logit_at(int place) {
+  const int d = place - SMC_ZERO, a = abs(d) + SMC_FIRST - 1;
+  return d == 0 ? 0.0f : bf16_bits_to_f32((uint32_t)(d < 0 ? a | 0x8000 : a));
+}
+
+// How many bits of a wave's mask belong to lanes before this one.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// Whether it has answered; if not (a logit without a place, too many distinct ones) nothing is written.
+template <int TH, bool ALIGNED>
+__device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, float T, int top_k, float top_p,
+                                               float min_p, SampleCounts<TH / 64>& sh) {
+  constexpr int EV = 8, WAVES = TH / 64, EACH = (SMC_LIST + TH - 1) / TH;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), V = p.vocab, layers = p.layers;
+  const void* x = (const char*)p.logits + (int64_t)row * p.ld * 2;
+  const int first = wave * layers * 64 * EV + lane * EV;
+  // four vectors are under way at a time
+  u32x4_t vec[4];
+  auto fetch = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vec[j] = smp_load<true, ALIGNED>(x, first + 64 * EV * (i0 + j), V);
+  };
+  auto each_vector = [&](auto f) __attribute__((always_inline)) {
+    for (int i0 = 0; i0 < layers; i0 += 4) {
+      if (i0) fetch(i0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j < layers && !f(i0 + j, vec[j])) return;
+    }
+  };
+  auto bits_at = [&](const u32x4_t& v, int e) { return (e & 1) ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu; };
+  fetch(0);
+#pragma unroll
+  for (int i = 0; i < 4096 / TH; ++i) *(u32x4_t*)(sh.count + 4 * (tid + TH * i)) = u32x4_t{0, 0, 0, 0};
+  if (tid < 32) sh.pow32[tid] = exp2(tid * 0.03125);
+  if (tid == 0) sh.other = 0;
+  __syncthreads();
+  each_vector([&](int, const u32x4_t& v) __attribute__((always_inline)) {
+    // the largest and the least absolute bits, zeros aside
+    u16x2_t most = {0, 0}, least = {0xffff, 0xffff};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u16x2_t a = __builtin_bit_cast(u16x2_t, v[i] & 0x7fff7fffu);
+      most = __builtin_elementwise_max(most, a);
+      least = __builtin_elementwise_min(least, (u16x2_t)(a - (uint16_t)1));
+    }
+    if (max(most.x, most.y) >= SMC_FIRST + SMC_ZERO - 1 || min(least.x, least.y) < SMC_FIRST - 1) {
+#pragma unroll
+      for (int e = 0; e < EV; ++e)
+        if (!has_place(bits_at(v, e)) && bits_at(v, e) != 0xff80u) sh.other = 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const s16x2_t at = places_of(v[i]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int k = e ? at.y : at.x;  // below 0: -inf, or too large
+        if (k >= 0) atomicAdd(&sh.count[k >> 1], 1u << ((k & 1) << 4));
+      }
+    }
+    return true;
+  });
+  __syncthreads();
+
+  // The list, from the largest down: 256 chunks of 128 places, dealt to the waves in turn, since most
+  // of them are empty and the others lie together.
+  constexpr int CHUNKS = 16384 / 64, STEPS = CHUNKS / WAVES, GROUPS = WAVES / 4;
+  const int word0 = 16383 - wave * 64 - lane;  // of the wave's first chunk
+#pragma unroll 8
+  for (int i = 0; i < STEPS; ++i) {
+    const uint32_t w = sh.count[word0 - 64 * WAVES * i];
+    const uint32_t n = __popcll(__ballot(w & 0xffffu)) + __popcll(__ballot(w >> 16));
+    if (lane == 0) sh.chunk[WAVES * i + wave] = (uint16_t)n;
+  }
+  __syncthreads();
+  if (sh.other) return false;
+  uint32_t n_list;
+  {
+    // lane l adds up the chunks 4 l .. 4 l + 3; the wave's own are with the lanes GROUPS i + wave / 4
+    const u32x2_t c = *(const u32x2_t*)(sh.chunk + 4 * lane);
+    uint32_t sum = 0, before = 0, own = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t n = (e & 1) ? c[e >> 1] >> 16 : c[e >> 1] & 0xffffu;
+      if (e == wave % 4) before = sum, own = n;
+      sum += n;
+    }
+    const uint32_t to = (uint32_t)wave_scan_u64(sum);
+    before += to - sum;
+    n_list = (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
+    if (n_list == 0) {
+      if (tid == 0) {
+        p.tokens[row] = -1;
+        if (p.probs) p.probs[row] = 0.0f;
+      }
+      return true;
+    }
+    if (n_list > SMC_LIST) return false;
+    uint64_t full = __ballot(own && lane % GROUPS == wave / 4);
+    while (full) {
+      const int l = __ffsll((unsigned long long)full) - 1;
+      full &= full - 1;
+      const int word = word0 - 64 * WAVES * (l / GROUPS);
+      const uint32_t w = sh.count[word];
+      uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)before, l) + lanes_below(__ballot(w & 0xffffu)) +
+                    lanes_below(__ballot(w >> 16));
+      if (w >> 16) sh.list[at++] = (uint32_t)(2 * word + 1) << 16 | w >> 16;
+      if (w & 0xffffu) sh.list[at] = (uint32_t)(2 * word) << 16 | (w & 0xffffu);
+    }
+  }
+  __syncthreads();
+  const SampleWeights W(logit_at(sh.list[0] >> 16), T, p.shift, sh.pow32);
+
+  // Entries each * tid .., their weights, and running sums of tokens and weight.
+  const int each = (int)(n_list + TH - 1) / TH;
+  uint32_t place[EACH], n[EACH];
+  uint64_t w[EACH], mass = 0;
+  uint32_t tokens = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = each * tid + i;
+    place[i] = n[i] = 0;
+    w[i] = 0;
+    if (i < each && e < (int)n_list) {
+      const uint32_t v = sh.list[e];
+      place[i] = v >> 16;
+      n[i] = v & 0xffffu;
+      w[i] = W.whole(W.of(logit_at(place[i])));
+    }
+    tokens += n[i];
+    mass += n[i] * w[i];
+  }
+  const uint64_t mass_to = wave_scan_u64(mass);
+  const uint32_t tokens_to = (uint32_t)wave_scan_u64(tokens);
+  if (lane == 63) sh.wave_sum[wave] = mass_to, sh.wave_cnt[wave] = tokens_to;
+  __syncthreads();
+  uint64_t mass0 = mass_to - mass, total = 0;  // before this thread's entries
+  uint32_t tokens0 = tokens_to - tokens, all_tokens = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    mass0 += i < wave ? sh.wave_sum[i] : 0;
+    tokens0 += i < wave ? sh.wave_cnt[i] : 0;
+    total += sh.wave_sum[i];
+    all_tokens += sh.wave_cnt[i];
+  }
+  // Kept: entries before `entry`, and the first `ties` tokens of it.
+  uint32_t entry = n_list - 1, ties = sh.list[n_list - 1] & 0xffffu;
+  if (top_k > 0 && (uint32_t)top_k < all_tokens) {
+    uint32_t t = tokens0;
+    uint64_t m = mass0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (t < (uint32_t)top_k && (uint32_t)top_k <= t + n[i]) {
+        sh.entry = each * tid + i;
+        sh.ties = top_k - t;
+        sh.above = m + (top_k - t) * w[i];
+      }
+      t += n[i];
+      m += n[i] * w[i];
+    }
+    __syncthreads();
+    entry = sh.entry;
+    ties = sh.ties;
+    total = sh.above;
+    __syncthreads();
+  }
+  if (top_p < 1.0f) {
+    const double share = ceil((double)top_p * (double)total);
+    const uint64_t goal = share >= 1.0 ? (uint64_t)share : 1;
+    uint64_t m = mass0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint64_t to = m + n[i] * w[i];
+      if (m < goal && goal <= to) {
+        sh.entry = each * tid + i;
+        sh.ties = (uint32_t)((goal - m + w[i] - 1) / w[i]);
+      }
+      m = to;
+    }
+    __syncthreads();
+    if (sh.entry < entry) entry = sh.entry, ties = sh.ties;
+    else if (sh.entry == entry) ties = min(ties, sh.ties);
+    __syncthreads();
+  }
+  if (min_p > 0.0f) {
+    // the last entry that weighs enough; the first always does
+    const double low = min((double)min_p, 1.0);
+    if (tid == 0) sh.entry = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (n[i] && (uint32_t)(each * tid + i) <= entry && W.of(logit_at(place[i])) >= low)
+        atomicMax(&sh.entry, (uint32_t)(each * tid + i));
+    __syncthreads();
+    if (sh.entry < entry) entry = sh.entry, ties = sh.list[entry] & 0xffffu;
+  }
+  if (entry >= SMC_KEPT) return false;
+  __syncthreads();  // the list has been read
+  {
+    uint64_t m = mass0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const uint32_t e = each * tid + i;
+      if (n[i] && e < entry) {
+        sh.weights[e] = w[i];
+        ((uint16_t*)sh.count)[place[i]] = (uint16_t)e;
+      } else if (n[i] && e == entry) {
+        sh.weights[e] = 0;  // its tokens count by their order
+        ((uint16_t*)sh.count)[place[i]] = (uint16_t)e;
+        sh.place = place[i];
+        sh.weight = w[i];
+        sh.above = m + ties * w[i];
+      }
+      m += n[i] * w[i];
+    }
+  }
+  __syncthreads();
+  const int border = sh.place;
+  const uint64_t tie_weight = sh.weight;
+  total = sh.above;
+
+  // Each wave's weight above the border, and its ties.
+  auto weight_at = [&](int at) __attribute__((always_inline)) {
+    return sh.weights[((const uint16_t*)sh.count)[max(at, border)]];
+  };
+  fetch(0);
+  uint64_t m = 0;
+  uint32_t nt = 0;
+  const s16x2_t borders = {(int16_t)border, (int16_t)border};
+  each_vector([&](int, const u32x4_t& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const s16x2_t k = places_of(v[i]), at = __builtin_elementwise_max(k, borders);
+      m += sh.weights[((const uint16_t*)sh.count)[at.x]] + sh.weights[((const uint16_t*)sh.count)[at.y]];
+      nt += (k.x == border) + (k.y == border);
+    }
+    return true;
+  });
+  m = wave_sum_u64(m);
+  nt = (uint32_t)wave_sum_u64(nt);
+  if (lane == 0) sh.wave_sum[wave] = m, sh.wave_cnt[wave] = nt;
+  __syncthreads();
+  uint64_t acc = 0, own = 0, sum = 0;
+  uint32_t seen = 0, all_seen = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    if (i == wave) acc = sum, seen = all_seen;
+    const uint32_t left = ties > all_seen ? ties - all_seen : 0;
+    const uint64_t of_wave = sh.wave_sum[i] + tie_weight * min(left, sh.wave_cnt[i]);
+    if (i == wave) own = of_wave;
+    sum += of_wave;
+    all_seen += sh.wave_cnt[i];
+  }
+  const double t = (double)p.u[row] * (double)total;
+  uint64_t target = t > 0.0 ? (uint64_t)t : 0;
+  if (target >= total) target = total - 1;
+  if (target < acc || target - acc >= own) return true;
+  if (layers > 4) fetch(0);
+  each_vector([&](int i, const u32x4_t& v) __attribute__((always_inline)) {
+    uint32_t ties_here = 0;
+#pragma unroll
+    for (int e = 0; e < EV; ++e) ties_here += place_of(bits_at(v, e)) == border;
+    uint32_t rank = seen, all_ties = 0;
+    if (__any(ties_here)) {
+      const uint32_t upto = (uint32_t)wave_scan_u64(ties_here);
+      rank += upto - ties_here;
+      all_ties = (uint32_t)__shfl((int)upto, 63, 64);
+    }
+    uint64_t we[EV], s = 0;
+#pragma unroll
+    for (int e = 0; e < EV; ++e) {
+      const int k = place_of(bits_at(v, e));
+      we[e] = k == border && rank < ties ? tie_weight : weight_at(k);
+      rank += k == border;
+      s += we[e];
+    }
+    const uint64_t upto = acc + wave_scan_u64(s), from = upto - s;
+    if (from <= target && target < upto) {
+      uint64_t run = from;
+      bool open = true;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        run += we[e];
+        if (open && run > target) {
+          open = false;
+          p.tokens[row] = first + 64 * EV * i + e;
+          if (p.probs) p.probs[row] = (float)((double)we[e] / (double)total);
+        }
+      }
+    }
+    acc = __shfl(upto, 63, 64);
+    seen += all_ties;
+    return acc <= target;
+  });
+  return true;
+}
+
+// Whether a border is looked for among many tokens.  (64 rows of 32000: top-k 200 21.6 us without counts,
+// 25.6 with; top-k 1000 27.6 and 23.2; min-p alone 20.1 and 24.6.)
+__host__ __device__ __forceinline__ bool counts_pay(int top_k, float top_p, int vocab) {
+  return top_k > 0 && top_k < vocab ? top_k > SMP_FEW : top_p < 1.0f;
+}
+
+// Rows of at most 65535 bf16 logits.
+template <int TH, bool ALIGNED>
+__global__ void __launch_bounds__(TH) sample_counts_kernel(SampleParams p) {
+  __shared__ union {
+    SampleCounts<TH / 64> counted;
+    SampleShared<TH / 64> general;
+  } sh;
+  const int row = blockIdx.x;
+  const float T = p.how.temperature ? p.how.temperature[row] : p.how.temperature_all;
+  const int top_k = p.how.top_k ? p.how.top_k[row] : p.how.top_k_all;
+  const float top_p = p.how.top_p ? p.how.top_p[row] : p.how.top_p_all;
+  const float min_p = p.how.min_p ? p.how.min_p[row] : p.how.min_p_all;
+  if (T > 0.0f && counts_pay(top_k, top_p, p.vocab)) {
+    if (sample_counted<TH, ALIGNED>(p, row, T, top_k, top_p, min_p, sh.counted)) return;
+    __syncthreads();
+  }
+  sample_row<TH, true, ALIGNED>(p, row, sh.general);
+}
+
 }  // namespace
 }  // namespace mig
 
@@ -697,12 +1085,19 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
   const bool bf16 = dtype == MI_BF16;
   // More rows than CUs: half the threads, so that two rows share a CU and one's waits are under the
   // other's work (512 rows of 32000 bf16 logits, top-p: 65 us with 1024 threads, 60 with 512)
+  // each row decides for itself; here whether any may gain
+  const bool counted = bf16 && vocab >= SMC_FROM && vocab <= 65535 &&
+                       (how->temperature || how->temperature_all > 0.0f) &&
+                       (how->top_k || how->top_p || counts_pay(how->top_k_all, how->top_p_all, (int)vocab));
   const int threads = rows > host_cus() ? 512 : 1024;
   const int per_layer = threads * (bf16 ? 8 : 4);
   p.layers = (int)((vocab + per_layer - 1) / per_layer);
   const bool aligned = ((uintptr_t)logits & 15) == 0 && (rows == 1 || ld % (bf16 ? 8 : 4) == 0);
   auto kernel = sample_kernel<1024, true, true>;
-  if (threads == 1024)
+  if (counted)
+    kernel = threads == 1024 ? (aligned ? sample_counts_kernel<1024, true> : sample_counts_kernel<1024, false>)
+                             : (aligned ? sample_counts_kernel<512, true> : sample_counts_kernel<512, false>);
+  else if (threads == 1024)
     kernel = bf16 ? (aligned ? sample_kernel<1024, true, true> : sample_kernel<1024, true, false>)
                   : (aligned ? sample_kernel<1024, false, true> : sample_kernel<1024, false, false>);
   else

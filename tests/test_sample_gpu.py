@@ -162,6 +162,57 @@ def test_peaked_and_flat_rows(mi, dev, rows, how):
     check(mi, x.bfloat16(), u, **how)
 
 
+@pytest.mark.parametrize("rows", [1, 13, 300])
+@pytest.mark.parametrize("how", [dict(p=0.9), dict(p=0.5, low=0.2, T=0.6), dict(k=257), dict(k=1000, p=0.9, low=1e-3),
+                                 dict(k=8999, T=2.0), dict(p=0.999999, T=5.0), dict(p=0.9, T=1e-3)])
+def test_long_rows_of_bf16(mi, dev, rows, how):
+    """Rows by what their distinct logits are: a few, thousands, zeros of both signs, masked and infinite
+    ones, the smallest and largest."""
+    import torch
+
+    x, u = make(rows, 9000, "bf16", rows)
+    inf = float("inf")
+    x[1::13] = x[1::13].float().round().bfloat16()          # ties by the hundred
+    x[2::13, 17:] = -inf                                    # nearly all masked
+    x[3::13] = -inf
+    x[4::13, 8999:] = inf
+    x[5::13, 100:120] = float("nan")
+    x[6::13] = (x[6::13].float() * 2.0 ** 70).bfloat16()
+    x[7::13, 5] = 1e-30
+    x[8::13] = torch.tensor([0.0, -0.0], device="cuda").bfloat16().repeat(4500)
+    x[9::13] = (torch.arange(9000, device="cuda") - 4500 + 0x3f80).to(torch.int16).view(torch.bfloat16)  # all distinct
+    x[10::13] = (torch.arange(9000, device="cuda") // 3 + 0x3f80 - 1500).to(torch.int16).view(torch.bfloat16)
+    x[11::13] = x[11::13] - 60.0                            # none above 0
+    x[12::13, ::2] = -1.8e19                                # the lowest places but two
+    x[12::13, ::3] = -1.85e19
+    check(mi, x, u, **how)
+
+
+@pytest.mark.parametrize("V", [8191, 8192, 8193, 65535, 65536])
+@pytest.mark.parametrize("how", [dict(p=0.9), dict(k=5000, p=0.99)])
+def test_lengths_of_long_rows_of_bf16(mi, dev, V, how):
+    import torch
+
+    x, u = make(3, V + 3, "bf16", V)
+    check(mi, x[:, :V], u, **how)
+    check(mi, x[:, 1:V + 1], u, **how)
+    check(mi, x[:1, 2:V + 2], u[:1], **how)
+    check(mi, (x[:, 2:V + 2] * 0).contiguous(), u, **how)  # all alike: one counter for the whole row
+    one = torch.full((3, V), -30.0, device="cuda").bfloat16()
+    one[0, 0] = one[1, V // 2] = one[2, V - 1] = 2.0
+    check(mi, one, u, **how)
+
+
+def test_settings_of_long_rows(mi, dev):
+    """In one batch: rows without borders, greedy ones, and those with each of the borders."""
+    import torch
+
+    x, u = make(300, 10007, "bf16", 11)
+    t = lambda v, dt: torch.tensor(v, dtype=dt, device="cuda").repeat(300 // len(v))  # noqa: E731
+    check(mi, x, u, T=t((1.0, 0.0, 0.7, 1.3, 0.9), torch.float32), k=t((0, 0, 40, 256, 257, 5000), torch.int32),
+          p=t((1.0, 0.9, 0.3, 0.99), torch.float32), low=t((0.0, 0.0, 0.05), torch.float32))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_row_pitch_and_alignment(mi, dev, dtype):
     import torch
