@@ -66,13 +66,17 @@ __device__ __forceinline__ float smp_elem(const u32x4_t& v, int e) {
   else return __uint_as_float(v[e]);
 }
 
+// 16 bytes at any element: odd pitches and vocabularies put rows anywhere, and one such load takes less
+// than eight (64 rows of 50257 bf16 logits, top-p: 36 us against 57; where aligned, the same).
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
 // Elements j .. of a row of V as one vector; past the row's end -inf.
-template <bool BF16, bool ALIGNED>
+template <bool BF16>
 __device__ __forceinline__ u32x4_t smp_load(const void* row, int j, int V) {
   constexpr int EV = BF16 ? 8 : 4;
   const uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
   u32x4_t v = {none, none, none, none};
-  if (ALIGNED && j + EV <= V) return *(const u32x4_t*)((const char*)row + (int64_t)j * (BF16 ? 2 : 4));
+  if (j + EV <= V) return *(const u32x4_any_t*)((const char*)row + (int64_t)j * (BF16 ? 2 : 4));
 #pragma unroll
   for (int e = 0; e < EV; ++e) {
     if (j + e >= V) continue;
@@ -146,7 +150,7 @@ struct SampleShared {
   uint32_t ties;
 };
 
-template <int TH, bool BF16, bool ALIGNED>
+template <int TH, bool BF16>
 __device__ __forceinline__ void sample_row(const SampleParams& p, int row, SampleShared<TH / 64>& sh) {
   constexpr int EV = BF16 ? 8 : 4, WAVES = TH / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -156,7 +160,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   // layers covers it, so runs of the last waves may lie past its end (the sum stays below 2^25)
   const int first = wave * layers * 64 * EV + lane * EV;
   auto layer = [&](int i) __attribute__((always_inline)) {
-    return smp_load<BF16, ALIGNED>(x, first + 64 * EV * i, V);
+    return smp_load<BF16>(x, first + 64 * EV * i, V);
   };
   // f(i, vector) over this lane's vectors, the next one on its way; f returns whether to go on (the
   // same in all lanes)
@@ -669,10 +673,10 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   });
 }
 
-template <int TH, bool BF16, bool ALIGNED>
+template <int TH, bool BF16>
 __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
   __shared__ SampleShared<TH / 64> sh;
-  sample_row<TH, BF16, ALIGNED>(p, blockIdx.x, sh);
+  sample_row<TH, BF16>(p, blockIdx.x, sh);
 }
 
 // Long rows of bf16 logits hold few distinct ones (32000 normal ones about 2200): they are counted by
@@ -680,9 +684,9 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
 // distinct ones are weighed and all three borders lie in running sums over the list.  The second pass
 // takes each token's weight from LDS by its bits.  The answers are those of the kernel above, to the bit.
 // Normal logits, top-p 0.9, without / with it (us):
-//             8192       16384      32000 logits
-//    64 rows  16.6/15.7  22.7/17.8  35.4/23.6
-//   512 rows  22.7/19.4  34.0/25.4  60.0/38.5   (4096 logits: 15.4/16.5)
+//             8192       16384      32000      131072 logits
+//    64 rows  16.6/15.7  22.7/17.8  35.4/23.9  113/60
+//   512 rows  22.7/19.4  34.0/25.4  60.0/38.8  240/119    (4096 logits: 15.4/16.5)
 // LDS and vector instructions bound it: of a row's 17 us alone 4 go to the counting, 4 to the second
 // pass, 7 to the list and its sums.  80 KB of LDS leave room for two blocks of 512 threads on a CU.
 constexpr int SMC_LIST = 3584;          // distinct logits of a row
@@ -734,8 +738,9 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// Whether it has answered; if not (a logit without a place, too many distinct ones) nothing is written.
-template <int TH, bool ALIGNED>
+// Whether it has answered; if not (a logit without a place, too many distinct ones or
+// too many alike) nothing is written.
+template <int TH>
 __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, float T, int top_k, float top_p,
                                                float min_p, SampleCounts<TH / 64>& sh) {
   constexpr int EV = 8, WAVES = TH / 64, EACH = (SMC_LIST + TH - 1) / TH;
@@ -746,7 +751,7 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
   u32x4_t vec[4];
   auto fetch = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vec[j] = smp_load<true, ALIGNED>(x, first + 64 * EV * (i0 + j), V);
+    for (int j = 0; j < 4; ++j) vec[j] = smp_load<true>(x, first + 64 * EV * (i0 + j), V);
   };
   auto each_vector = [&](auto f) __attribute__((always_inline)) {
     for (int i0 = 0; i0 < layers; i0 += 4) {
@@ -763,6 +768,7 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
   if (tid < 32) sh.pow32[tid] = exp2(tid * 0.03125);
   if (tid == 0) sh.other = 0;
   __syncthreads();
+  uint32_t finite = 0;
   each_vector([&](int, const u32x4_t& v) __attribute__((always_inline)) {
     // the largest and the least absolute bits, zeros aside
     u16x2_t most = {0, 0}, least = {0xffff, 0xffff};
@@ -783,12 +789,18 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int k = e ? at.y : at.x;  // below 0: -inf, or too large
+        finite += k >= 0;
         if (k >= 0) atomicAdd(&sh.count[k >> 1], 1u << ((k & 1) << 4));
       }
     }
     return true;
   });
+  finite = (uint32_t)wave_sum_u64(finite);
+  if (lane == 0) sh.wave_cnt[wave] = finite;
   __syncthreads();
+  finite = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) finite += sh.wave_cnt[i];
 
   // The list, from the largest down: 256 chunks of 128 places, dealt to the waves in turn, since most
   // of them are empty and the others lie together.
@@ -816,14 +828,14 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
     const uint32_t to = (uint32_t)wave_scan_u64(sum);
     before += to - sum;
     n_list = (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
-    if (n_list == 0) {
+    if (finite == 0) {
       if (tid == 0) {
         p.tokens[row] = -1;
         if (p.probs) p.probs[row] = 0.0f;
       }
       return true;
     }
-    if (n_list > SMC_LIST) return false;
+    if (n_list == 0 || n_list > SMC_LIST) return false;
     uint64_t full = __ballot(own && lane % GROUPS == wave / 4);
     while (full) {
       const int l = __ffsll((unsigned long long)full) - 1;
@@ -871,6 +883,8 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
     total += sh.wave_sum[i];
     all_tokens += sh.wave_cnt[i];
   }
+  // A counter that ran over has lost 65536 tokens, and may have given its neighbour one.
+  if (all_tokens != finite) return false;
   // Kept: entries before `entry`, and the first `ties` tokens of it.
   uint32_t entry = n_list - 1, ties = sh.list[n_list - 1] & 0xffffu;
   if (top_k > 0 && (uint32_t)top_k < all_tokens) {
@@ -1029,8 +1043,8 @@ __host__ __device__ __forceinline__ bool counts_pay(int top_k, float top_p, int 
   return top_k > 0 && top_k < vocab ? top_k > SMP_FEW : top_p < 1.0f;
 }
 
-// Rows of at most 65535 bf16 logits.
-template <int TH, bool ALIGNED>
+// Long rows of bf16 logits.
+template <int TH>
 __global__ void __launch_bounds__(TH) sample_counts_kernel(SampleParams p) {
   __shared__ union {
     SampleCounts<TH / 64> counted;
@@ -1042,10 +1056,10 @@ __global__ void __launch_bounds__(TH) sample_counts_kernel(SampleParams p) {
   const float top_p = p.how.top_p ? p.how.top_p[row] : p.how.top_p_all;
   const float min_p = p.how.min_p ? p.how.min_p[row] : p.how.min_p_all;
   if (T > 0.0f && counts_pay(top_k, top_p, p.vocab)) {
-    if (sample_counted<TH, ALIGNED>(p, row, T, top_k, top_p, min_p, sh.counted)) return;
+    if (sample_counted<TH>(p, row, T, top_k, top_p, min_p, sh.counted)) return;
     __syncthreads();
   }
-  sample_row<TH, true, ALIGNED>(p, row, sh.general);
+  sample_row<TH, true>(p, row, sh.general);
 }
 
 }  // namespace
@@ -1083,26 +1097,18 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
   p.probs = probs;
   p.how = *how;
   const bool bf16 = dtype == MI_BF16;
-  // More rows than CUs: half the threads, so that two rows share a CU and one's waits are under the
-  // other's work (512 rows of 32000 bf16 logits, top-p: 65 us with 1024 threads, 60 with 512)
-  // each row decides for itself; here whether any may gain
-  const bool counted = bf16 && vocab >= SMC_FROM && vocab <= 65535 &&
+  // Whether any row may gain by counts; each decides for itself.
+  const bool counted = bf16 && vocab >= SMC_FROM &&
                        (how->temperature || how->temperature_all > 0.0f) &&
                        (how->top_k || how->top_p || counts_pay(how->top_k_all, how->top_p_all, (int)vocab));
-  const int threads = rows > host_cus() ? 512 : 1024;
-  const int per_layer = threads * (bf16 ? 8 : 4);
+  // More rows than CUs: half the threads, so that two rows share a CU and one's waits are under the
+  // other's work (512 rows of 32000 bf16 logits, top-p, by weights: 65 us with 1024 threads, 60 with 512)
+  const bool halved = rows > host_cus();
+  const int threads = halved ? 512 : 1024, per_layer = threads * (bf16 ? 8 : 4);
   p.layers = (int)((vocab + per_layer - 1) / per_layer);
-  const bool aligned = ((uintptr_t)logits & 15) == 0 && (rows == 1 || ld % (bf16 ? 8 : 4) == 0);
-  auto kernel = sample_kernel<1024, true, true>;
-  if (counted)
-    kernel = threads == 1024 ? (aligned ? sample_counts_kernel<1024, true> : sample_counts_kernel<1024, false>)
-                             : (aligned ? sample_counts_kernel<512, true> : sample_counts_kernel<512, false>);
-  else if (threads == 1024)
-    kernel = bf16 ? (aligned ? sample_kernel<1024, true, true> : sample_kernel<1024, true, false>)
-                  : (aligned ? sample_kernel<1024, false, true> : sample_kernel<1024, false, false>);
-  else
-    kernel = bf16 ? (aligned ? sample_kernel<512, true, true> : sample_kernel<512, true, false>)
-                  : (aligned ? sample_kernel<512, false, true> : sample_kernel<512, false, false>);
+  auto kernel = halved ? sample_kernel<512, false> : sample_kernel<1024, false>;
+  if (counted) kernel = halved ? sample_counts_kernel<512> : sample_counts_kernel<1024>;
+  else if (bf16) kernel = halved ? sample_kernel<512, true> : sample_kernel<1024, true>;
   kernel<<<(unsigned)rows, threads, 0, (hipStream_t)stream>>>(p);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MI_OK : host_fail(MI_ERR_HIP, "sample launch: %s", hipGetErrorString(e));

@@ -188,7 +188,7 @@ def test_long_rows_of_bf16(mi, dev, rows, how):
     check(mi, x, u, **how)
 
 
-@pytest.mark.parametrize("V", [8191, 8192, 8193, 65535, 65536])
+@pytest.mark.parametrize("V", [8191, 8192, 8193, 65535, 65536, 65537, 140001, 300000])
 @pytest.mark.parametrize("how", [dict(p=0.9), dict(k=5000, p=0.99)])
 def test_lengths_of_long_rows_of_bf16(mi, dev, V, how):
     import torch
@@ -198,6 +198,8 @@ def test_lengths_of_long_rows_of_bf16(mi, dev, V, how):
     check(mi, x[:, 1:V + 1], u, **how)
     check(mi, x[:1, 2:V + 2], u[:1], **how)
     check(mi, (x[:, 2:V + 2] * 0).contiguous(), u, **how)  # all alike: one counter for the whole row
+    check(mi, (x[:, 2:V + 2] * 0 + 1).contiguous(), u, **how)
+    check(mi, (x[:, 2:V + 2] * 0 + 1.0078125).contiguous(), u, **how)
     one = torch.full((3, V), -30.0, device="cuda").bfloat16()
     one[0, 0] = one[1, V // 2] = one[2, V - 1] = 2.0
     check(mi, one, u, **how)
