@@ -465,9 +465,9 @@ int mi_kv_append(void* stream, const void* q, int64_t q_t, int64_t q_h, void* q_
  * strides in elements and multiples of 8, 16-byte aligned; head_dim a multiple of 8 up to 128;
  * O may be Q with the same strides.  lse (optional, fp32 [total_q, n_heads]) receives
  * the natural-log log-sum-exp.  A row without a key gets zeros and -inf.  max_q_len and
- * max_kv_len are the host's bounds on the new and cached tokens of a sequence, from which the
- * launch is shaped: max_q_len must not be exceeded (rows past it are not computed), a
- * sequence longer than max_kv_len is right but slower.  Long sequences with few rows are
+ * max_kv_len are the host's bounds on the new and cached tokens of a sequence, which only shape
+ * the launch: a sequence past them is right but slower.  K and V of the tokens that any row of a
+ * sequence sees are finite; what the pages hold elsewhere may be anything.  Long sequences with few rows are
  * split over workgroups whose parts a second kernel joins in a fixed order; their fp32 parts
  * lie in the workspace (16-byte aligned, mi_paged_attn_workspace_size bytes, or less: fewer
  * parts, NULL: no split).  Results do not depend on timing.

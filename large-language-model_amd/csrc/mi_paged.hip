@@ -21,6 +21,7 @@ namespace {
 
 constexpr int PA_ROWS = 128;    // query rows of a workgroup, 32 for each wave
 constexpr int PA_KEYS = 64;     // keys of a block
+constexpr int PA_PIECES = 256;  // pieces of a tile's keys at most
 constexpr int PF_ROWS = 16;     // the same for few rows: one 16-row tile,
 constexpr int PF_KEYS = 32;     // of which every wave takes blocks of its own
 constexpr int PF_WAVES = 4;
@@ -729,7 +730,8 @@ __device__ __forceinline__ int pa_pieces_of(const AttnParams& p, PaTile t, int r
 // (64 sequences of 500 to 8000 keys, 372 MB: 83 us, in pieces 92 at best).  A workgroup's share lies
 // in one sequence or runs over several; only its first and its last may be cut.
 constexpr int PF_BLOCK = PF_KEYS * PF_WAVES;
-constexpr int PF_SEQS = 1024;  // sequences whose lengths a workgroup sums up
+constexpr int PF_SEQS = 1024;   // sequences whose lengths a workgroup sums up
+constexpr int PF_SHARES = 1024;  // shares of a KV head, all of which one sequence may be cut into
 
 // First block of workgroup w's share of n blocks.
 __device__ __forceinline__ uint32_t pf_share(uint32_t n, uint32_t w, uint32_t of) {
@@ -805,20 +807,26 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
 
 // Joins n parts of one row, part i at at(i): o = sum 2^(lse_i - max) o_i over the sum of the weights.  A
 // workgroup: 32 lanes read a part's components, eight parts at a time and eight such in flight; their sums
-// are joined in a fixed order.  n <= 256.
-template <class At>
+// are joined in a fixed order.
+template <int MOST, class At>  // n <= MOST
 __device__ __forceinline__ void pa_join(const AttnParams& p, int64_t row, int head, int n, At at) {
   __shared__ f32x4_t part[8][32];
-  __shared__ float weight[256], wave_max[4], slice_sum[8];
+  __shared__ float weight[MOST], wave_max[4], slice_sum[8];
   const int tid = threadIdx.x, slice = tid >> 5, l32 = tid & 31;
-  const float mine = tid < n ? p.part_lse[at(tid)] : -INFINITY;
-  float mx = mine;
+  float mine[MOST / 256], mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < MOST / 256; ++j) {
+    mine[j] = tid + 256 * j < n ? p.part_lse[at(tid + 256 * j)] : -INFINITY;
+    mx = fmaxf(mx, mine[j]);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
   if ((tid & 63) == 0) wave_max[tid >> 6] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-  weight[tid] = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - mx);
+#pragma unroll
+  for (int j = 0; j < MOST / 256; ++j)
+    weight[tid + 256 * j] = mine[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine[j] - mx);
   __syncthreads();
   const int c = 4 * l32;
   f32x4_t acc = {0, 0, 0, 0};
@@ -861,7 +869,7 @@ __global__ void __launch_bounds__(256) paged_attn_share_join_kernel(AttnParams p
     if (n == 1) return;
     k0 = pf_share(total, w0, p.share) != first;  // its last one, not its first
   }
-  pa_join(p, s, head, n, [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0 ? k0 : 0)) * p.n_heads + head; });
+  pa_join<PF_SHARES>(p, s, head, n, [&](int i) { return (int64_t)(2 * (w0 + i) + (i == 0 ? k0 : 0)) * p.n_heads + head; });
 }
 
 // The pieces of the rows that have more than one: a workgroup a row.
@@ -873,7 +881,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnParams p) {
   const int n = pa_pieces_of(p, t, row, head);
   if (n < 2) return;
   const int64_t pitch = (int64_t)p.pv.total_q * p.n_heads;
-  pa_join(p, row, head, n, [&](int i) { return i * pitch + at; });
+  pa_join<PA_PIECES>(p, row, head, n, [&](int i) { return i * pitch + at; });
 }
 
 // The same for up to eight pieces of many rows: a workgroup a token, 32 lanes a head, all pieces' loads in flight.
@@ -936,6 +944,7 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
                bool one_each, int cus) {
   PaPlan pl;
   const int64_t g = n_heads / n_kv, q = std::max<int64_t>(1, std::min(max_q, total_q));
+  max_kv = std::min<int64_t>(max_kv, INT32_MAX);
   pl.few = q * g <= PF_ROWS;
   pl.tile_shift = pl.few ? 4 : 7;
   const int64_t rows = int64_t{1} << pl.tile_shift;
@@ -944,10 +953,11 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   const int64_t want = ((pl.few ? 1 : 3) * (int64_t)cus + units - 1) / units;
   pl.min_piece = pl.few ? (max_kv <= 512 ? 512 : 128) : 256;
   const int64_t most = (max_kv + pl.min_piece - 1) / pl.min_piece;
-  pl.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 256}));
+  pl.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, PA_PIECES}));
   // two workgroups on a CU, three of 64 components
   pl.share = one_each && g <= PF_ROWS && n_seqs > 1 && n_seqs <= PF_SEQS && max_kv > 1024 * (int64_t)pl.pieces
-                 ? (int)std::max<int64_t>(1, (d <= 64 ? 3 : 2) * (int64_t)cus / n_kv) : 0;
+                 ? (int)std::max<int64_t>(1, std::min<int64_t>((d <= 64 ? 3 : 2) * (int64_t)cus / n_kv, PF_SHARES))
+                 : 0;
   return pl;
 }
 
@@ -961,6 +971,7 @@ extern "C" {
 size_t mi_paged_attn_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t n_seqs, int64_t total_q,
                                     int64_t max_q_len, int64_t max_kv_len) {
   if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || head_dim < 1 || n_seqs < 1 || total_q < 1) return 0;
+  if (n_seqs > INT32_MAX || total_q > INT32_MAX / n_heads) return 0;  // refused by the call
   // CUs of the current device; without one, those of an MI355X
   const PaPlan plan = pa_plan(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len,
                               total_q == n_seqs && max_q_len == 1, host_cus());
@@ -973,7 +984,7 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   int st = check_paged(cache, seqs);
   if (st != MI_OK) return st;
   if (n_heads < 0 || max_q_len < 0 || max_kv_len < 0) return host_fail(MI_ERR_SHAPE, "negative size");
-  if (seqs->n_seqs == 0 || seqs->total_q == 0 || n_heads == 0 || max_q_len == 0) return MI_OK;
+  if (seqs->n_seqs == 0 || seqs->total_q == 0 || n_heads == 0) return MI_OK;
   if (cache->n_kv < 1 || n_heads % cache->n_kv || n_heads > 65536)
     return host_fail(MI_ERR_SHAPE, "n_heads=%lld is no multiple of n_kv=%lld", (long long)n_heads,
                      (long long)cache->n_kv);
@@ -989,11 +1000,12 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
     return host_fail(MI_ERR_LD, "a stride of O is shorter than a row of %lld", (long long)d);
   if (Q == O && ((rows > 1 && q_t != o_t) || (n_heads > 1 && q_h != o_h)))
     return host_fail(MI_ERR_UNSUPPORTED, "in place needs the same strides of Q and O");
-  if (!(scale > 0.0f) || !isfinite(scale)) return host_fail(MI_ERR_UNSUPPORTED, "scale must be positive and finite");
+  if (!(scale > 0.0f) || !isfinite(scale * 1.4426950408889634f)) return host_fail(MI_ERR_UNSUPPORTED, "scale must be positive and finite");
   if (rows * n_heads > INT32_MAX) return host_fail(MI_ERR_SHAPE, "total_q * n_heads exceeds 2^31-1");
   st = host_device();
   if (st != MI_OK) return st;
   PaPlan plan = pa_plan(n_heads, cache->n_kv, d, seqs->n_seqs, rows, max_q_len, max_kv_len, !seqs->q_start, host_cus());
+  if (seqs->n_seqs * (seqs->max_pages * cache->page_size / PF_BLOCK + 1) > INT32_MAX) plan.share = 0;  // its sums
   // as many pieces as the workspace holds
   const int64_t piece_bytes = rows * n_heads * (d + 1) * 4;
   if (!workspace) plan.pieces = 1;

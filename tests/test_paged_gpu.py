@@ -180,6 +180,22 @@ def test_decode_many_uneven(mi, dev, S, nH, nKV, d, P):
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
 
 
+@pytest.mark.parametrize("kv,nKV,d", [([140000, 5], 1, 128), ([140001, 140000], 1, 64), ([7, 66000], 2, 40)])
+def test_one_sequence_cut_by_all_workgroups(mi, dev, kv, nKV, d):
+    """Few KV heads and two sequences, one of which holds most keys: its row is joined from several hundred
+    shares. A share sums a thousand keys at most and the join as many parts, 2^11 * 2^-24 together."""
+    b = Batch([1, 1], kv, 64, 2, nKV, d, seed=d, one_each=True)
+    ref = b.reference()
+    check(*run(mi, b), ref)
+
+
+@pytest.mark.parametrize("most", [0, 1, 3, 10 ** 6])
+@pytest.mark.parametrize("nH,nKV,d", [(8, 2, 128), (4, 4, 64)])
+def test_bounds_only_shape_the_launch(mi, dev, most, nH, nKV, d):
+    b = Batch([5, 300, 0, 1], [5, 700, 40, 1500], 16, nH, nKV, d, seed=most % 97)
+    check(*run(mi, b, max_q_len=most, max_kv_len=most), b.reference())
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_long_page_tables(mi, dev, d):
     """More pages in a workgroup's keys than it looks up at a time (pages of one token)."""
