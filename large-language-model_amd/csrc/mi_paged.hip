@@ -128,266 +128,6 @@ struct PaLds {
   }
 };
 
-template <int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_attn_kernel(AttnParams p) {
-  using L = PaLds<D>;
-  constexpr int NS = D / 16, NC = D / 32, STAGE = 2 * L::BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  const uint32_t lds0 = lds_addr(smem);
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int h32 = lane >> 5, l32 = lane & 31;
-
-  // Workgroup b runs on XCD b mod 8.  With the KV heads innermost an XCD's L2 holds the keys of few of
-  // them, which the row tiles of a sequence read at about the same time; the last tiles, which see the
-  // most keys, come first.
-  const int rest = uniform(blockIdx.x / p.n_kv), kvh = uniform(blockIdx.x - rest * p.n_kv);
-  const int piece = uniform(rest / p.tiles), x = uniform(p.tiles - 1 - (rest - piece * p.tiles));
-  const PaTile t = pa_tile(p, x);
-  if (t.s < 0) return;
-  const int end = t.end(p), plen = pa_piece(p, end);
-  if (piece > 0 && (int64_t)piece * plen >= end) return;
-  const int k_begin = piece * plen, k_end = k_begin + min(plen, end - k_begin);
-  const bool whole = plen >= end;
-
-  // this lane's row; rows past the sequence's last one repeat it and are not stored
-  const int n_packed = min(t.n * p.group - t.first, PA_ROWS);
-  const bool wave_has_rows = 32 * wave < n_packed;
-  const int pr = t.first + min(32 * wave + l32, n_packed - 1);
-  const int token = pr / p.group, head = kvh * p.group + pr - token * p.group;
-  const int lim = t.limit(p, token);
-  // the wave's rows see at least lim_lo and at most lim_hi keys
-  const int lim_lo = t.limit(p, (t.first + min(32 * wave, n_packed - 1)) / p.group);
-  const int lim_hi = t.limit(p, (t.first + min(32 * wave + 31, n_packed - 1)) / p.group);
-
-  u32x4_t qf[NS];
-  {
-    const uint16_t* qr = p.q + (int64_t)(t.q0 + token) * p.q_t + (int64_t)head * p.q_h;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int c = 8 * (2 * s + h32);
-      qf[s] = c < p.d ? *(const u32x4_t*)(qr + c) : u32x4_t{0, 0, 0, 0};
-    }
-  }
-
-  // DMA: wave w brings rows 16w .. 16w+15 of a block; in load u lane l brings a chunk of row
-  // 16w + RPB*u + l/NCH.
-  const uint16_t* kbase = p.k + (int64_t)kvh * p.pv.head_stride;
-  const uint16_t* vbase = p.v + (int64_t)kvh * p.pv.head_stride;
-  int page_next = -1;   // page of key `lane` of the next block to be issued, read a block ahead of its use
-  uint64_t seen_next = 0;  // keys of the block issued last that exist
-  auto look_up = [&](int base) __attribute__((always_inline)) {
-    const int pos = base + lane;
-    page_next = pos < k_end ? p.pv.pages[(int64_t)t.s * p.pv.pages_ld + (pos >> p.pv.page_shift)] : -1;
-  };
-  // The wave's 16 rows lie in one page where pages are of 16 tokens or more: a scalar base and these offsets.
-  const bool even = p.pv.page_shift >= 4 && p.d == D && p.pv.slot_stride <= (1 << 24);
-  uint32_t k_off[L::NU], v_off[L::NU];
-#pragma unroll
-  for (int u = 0; u < L::NU; ++u) {
-    const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
-    k_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::k_pos(r, at));
-    v_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::v_pos(r, at));
-  }
-  auto to_lds = [&](const uint16_t* src, uint32_t dst) __attribute__((always_inline)) {
-    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(uintptr_t)src,
-                                     (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0, 0);
-  };
-  // asks for the block at `base`, whose pages have been looked up
-  auto issue = [&](int base, int stage) __attribute__((always_inline)) {
-    const bool there = (uint32_t)page_next < (uint32_t)p.pv.num_pages;
-    const int mask = (1 << p.pv.page_shift) - 1;
-    const uint32_t dst = lds0 + (uint32_t)(stage * STAGE + wave * L::NU * 1024);
-    seen_next = __ballot(there);
-    if (even && seen_next == ~uint64_t{0}) {
-      const int64_t at = __builtin_amdgcn_readlane(page_next, 16 * wave) * p.pv.page_stride +
-                         ((base + 16 * wave) & mask) * p.pv.slot_stride;
-#pragma unroll
-      for (int u = 0; u < L::NU; ++u) {
-        to_lds(kbase + at + k_off[u], dst + u * 1024);
-        to_lds(vbase + at + v_off[u], dst + u * 1024 + L::BYTES);
-      }
-      return;
-    }
-    const int64_t row_off = there ? page_next * p.pv.page_stride + ((base + lane) & mask) * p.pv.slot_stride : -1;
-#pragma unroll
-    for (int u = 0; u < L::NU; ++u) {
-      const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
-      const int64_t off = __shfl(row_off, r, 64);
-      const int kc = 8 * L::k_pos(r, at), vc = 8 * L::v_pos(r, at);
-      to_lds(off >= 0 && kc < p.d ? kbase + off + kc : (const uint16_t*)pa_zero, dst + u * 1024);
-      to_lds(off >= 0 && vc < p.d ? vbase + off + vc : (const uint16_t*)pa_zero, dst + u * 1024 + L::BYTES);
-    }
-  };
-
-  // the row of a 32-key half that a lane reads: bits 2 and 3 of the key swapped, so that the scores of a
-  // lane are, in order, the 8-key runs that the second operand of P V takes
-  const int k_row = (l32 & ~0xC) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
-  uint32_t v_rd[NC];
-  {
-    const int g = lane >> 4, jj = lane & 15;
-    const int krb = 8 * (g >> 1) + (jj >> 2);
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int col = 32 * c + 16 * (g & 1) + 4 * (jj & 3);
-      v_rd[c] = (uint32_t)(L::BYTES + krb * L::ROW + 16 * L::v_pos(krb, col >> 3) + (col & 7) * 2);
-    }
-  }
-
-  f32x16_t o[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
-  float m_run = -INFINITY, l_run = 0.0f;
-  const float sl2 = p.scale_log2;
-
-  // One 64-key block; `seen`: the keys that this lane's row sees, of which none is missing in any row of the
-  // wave unless `masked`.
-  auto block = [&](uint32_t st, uint64_t seen, bool masked) __attribute__((always_inline)) {
-    f32x16_t sc[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[kb][e] = 0.0f;
-    u32x4_t kf[NS][2];
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        kf[s][kb] = *(const lds_u32x4_t*)(uintptr_t)(st + (uint32_t)((32 * kb + k_row) * L::ROW +
-                                                                     16 * L::k_pos(k_row, 2 * s + h32)));
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf[s][kb]),
-                                                        __builtin_bit_cast(bf16x8_t, qf[s]), sc[kb], 0, 0, 0);
-    // sc[kb][4q + e] is key 32kb + 8*h32 + 16(q>>1) + 4(q&1) + e
-    if (masked) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const uint32_t bits = (uint32_t)(seen >> (32 * kb)) >> (8 * h32);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 16 * ((i >> 2) >> 1) + 4 * ((i >> 2) & 1) + (i & 3);
-          sc[kb][i] = (bits >> at) & 1 ? sc[kb][i] : -INFINITY;
-        }
-      }
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    // a row keeps its reference maximum until a block raises it by more than PA_TAU
-    const float m_old = m_run;
-    const bool fresh = m_old == -INFINITY, raise = !fresh && (mx - m_old) * sl2 > PA_TAU;
-    const float m_ref = fresh || raise ? mx : m_old;
-    if (__any(raise)) {
-      const float alpha = raise ? __builtin_amdgcn_exp2f((m_old - m_ref) * sl2) : 1.0f;
-      l_run *= alpha;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[c][e] *= alpha;
-    }
-    m_run = m_ref;
-    const float nmc = m_ref == -INFINITY ? 0.0f : -m_ref * sl2;
-    float sum = 0.0f;
-    u32x4_t pf[4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int kb = ks >> 1, base = 8 * (ks & 1);
-#pragma unroll
-      for (int w2 = 0; w2 < 4; ++w2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2], sl2, nmc));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2 + 1], sl2, nmc));
-        sum += e0 + e1;
-        pf[ks][w2] = pack_bf16x2(e0, e1);
-      }
-    }
-    l_run += sum;
-    static_for<4>([&](auto ks_c) __attribute__((always_inline)) {
-      constexpr int ks = decltype(ks_c)::value;
-      u32x4_t vf[NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        static_for<2>([&](auto t_c) __attribute__((always_inline)) {
-          constexpr int tt = decltype(t_c)::value;
-          u32x2_t w2 = {0u, 0u};
-#if defined(__HIP_DEVICE_COMPILE__)
-          // inline asm: the builtin would also wait for the loads into LDS that are in flight
-          asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
-                       : "=v"(w2)
-                       : "v"(st + v_rd[c]), "i"((16 * ks + 4 * tt) * L::ROW));
-#endif
-          vf[c][2 * tt] = w2[0];
-          vf[c][2 * tt + 1] = w2[1];
-        });
-      }
-      // the results are valid after lgkmcnt(0), which the compiler does not know of
-      __builtin_amdgcn_s_waitcnt(0xC07F);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
-                                                       __builtin_bit_cast(bf16x8_t, pf[ks]), o[c], 0, 0, 0);
-    });
-  };
-
-  const int n_blocks = uniform((k_end - k_begin + PA_KEYS - 1) / PA_KEYS);
-  if (n_blocks > 0) {
-    look_up(k_begin);
-    issue(k_begin, 0);
-    look_up(k_begin + PA_KEYS);
-  }
-  for (int j = 0; j < n_blocks; ++j) {
-    const uint64_t seen = seen_next;
-    const int base = k_begin + j * PA_KEYS;
-    wait_vmcnt<0>();     // this wave's share of block j has landed, and the pages of block j + 1
-    lds_ring_barrier();  // and everyone's; and block j - 1 has been read
-    if (j + 1 < n_blocks) {
-      issue(base + PA_KEYS, (j + 1) & 1);
-      look_up(base + 2 * PA_KEYS);
-    }
-    const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
-    if (!wave_has_rows || base >= lim_hi) continue;
-    const bool masked = base + PA_KEYS > lim_lo || seen != ~uint64_t{0};
-    const int room = lim - base;
-    block(st, room >= 64 ? seen : room <= 0 ? 0 : seen & ((uint64_t{1} << room) - 1), masked);
-  }
-
-  if (!wave_has_rows || 32 * wave + l32 >= n_packed) return;
-  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-  const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-  const int64_t row = t.q0 + token;
-  const float lse2 = l_tot == 0.0f ? -INFINITY : m_run * sl2 + __log2f(l_tot);
-  if (whole) {
-    uint16_t* out = p.o + row * p.o_t + (int64_t)head * p.o_h;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (32 * c + 8 * q < p.d)
-          *(u32x2_t*)(out + 32 * c + 8 * q + 4 * h32) =
-              u32x2_t{pack_bf16x2(o[c][4 * q] * inv, o[c][4 * q + 1] * inv),
-                      pack_bf16x2(o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv)};
-    if (p.lse && h32 == 0) p.lse[row * p.n_heads + head] = lse2 * 0.69314718055994531f;
-  } else {
-    const int64_t at = ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head;
-    float* out = p.part_o + at * p.d;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (32 * c + 8 * q < p.d)
-          *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{o[c][4 * q] * inv, o[c][4 * q + 1] * inv,
-                                                                 o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv};
-    if (h32 == 0) p.part_lse[at] = lse2;
-  }
-}
-
 // Few rows (decode): 16 rows of one (sequence, KV head) for a workgroup, bound by the keys and values that
 // it streams.  Every wave takes 32-key blocks of its own, so nothing waits at a barrier until the waves'
 // sums are joined at the end: K of the next block comes into registers, where the product wants it, V of
@@ -681,6 +421,276 @@ __device__ __forceinline__ void pf_segment(const AttnParams& p, PfShared<D>& lds
   }
 }
 
+template <int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_attn_kernel(AttnParams p) {
+  using L = PaLds<D>;
+  constexpr int NS = D / 16, NC = D / 32, STAGE = 2 * L::BYTES;
+  __shared__ union {
+    __attribute__((aligned(16))) char ring[2 * STAGE];
+    PfShared<D> few;
+  } lds;
+  const uint32_t lds0 = lds_addr(lds.ring);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int h32 = lane >> 5, l32 = lane & 31;
+
+  // Workgroup b runs on XCD b mod 8.  With the KV heads innermost an XCD's L2 holds the keys of few of
+  // them, which the row tiles of a sequence read at about the same time; the last tiles, which see the
+  // most keys, come first.
+  const int rest = uniform(blockIdx.x / p.n_kv), kvh = uniform(blockIdx.x - rest * p.n_kv);
+  const int piece = uniform(rest / p.tiles), x = uniform(p.tiles - 1 - (rest - piece * p.tiles));
+  const PaTile t = pa_tile(p, x);
+  if (t.s < 0) return;
+  const int end = t.end(p), plen = pa_piece(p, end);
+  if (piece > 0 && (int64_t)piece * plen >= end) return;
+  const int k_begin = piece * plen, k_end = k_begin + min(plen, end - k_begin);
+  const bool whole = plen >= end;
+
+  // this lane's row; rows past the sequence's last one repeat it and are not stored
+  const int n_packed = min(t.n * p.group - t.first, PA_ROWS);
+  // Decode rows beside prompts, and the ends of those: all four waves at one row tile (a prompt of 500 and 63
+  // rows over 4000 keys each: 114 us, 121 without; with 12 heads of 64 and 30 uneven rows 38 and 41.5).
+  if (n_packed <= PF_ROWS) {
+    pf_segment<D>(p, lds.few, t, kvh, k_begin, k_end, whole,
+                  [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
+    return;
+  }
+  const bool wave_has_rows = 32 * wave < n_packed;
+  const int pr = t.first + min(32 * wave + l32, n_packed - 1);
+  const int token = pr / p.group, head = kvh * p.group + pr - token * p.group;
+  const int lim = t.limit(p, token);
+  // the wave's rows see at least lim_lo and at most lim_hi keys
+  const int lim_lo = t.limit(p, (t.first + min(32 * wave, n_packed - 1)) / p.group);
+  const int lim_hi = t.limit(p, (t.first + min(32 * wave + 31, n_packed - 1)) / p.group);
+
+  u32x4_t qf[NS];
+  {
+    const uint16_t* qr = p.q + (int64_t)(t.q0 + token) * p.q_t + (int64_t)head * p.q_h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int c = 8 * (2 * s + h32);
+      qf[s] = c < p.d ? *(const u32x4_t*)(qr + c) : u32x4_t{0, 0, 0, 0};
+    }
+  }
+
+  // DMA: wave w brings rows 16w .. 16w+15 of a block; in load u lane l brings a chunk of row
+  // 16w + RPB*u + l/NCH.
+  const uint16_t* kbase = p.k + (int64_t)kvh * p.pv.head_stride;
+  const uint16_t* vbase = p.v + (int64_t)kvh * p.pv.head_stride;
+  int page_next = -1;   // page of key `lane` of the next block to be issued, read a block ahead of its use
+  uint64_t seen_next = 0;  // keys of the block issued last that exist
+  auto look_up = [&](int base) __attribute__((always_inline)) {
+    const int pos = base + lane;
+    page_next = pos < k_end ? p.pv.pages[(int64_t)t.s * p.pv.pages_ld + (pos >> p.pv.page_shift)] : -1;
+  };
+  // The wave's 16 rows lie in one page where pages are of 16 tokens or more: a scalar base and these offsets.
+  const bool even = p.pv.page_shift >= 4 && p.d == D && p.pv.slot_stride <= (1 << 24);
+  uint32_t k_off[L::NU], v_off[L::NU];
+#pragma unroll
+  for (int u = 0; u < L::NU; ++u) {
+    const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
+    k_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::k_pos(r, at));
+    v_off[u] = (uint32_t)((r & 15) * p.pv.slot_stride + 8 * L::v_pos(r, at));
+  }
+  auto to_lds = [&](const uint16_t* src, uint32_t dst) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(uintptr_t)src,
+                                     (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0, 0);
+  };
+  // asks for the block at `base`, whose pages have been looked up
+  auto issue = [&](int base, int stage) __attribute__((always_inline)) {
+    const bool there = (uint32_t)page_next < (uint32_t)p.pv.num_pages;
+    const int mask = (1 << p.pv.page_shift) - 1;
+    const uint32_t dst = lds0 + (uint32_t)(stage * STAGE + wave * L::NU * 1024);
+    seen_next = __ballot(there);
+    if (even && seen_next == ~uint64_t{0}) {
+      const int64_t at = __builtin_amdgcn_readlane(page_next, 16 * wave) * p.pv.page_stride +
+                         ((base + 16 * wave) & mask) * p.pv.slot_stride;
+#pragma unroll
+      for (int u = 0; u < L::NU; ++u) {
+        to_lds(kbase + at + k_off[u], dst + u * 1024);
+        to_lds(vbase + at + v_off[u], dst + u * 1024 + L::BYTES);
+      }
+      return;
+    }
+    const int64_t row_off = there ? page_next * p.pv.page_stride + ((base + lane) & mask) * p.pv.slot_stride : -1;
+#pragma unroll
+    for (int u = 0; u < L::NU; ++u) {
+      const int r = 16 * wave + L::RPB * u + lane / L::NCH, at = lane % L::NCH;
+      const int64_t off = __shfl(row_off, r, 64);
+      const int kc = 8 * L::k_pos(r, at), vc = 8 * L::v_pos(r, at);
+      to_lds(off >= 0 && kc < p.d ? kbase + off + kc : (const uint16_t*)pa_zero, dst + u * 1024);
+      to_lds(off >= 0 && vc < p.d ? vbase + off + vc : (const uint16_t*)pa_zero, dst + u * 1024 + L::BYTES);
+    }
+  };
+
+  // the row of a 32-key half that a lane reads: bits 2 and 3 of the key swapped, so that the scores of a
+  // lane are, in order, the 8-key runs that the second operand of P V takes
+  const int k_row = (l32 & ~0xC) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);
+  uint32_t v_rd[NC];
+  {
+    const int g = lane >> 4, jj = lane & 15;
+    const int krb = 8 * (g >> 1) + (jj >> 2);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = 32 * c + 16 * (g & 1) + 4 * (jj & 3);
+      v_rd[c] = (uint32_t)(L::BYTES + krb * L::ROW + 16 * L::v_pos(krb, col >> 3) + (col & 7) * 2);
+    }
+  }
+
+  f32x16_t o[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+  const float sl2 = p.scale_log2;
+
+  // One 64-key block; `seen`: the keys that this lane's row sees, of which none is missing in any row of the
+  // wave unless `masked`.
+  auto block = [&](uint32_t st, uint64_t seen, bool masked) __attribute__((always_inline)) {
+    f32x16_t sc[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[kb][e] = 0.0f;
+    u32x4_t kf[NS][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        kf[s][kb] = *(const lds_u32x4_t*)(uintptr_t)(st + (uint32_t)((32 * kb + k_row) * L::ROW +
+                                                                     16 * L::k_pos(k_row, 2 * s + h32)));
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf[s][kb]),
+                                                        __builtin_bit_cast(bf16x8_t, qf[s]), sc[kb], 0, 0, 0);
+    // sc[kb][4q + e] is key 32kb + 8*h32 + 16(q>>1) + 4(q&1) + e
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const uint32_t bits = (uint32_t)(seen >> (32 * kb)) >> (8 * h32);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 16 * ((i >> 2) >> 1) + 4 * ((i >> 2) & 1) + (i & 3);
+          sc[kb][i] = (bits >> at) & 1 ? sc[kb][i] : -INFINITY;
+        }
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // a row keeps its reference maximum until a block raises it by more than PA_TAU
+    const float m_old = m_run;
+    const bool fresh = m_old == -INFINITY, raise = !fresh && (mx - m_old) * sl2 > PA_TAU;
+    const float m_ref = fresh || raise ? mx : m_old;
+    if (__any(raise)) {
+      const float alpha = raise ? __builtin_amdgcn_exp2f((m_old - m_ref) * sl2) : 1.0f;
+      l_run *= alpha;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[c][e] *= alpha;
+    }
+    m_run = m_ref;
+    const float nmc = m_ref == -INFINITY ? 0.0f : -m_ref * sl2;
+    float sum = 0.0f;
+    u32x4_t pf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const int kb = ks >> 1, base = 8 * (ks & 1);
+#pragma unroll
+      for (int w2 = 0; w2 < 4; ++w2) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2], sl2, nmc));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2 + 1], sl2, nmc));
+        sum += e0 + e1;
+        pf[ks][w2] = pack_bf16x2(e0, e1);
+      }
+    }
+    l_run += sum;
+    static_for<4>([&](auto ks_c) __attribute__((always_inline)) {
+      constexpr int ks = decltype(ks_c)::value;
+      u32x4_t vf[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        static_for<2>([&](auto t_c) __attribute__((always_inline)) {
+          constexpr int tt = decltype(t_c)::value;
+          u32x2_t w2 = {0u, 0u};
+#if defined(__HIP_DEVICE_COMPILE__)
+          // inline asm: the builtin would also wait for the loads into LDS that are in flight
+          asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
+                       : "=v"(w2)
+                       : "v"(st + v_rd[c]), "i"((16 * ks + 4 * tt) * L::ROW));
+#endif
+          vf[c][2 * tt] = w2[0];
+          vf[c][2 * tt + 1] = w2[1];
+        });
+      }
+      // the results are valid after lgkmcnt(0), which the compiler does not know of
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
+                                                       __builtin_bit_cast(bf16x8_t, pf[ks]), o[c], 0, 0, 0);
+    });
+  };
+
+  const int n_blocks = uniform((k_end - k_begin + PA_KEYS - 1) / PA_KEYS);
+  if (n_blocks > 0) {
+    look_up(k_begin);
+    issue(k_begin, 0);
+    look_up(k_begin + PA_KEYS);
+  }
+  for (int j = 0; j < n_blocks; ++j) {
+    const uint64_t seen = seen_next;
+    const int base = k_begin + j * PA_KEYS;
+    wait_vmcnt<0>();     // this wave's share of block j has landed, and the pages of block j + 1
+    lds_ring_barrier();  // and everyone's; and block j - 1 has been read
+    if (j + 1 < n_blocks) {
+      issue(base + PA_KEYS, (j + 1) & 1);
+      look_up(base + 2 * PA_KEYS);
+    }
+    const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
+    if (!wave_has_rows || base >= lim_hi) continue;
+    const bool masked = base + PA_KEYS > lim_lo || seen != ~uint64_t{0};
+    const int room = lim - base;
+    block(st, room >= 64 ? seen : room <= 0 ? 0 : seen & ((uint64_t{1} << room) - 1), masked);
+  }
+
+  if (!wave_has_rows || 32 * wave + l32 >= n_packed) return;
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+  const int64_t row = t.q0 + token;
+  const float lse2 = l_tot == 0.0f ? -INFINITY : m_run * sl2 + __log2f(l_tot);
+  if (whole) {
+    uint16_t* out = p.o + row * p.o_t + (int64_t)head * p.o_h;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * c + 8 * q < p.d)
+          *(u32x2_t*)(out + 32 * c + 8 * q + 4 * h32) =
+              u32x2_t{pack_bf16x2(o[c][4 * q] * inv, o[c][4 * q + 1] * inv),
+                      pack_bf16x2(o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv)};
+    if (p.lse && h32 == 0) p.lse[row * p.n_heads + head] = lse2 * 0.69314718055994531f;
+  } else {
+    const int64_t at = ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head;
+    float* out = p.part_o + at * p.d;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * c + 8 * q < p.d)
+          *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{o[c][4 * q] * inv, o[c][4 * q + 1] * inv,
+                                                                 o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv};
+    if (h32 == 0) p.part_lse[at] = lse2;
+  }
+}
+
 // A tile's keys in pieces, each a workgroup's.
 template <int D>
 __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
@@ -938,8 +948,10 @@ struct PaPlan {
 // and a join 10.5); else a workgroup for each CU, of 128 keys at least (one sequence of 32768: 23.9 us,
 // in twice as many pieces 29); where those pieces are long and the sequences several, even shares (64 of
 // up to 8000: 115 us in pieces, 83 in shares; 64 of up to 1000: 19 and 24).
-// Many rows: pieces of 256 keys at least until there are three workgroups for each CU, of two that fit
-// (16 sequences of up to 333 rows over 2500 keys, 12 heads of 64: 43 us with two, 36 with three).
+// Many rows: pieces of 512 keys at least until there are four workgroups for each CU, of two that fit (4
+// chunks of up to 1024 rows over 4095 keys: 65 us, 70 with three of 256; 8 of 700 over 1400: 40 and 50;
+// 4096 rows over 8192: 238 and 251; five and more, or a shorter least piece, cost more in joins).  Where
+// that leaves CUs empty, 256 or 128 (16 of 16 rows over 2000: 19 us, 24 of 512; 8 rows over 4000: 12.5, 20).
 PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t total_q, int64_t max_q, int64_t max_kv,
                bool one_each, int cus) {
   PaPlan pl;
@@ -950,8 +962,9 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   const int64_t rows = int64_t{1} << pl.tile_shift;
   pl.tiles = one_each ? n_seqs * ((g + rows - 1) / rows) : n_seqs + total_q * g / rows;
   const int64_t units = std::max<int64_t>(1, std::min(pl.tiles, n_seqs * ((q * g + rows - 1) / rows)) * n_kv);
-  const int64_t want = ((pl.few ? 1 : 3) * (int64_t)cus + units - 1) / units;
-  pl.min_piece = pl.few ? (max_kv <= 512 ? 512 : 128) : 256;
+  const int64_t want = ((pl.few ? 1 : 4) * (int64_t)cus + units - 1) / units;
+  pl.min_piece = pl.few ? (max_kv <= 512 ? 512 : 128) : 512;
+  if (!pl.few && units * ((max_kv + 511) / 512) <= cus) pl.min_piece = units * ((max_kv + 255) / 256) <= cus / 2 ? 128 : 256;
   const int64_t most = (max_kv + pl.min_piece - 1) / pl.min_piece;
   pl.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, PA_PIECES}));
   // two workgroups on a CU, three of 64 components
