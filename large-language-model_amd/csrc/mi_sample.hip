@@ -190,10 +190,22 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
 
   // largest and smallest logit above -inf (NaN is neither)
   float mx = -INFINITY, mn = INFINITY;
-  each([&](float v) __attribute__((always_inline)) {
-    mx = fmaxf(mx, v);
-    mn = fminf(mn, v > -INFINITY ? v : INFINITY);
-  });
+  for (int i0 = 0; i0 < layers; i0 += 4) {  // four vectors on their way: this pass waits for memory
+    u32x4_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j < layers) v[j] = layer(i0 + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j >= layers) break;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const float l = smp_elem<BF16>(v[j], e);
+        mx = fmaxf(mx, l);
+        mn = fminf(mn, l > -INFINITY ? l : INFINITY);
+      }
+    }
+  }
   const float lane_mx = mx;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
