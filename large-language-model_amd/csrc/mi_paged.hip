@@ -948,10 +948,11 @@ struct PaPlan {
 // and a join 10.5); else a workgroup for each CU, of 128 keys at least (one sequence of 32768: 23.9 us,
 // in twice as many pieces 29); where those pieces are long and the sequences several, even shares (64 of
 // up to 8000: 115 us in pieces, 83 in shares; 64 of up to 1000: 19 and 24).
-// Many rows: pieces of 512 keys at least until there are four workgroups for each CU, of two that fit (4
-// chunks of up to 1024 rows over 4095 keys: 65 us, 70 with three of 256; 8 of 700 over 1400: 40 and 50;
-// 4096 rows over 8192: 238 and 251; five and more, or a shorter least piece, cost more in joins).  Where
-// that leaves CUs empty, 256 or 128 (16 of 16 rows over 2000: 19 us, 24 of 512; 8 rows over 4000: 12.5, 20).
+// Many rows: pieces of 512 keys at least until there are two workgroups for each CU, which fit at once; four
+// where the sequences are eight or more, of which some are short (4 chunks of up to 1024 rows over 4095
+// keys: 59 us, with four 65; 3 of 500 over 9000: 81 and 88; 16 of up to 333 over 2500: 55 with two, 49; 32 of
+// 64 over 6000: 71 and 62).  Shorter ones cost more in joins (8 of 700 over 1400: 50 us of 256, 40).
+// Where that leaves CUs empty, 256 or 128 (16 of 16 rows over 2000: 19 us, 24 of 512; 8 rows over 4000: 12.5, 20).
 PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t total_q, int64_t max_q, int64_t max_kv,
                bool one_each, int cus) {
   PaPlan pl;
@@ -962,7 +963,7 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   const int64_t rows = int64_t{1} << pl.tile_shift;
   pl.tiles = one_each ? n_seqs * ((g + rows - 1) / rows) : n_seqs + total_q * g / rows;
   const int64_t units = std::max<int64_t>(1, std::min(pl.tiles, n_seqs * ((q * g + rows - 1) / rows)) * n_kv);
-  const int64_t want = ((pl.few ? 1 : 4) * (int64_t)cus + units - 1) / units;
+  const int64_t want = ((pl.few ? 1 : n_seqs < 8 ? 2 : 4) * (int64_t)cus + units - 1) / units;
   pl.min_piece = pl.few ? (max_kv <= 512 ? 512 : 128) : 512;
   if (!pl.few && units * ((max_kv + 511) / 512) <= cus) pl.min_piece = units * ((max_kv + 255) / 256) <= cus / 2 ? 128 : 256;
   const int64_t most = (max_kv + pl.min_piece - 1) / pl.min_piece;
