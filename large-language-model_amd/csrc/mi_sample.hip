@@ -550,11 +550,13 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   }
   if (top_p < 1.0f) {
     clear();
-    each_kept(all, [&](float v, bool is) __attribute__((always_inline)) {
+    auto weigh = [&](float v, bool is) __attribute__((always_inline)) {
       const int b = bin_of(v);
       const uint64_t w = whole_of(weight_of(v));
       if (is && b < SMP_BINS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)w);
-    });
+    };
+    if (border == -INFINITY) each([&](float v) __attribute__((always_inline)) { weigh(v, v > -INFINITY); });
+    else each_kept(all, weigh);
     __syncthreads();
     const uint64_t tie = ties ? whole_of(tie_w) : 0;
     uint64_t sum_all = 0;
