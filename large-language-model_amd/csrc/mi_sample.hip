@@ -90,6 +90,33 @@ __device__ __forceinline__ u32x4_t smp_load(const void* row, int j, int V) {
   return v;
 }
 
+// The vectors of this lane of a row of V: vector i of a wave's run of `layers` holds the elements from
+// first + 64 EV i on.  ahead() only asks for one, without a branch, so that the wait for those asked for
+// before need not be for this one too; at() is what it holds, which past the row's end is read again there.
+__device__ const uint32_t smp_none[4] = {0, 0, 0, 0};
+template <bool BF16>
+struct SampleRun {
+  static constexpr int EV = BF16 ? 8 : 4;
+  const char* row;
+  int V, first, wave_first;
+  __device__ __forceinline__ SampleRun(const SampleParams& p, int r)
+      : row((const char*)p.logits + (int64_t)r * p.ld * (BF16 ? 2 : 4)), V(p.vocab) {
+    wave_first = uniform(threadIdx.x >> 6) * p.layers * 64 * EV;
+    first = wave_first + (int)(threadIdx.x & 63) * EV;
+  }
+  __device__ __forceinline__ u32x4_t ahead(int i) const {
+    const char* at = row + (int64_t)min(first + 64 * EV * i, V - EV) * (BF16 ? 2 : 4);
+    return *(const u32x4_any_t*)(V >= EV ? at : (const char*)smp_none);
+  }
+  __device__ __forceinline__ u32x4_t at(u32x4_t v, int i) const {
+    if (wave_first + 64 * EV * (i + 1) > V) {
+      v = smp_load<BF16>(row, first + 64 * EV * i, V);
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), here and not where the branches meet
+    }
+    return v;
+  }
+};
+
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -155,20 +182,17 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   constexpr int EV = BF16 ? 8 : 4, WAVES = TH / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int V = p.vocab, layers = p.layers;
-  const void* x = (const char*)p.logits + (int64_t)row * p.ld * (BF16 ? 2 : 4);
-  // this wave's run of the row: layer i holds elements first + (64 i + lane) EV ..; a whole number of
-  // layers covers it, so runs of the last waves may lie past its end (the sum stays below 2^25)
-  const int first = wave * layers * 64 * EV + lane * EV;
-  auto layer = [&](int i) __attribute__((always_inline)) {
-    return smp_load<BF16>(x, first + 64 * EV * i, V);
-  };
+  // a whole number of layers covers the row, so runs of the last waves may lie past its end (the sum
+  // stays below 2^25)
+  const SampleRun<BF16> run(p, row);
+  const int first = run.first;
   // f(i, vector) over this lane's vectors, the next one on its way; f returns whether to go on (the
   // same in all lanes)
   auto each_vector = [&](auto f) __attribute__((always_inline)) {
-    u32x4_t v = layer(0);
+    u32x4_t v = run.ahead(0);
     for (int i = 0; i < layers; ++i) {
-      const u32x4_t next = layer(i + 1);
-      if (!f(i, v)) break;
+      const u32x4_t next = run.ahead(i + 1);
+      if (!f(i, run.at(v, i))) break;
       v = next;
     }
   };
@@ -193,14 +217,14 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   for (int i0 = 0; i0 < layers; i0 += 4) {  // four vectors on their way: this pass waits for memory
     u32x4_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i0 + j < layers) v[j] = layer(i0 + j);
+    for (int j = 0; j < 4; ++j) v[j] = run.ahead(i0 + j);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (i0 + j >= layers) break;
+      const u32x4_t vec = run.at(v[j], i0 + j);
 #pragma unroll
       for (int e = 0; e < EV; ++e) {
-        const float l = smp_elem<BF16>(v[j], e);
+        const float l = smp_elem<BF16>(vec, e);
         mx = fmaxf(mx, l);
         mn = fminf(mn, l > -INFINITY ? l : INFINITY);
       }
@@ -555,8 +579,24 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
       const uint64_t w = whole_of(weight_of(v));
       if (is && b < SMP_BINS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)w);
     };
-    if (border == -INFINITY) each([&](float v) __attribute__((always_inline)) { weigh(v, v > -INFINITY); });
-    else each_kept(all, weigh);
+    if (border == -INFINITY) {
+      // a vector's weights side by side: the asm keeps them out of the branches about the sums
+      each_vector([&](int, const u32x4_t& vec) __attribute__((always_inline)) {
+        uint64_t w[EV];
+#pragma unroll
+        for (int e = 0; e < EV; ++e) w[e] = whole_of(weight_of(smp_elem<BF16>(vec, e)));
+#pragma unroll
+        for (int e = 0; e < EV; ++e) asm volatile("" : "+v"(w[e]));
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          const int b = bin_of(smp_elem<BF16>(vec, e));  // SMP_BINS of -inf and NaN
+          if (b < SMP_BINS) atomicAdd((unsigned long long*)&sh.bins[b], (unsigned long long)w[e]);
+        }
+        return true;
+      });
+    } else {
+      each_kept(all, weigh);
+    }
     __syncthreads();
     const uint64_t tie = ties ? whole_of(tie_w) : 0;
     uint64_t sum_all = 0;
@@ -759,13 +799,13 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
                                                float min_p, SampleCounts<TH / 64>& sh) {
   constexpr int EV = 8, WAVES = TH / 64, EACH = (SMC_LIST + TH - 1) / TH;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), V = p.vocab, layers = p.layers;
-  const void* x = (const char*)p.logits + (int64_t)row * p.ld * 2;
-  const int first = wave * layers * 64 * EV + lane * EV;
+  const SampleRun<true> run(p, row);
+  const int first = run.first;
   // four vectors are under way at a time
   u32x4_t vec[4];
   auto fetch = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vec[j] = smp_load<true>(x, first + 64 * EV * (i0 + j), V);
+    for (int j = 0; j < 4; ++j) vec[j] = smp_load<true>(run.row, first + 64 * EV * (i0 + j), V);
   };
   auto each_vector = [&](auto f) __attribute__((always_inline)) {
     for (int i0 = 0; i0 < layers; i0 += 4) {
