@@ -4,8 +4,16 @@
 // h / group:  O = sum_j e_j v_j / sum_j e_j,  e_j = exp(scale q.k_j - m),  j <= p (causal) or
 // j < n, with the running maximum m and sum of an online softmax in fp32.
 //
+// Bound by reading the keys once for a KV head's group where rows are few, by the matrix cores where they
+// are many.  Few rows (decode) have kernels of their own below: 64 sequences of up to 8000 keys, 372 MB in
+// 79 us (4.7 TB/s; equal lengths reach 5.3 to 5.9, plain reads 6.0); one of 2048 keys takes 11 us, two
+// launches.  Many: 4096 rows over 8192 keys in 242 us (850 TFLOP/s), 4 chunks of up to 1024 rows over 4095
+// in 60 (509).  What keeps these from the rate of a large product is a block's chain of product, maximum,
+// exponentials and product, 1.75 us alone on a CU, half of it hidden by a second workgroup.
+//
 // A workgroup owns 128 rows of one (sequence, KV head), the group's query heads of a token side by side,
 // so one pass over K and V serves all of them; it streams 64-key blocks through a two-stage LDS ring.
+// P is rounded to bf16 for its product with V, 2^-8 of each weight at most, as V itself is.
 // Blocks are gathered row by row from the pages, straight into LDS.  Keys beyond the sequence, in bad
 // pages or past head_dim are read from zeros: what a page holds past the sequence may be anything.
 #include <hip/hip_runtime.h>
@@ -737,7 +745,7 @@ __device__ __forceinline__ int pa_pieces_of(const AttnParams& p, PaTile t, int r
 
 // One new token for each sequence: the keys of all sequences, in blocks of PF_BLOCK, are one line that the
 // workgroups of a KV head share evenly, so that sequences of any lengths keep all CUs busy to the end
-// (64 sequences of 500 to 8000 keys, 372 MB: 83 us, in pieces 92 at best).  A workgroup's share lies
+// (64 sequences of 500 to 8000 keys, 372 MB: 79 us, in pieces 92 at best).  A workgroup's share lies
 // in one sequence or runs over several; only its first and its last may be cut.
 constexpr int PF_BLOCK = PF_KEYS * PF_WAVES;
 constexpr int PF_SEQS = 1024;   // sequences whose lengths a workgroup sums up
@@ -947,7 +955,7 @@ struct PaPlan {
 // Decode (graph replays; 16 / 4 heads of 128): one piece up to 512 keys (256 keys 8.6 us, in two pieces
 // and a join 10.5); else a workgroup for each CU, of 128 keys at least (one sequence of 32768: 23.9 us,
 // in twice as many pieces 29); where those pieces are long and the sequences several, even shares (64 of
-// up to 8000: 115 us in pieces, 83 in shares; 64 of up to 1000: 19 and 24).
+// up to 8000: 115 us in that many pieces, 79 in shares; 64 of up to 1000: 19 and 24).
 // Many rows: pieces of 512 keys at least until there are two workgroups for each CU, which fit at once; four
 // where the sequences are eight or more, of which some are short (4 chunks of up to 1024 rows over 4095
 // keys: 59 us, with four 65; 3 of 500 over 9000: 81 and 88; 16 of up to 333 over 2500: 55 with two, 49; 32 of

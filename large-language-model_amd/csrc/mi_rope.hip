@@ -4,7 +4,9 @@
 //   a' = scale (a cos - b sin),  b' = scale (b cos + a sin)
 // with (a, b) = (x[i], x[i + rot/2]) or (x[2i], x[2i+1]); the way back is the transposed map, the
 // same with the sine negated.  Three operations for each element that is read and written once:
-// bound by HBM.
+// bound by HBM.  8 x 1024 tokens of 16 + 2 x 4 heads of 128, bf16, there and back: 201 MB in 37 us
+// from the caches behind L2, 43 from memory, where a copy of 1 GiB takes 40 for as much; 16381 tokens
+// with interleaved pairs 33 and 41.  A decode step's append (64 tokens) takes 4 us, its launch.
 //
 // A workgroup takes a few tokens with all heads of all tensors.  It first computes each token's
 // cosines and sines once into LDS, where every head of the token reads them: 64 pairs of a
