@@ -267,6 +267,29 @@ def test_streams_and_graph(mi, dev):
         assert torch.equal(out, eager)
 
 
+def test_graph_of_long_rows(mi, dev):
+    """Counted rows, and after them rows that the counts cannot hold, from one captured call."""
+    import torch
+
+    x, u = make(300, 9000, "bf16", 5)
+    p = torch.full((300,), 0.9, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    mi.sample(x, u, top_p=p)
+    with torch.cuda.graph(g):
+        out = mi.sample(x, u, top_p=p, sync=False)
+    for seed in (6, 7, 8):
+        y, w = make(300, 9000, "bf16", seed)
+        if seed == 7:
+            y[::2, 9] = 1e-30
+        x.copy_(y)
+        u.copy_(w)
+        p.copy_(w * 0.5 + 0.4)
+        eager = check(mi, x, u, p=p)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+
+
 def test_logits_of_the_head(mi, dev):
     """The LM head's product, then its tokens, as a decode step ends: hidden rows -> logits -> tokens."""
     import torch
