@@ -902,39 +902,39 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(AttnParams p) {
   pa_join<PA_PIECES>(p, row, head, n, [&](int i) { return i * pitch + at; });
 }
 
-// The same for up to eight pieces of many rows: a workgroup a token, 32 lanes a head, all pieces' loads in flight.
+// The same for up to eight pieces of many rows: 32 lanes a head, eight heads of a token a workgroup, all
+// pieces' loads in flight.
 __global__ void __launch_bounds__(256) paged_attn_join8_kernel(AttnParams p) {
-  const int l32 = threadIdx.x & 31, c = 4 * l32, row = blockIdx.x;
+  const int each = (p.n_heads + 7) >> 3, row = uniform(blockIdx.x / each);
+  const int l32 = threadIdx.x & 31, c = 4 * l32, head = 8 * (int)(blockIdx.x - row * each) + (threadIdx.x >> 5);
   const PaTile t = pa_row_tile(p, row);
-  if (t.s < 0) return;
+  if (t.s < 0 || head >= p.n_heads) return;
   const int64_t pitch = (int64_t)p.pv.total_q * p.n_heads;
-  for (int head = threadIdx.x >> 5; head < p.n_heads; head += 8) {
-    const int n = pa_pieces_of(p, t, row, head);
-    if (n < 2) continue;
-    const int64_t at = (int64_t)row * p.n_heads + head;
-    float lse[8];
-    f32x4_t x[8];
+  const int n = pa_pieces_of(p, t, row, head);
+  if (n < 2) return;
+  const int64_t at = (int64_t)row * p.n_heads + head;
+  float lse[8];
+  f32x4_t x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lse[i] = i < n ? p.part_lse[i * pitch + at] : -INFINITY;
-      x[i] = i < n && c < p.d ? *(const f32x4_t*)(p.part_o + (i * pitch + at) * p.d + c) : f32x4_t{0, 0, 0, 0};
-    }
-    float mx = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, lse[i]);
-    f32x4_t acc = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = lse[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lse[i] - mx);
-      sum += w;
-      acc += w * x[i];
-    }
-    acc *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (c < p.d)
-      *(u32x2_t*)(p.o + (int64_t)row * p.o_t + (int64_t)head * p.o_h + c) =
-          u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
-    if (p.lse && l32 == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
+  for (int i = 0; i < 8; ++i) {
+    lse[i] = i < n ? p.part_lse[i * pitch + at] : -INFINITY;
+    x[i] = i < n && c < p.d ? *(const f32x4_t*)(p.part_o + (i * pitch + at) * p.d + c) : f32x4_t{0, 0, 0, 0};
   }
+  float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx = fmaxf(mx, lse[i]);
+  f32x4_t acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = lse[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lse[i] - mx);
+    sum += w;
+    acc += w * x[i];
+  }
+  acc *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (c < p.d)
+    *(u32x2_t*)(p.o + (int64_t)row * p.o_t + (int64_t)head * p.o_h + c) =
+        u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+  if (p.lse && l32 == 0) p.lse[at] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
 }
 
 // How a launch is laid out: tiles of rows, pieces of a tile's keys, and keys of a piece at least.
@@ -1080,7 +1080,8 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   else paged_attn_kernel<128><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>(p);
   e = hipGetLastError();
   if (e == hipSuccess && plan.pieces > 1) {
-    if (plan.pieces <= 8 && !plan.few) paged_attn_join8_kernel<<<(unsigned)rows, 256, 0, (hipStream_t)stream>>>(p);
+    const unsigned wgs8 = (unsigned)(rows * ((n_heads + 7) / 8));
+    if (plan.pieces <= 8 && !plan.few) paged_attn_join8_kernel<<<wgs8, 256, 0, (hipStream_t)stream>>>(p);
     else paged_attn_join_kernel<<<(unsigned)(rows * n_heads), 256, 0, (hipStream_t)stream>>>(p);
     e = hipGetLastError();
   }
