@@ -8,8 +8,9 @@
 // are many.  Few rows (decode) have kernels of their own below: 64 sequences of up to 8000 keys, 372 MB in
 // 79 us (4.7 TB/s; equal lengths reach 5.3 to 5.9, plain reads 6.0); one of 2048 keys takes 11 us, two
 // launches.  Many: 4096 rows over 8192 keys in 242 us (850 TFLOP/s), 4 chunks of up to 1024 rows over 4095
-// in 60 (509).  What keeps these from the rate of a large product is a block's chain of product, maximum,
-// exponentials and product, 1.75 us alone on a CU, half of it hidden by a second workgroup.
+// in 60 (509).  What keeps these from the rate of a large product is LDS: each of four waves reads all of a
+// block's K and V, 128 KB, beside a chain of product, maximum, exponentials and product; computing the next
+// block's scores under the exponentials instead only took registers (66 -> 72 us).
 //
 // A workgroup owns 128 rows of one (sequence, KV head), the group's query heads of a token side by side,
 // so one pass over K and V serves all of them; it streams 64-key blocks through a two-stage LDS ring.
