@@ -1397,25 +1397,32 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         raise ValueError("logits must have a contiguous last dimension")
     if out is None:
         out = logits.new_empty((rows,), dtype=torch.int32)
-    f32, i32 = torch.float32, torch.int32
-    tensors, at, values = [logits], [], []
-    for name, v, dt, off in (("temperature", temperature, f32, 0.0), ("top_k", top_k, i32, 0), ("top_p", top_p, f32, 0.0),
-                             ("min_p", min_p, f32, 0.0), ("u", u, f32, None), ("out", out, i32, None),
-                             ("prob", prob, f32, None)):
-        if isinstance(v, torch.Tensor):
-            if v.dtype != dt or v.shape != (rows,) or not v.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {dt} [{rows}] tensor" + ("" if off is None else " or a number"))
-            tensors.append(v)
-            at.append(v.data_ptr())
-            values.append(off)
-        elif off is None and v is not None:
+    f32, i32, Tensor = torch.float32, torch.int32, torch.Tensor
+    tensors = [logits]
+
+    def of_rows(name, v, dt, or_number=""):
+        if not isinstance(v, Tensor):
             raise ValueError(f"{name} must be a tensor")
-        else:
-            at.append(0)
-            values.append(v)
-    stream = _stream_of(*tensors)
-    how = _PACK_SAMPLING(*at[:4], values[0], int(values[1]), values[2], values[3])
-    st = load_library().mi_sample(stream, logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V, how, *at[4:])
+        if v.dtype != dt or v.shape != (rows,) or not v.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dt} [{rows}] tensor{or_number}")
+        tensors.append(v)
+        return v.data_ptr()
+
+    t_at = k_at = p_at = m_at = prob_at = 0
+    if isinstance(temperature, Tensor):
+        t_at, temperature = of_rows("temperature", temperature, f32, " or a number"), 0.0
+    if isinstance(top_k, Tensor):
+        k_at, top_k = of_rows("top_k", top_k, i32, " or a number"), 0
+    if isinstance(top_p, Tensor):
+        p_at, top_p = of_rows("top_p", top_p, f32, " or a number"), 0.0
+    if isinstance(min_p, Tensor):
+        m_at, min_p = of_rows("min_p", min_p, f32, " or a number"), 0.0
+    u_at, out_at = of_rows("u", u, f32), of_rows("out", out, i32)
+    if prob is not None:
+        prob_at = of_rows("prob", prob, f32)
+    how = _PACK_SAMPLING(t_at, k_at, p_at, m_at, temperature, int(top_k), top_p, min_p)
+    st = load_library().mi_sample(_stream_of(*tensors), logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V,
+                                  how, u_at, out_at, prob_at)
     _done("mi_sample", st, sync)
     return out
 
