@@ -1255,18 +1255,19 @@ def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
     """mi_paged_cache and mi_paged_seqs, packed, of caches [pages, nKV, page size, d] (any strides with
     contiguous components) and int32 device tables; and (nKV, page size, d, sequences, table width)."""
     torch = _torch()
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != strides:
         raise ValueError("k_cache and v_cache are [pages, nKV, page size, d] of one shape and strides")
-    num, n_kv, size, d = k_cache.shape
-    sp, sh, ss, sc = k_cache.stride()
+    num, n_kv, size, d = shape
+    sp, sh, ss, sc = strides
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16 or (sc != 1 and d > 1):
         raise ValueError("the caches must be bf16 with contiguous components")
-    i32 = torch.int32
-    if pages.dtype != i32 or pages.dim() != 2 or (pages.stride(1) != 1 and pages.shape[1] > 1):
+    i32, table, rows_at = torch.int32, pages.shape, pages.stride()
+    if pages.dtype != i32 or len(table) != 2 or (rows_at[1] != 1 and table[1] > 1):
         raise ValueError("pages must be int32, 2-D, with a contiguous last dimension")
     if kv_len.dtype != i32 or kv_len.dim() != 1 or not kv_len.is_contiguous():
         raise ValueError("kv_len must be int32, 1-D, contiguous")
-    n, (table_rows, width) = kv_len.numel(), pages.shape
+    n, (table_rows, width) = kv_len.numel(), table
     if table_rows != n:
         raise ValueError(f"pages needs {n} rows, as kv_len has")
     if q_start is None:
@@ -1276,7 +1277,7 @@ def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
         raise ValueError(f"q_start must be int32, 1-D, contiguous, with {n + 1} entries")
     cache = _PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), num, size, n_kv, d, sp, sh, ss)
     seqs = _PACK_SEQS(n, rows, 0 if q_start is None else q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
-                      width, pages.stride(0) if n > 1 else width)
+                      width, rows_at[0] if n > 1 else width)
     return cache, seqs, (n_kv, size, d, n, width)
 
 
@@ -1311,8 +1312,9 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
         n_heads = q.shape[1] if q.dim() == 3 else 0
         q_t, q_h = _heads_of("q", q, N, n_heads, d)
         if q_out is None:
-            q_out = q.new_empty((N, n_heads, d))
-        o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
+            q_out, o_t, o_h = q.new_empty((N, n_heads, d)), n_heads * d, d
+        else:
+            o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
     stream = _stream_of(k, v, k_cache, v_cache, pages, kv_len, q_start, q, q_out, inv_freq, positions)
     rotary = None
@@ -1355,8 +1357,9 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
         raise ValueError(f"the cache has heads of {cd}, q of {d}")
     q_t, q_h = _heads_of("q", q, N, n_heads, d)
     if out is None:
-        out = q.new_empty((N, n_heads, d))
-    o_t, o_h = _heads_of("out", out, N, n_heads, d)
+        out, o_t, o_h = q.new_empty((N, n_heads, d)), n_heads * d, d
+    else:
+        o_t, o_h = _heads_of("out", out, N, n_heads, d)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, n_heads) or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 [{N}, {n_heads}] tensor")
     stream = _stream_of(q, k_cache, v_cache, pages, kv_len, q_start, out, lse,
