@@ -14,7 +14,10 @@
 //
 // A workgroup owns 128 rows of one (sequence, KV head), the group's query heads of a token side by side,
 // so one pass over K and V serves all of them; it streams 64-key blocks through a two-stage LDS ring.
-// P is rounded to bf16 for its product with V, 2^-8 of each weight at most, as V itself is.
+// P goes into its product with V as the sum of two bf16, in every kernel: what is left out is 2^-16 of a weight,
+// so an output is as exact as its own rounding, whichever rows share its tile.  Rounded to one bf16 the weights
+// of many rows cost a product less, 65 us in place of 79 (4 chunks of up to 1024 rows over 4095 keys) and 259 of
+// 335 (4096 over 8192), but outputs are off by up to 2^-8 of sum p |v| more than those of decode.
 // Blocks are gathered row by row from the pages, straight into LDS.  Keys beyond the sequence, in bad
 // pages or past head_dim are read from zeros: what a page holds past the sequence may be anything.
 #include <hip/hip_runtime.h>
@@ -145,8 +148,7 @@ struct PaLds {
 //   S = K Q^T on v_mfma_f32_16x16x32_bf16: lane l holds row l % 16 and, in the two 16-key tiles t, the keys
 //   8 (l / 16) + 4t + e: tile t's row r reads key 8 (r / 4) + 4t + r % 4, so that these eight are, in order,
 //   the run of keys that the second operand of P V takes.
-// P goes into that product as the sum of two bf16, which costs nothing here: the output is then as exact
-// as its own rounding.
+// The second bf16 of P costs nothing here.
 template <int D>
 struct PfLds {
   static constexpr int ROW = D * 2;
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     m_run = m_ref;
     const float nmc = m_ref == -INFINITY ? 0.0f : -m_ref * sl2;
     float sum = 0.0f;
-    u32x4_t pf[4];
+    u32x4_t hi[4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const int kb = ks >> 1, base = 8 * (ks & 1);
@@ -616,7 +618,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2], sl2, nmc));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2 + 1], sl2, nmc));
         sum += e0 + e1;
-        pf[ks][w2] = pack_bf16x2(e0, e1);
+        hi[ks][w2] = pack_bf16x2(e0, e1);
+        sc[kb][base + 2 * w2] = e0;  // for what hi leaves, taken while V is read
+        sc[kb][base + 2 * w2 + 1] = e1;
       }
     }
     l_run += sum;
@@ -638,13 +642,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
           vf[c][2 * tt + 1] = w2[1];
         });
       }
+      u32x4_t lo;
+      {
+        constexpr int kb = ks >> 1, base = 8 * (ks & 1);
+#pragma unroll
+        for (int w2 = 0; w2 < 4; ++w2)
+          lo[w2] = pack_bf16x2(sc[kb][base + 2 * w2] - bf16_bits_to_f32(hi[ks][w2] & 0xffffu),
+                               sc[kb][base + 2 * w2 + 1] - __uint_as_float(hi[ks][w2] & 0xffff0000u));
+      }
       // the results are valid after lgkmcnt(0), which the compiler does not know of
       __builtin_amdgcn_s_waitcnt(0xC07F);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
-                                                       __builtin_bit_cast(bf16x8_t, pf[ks]), o[c], 0, 0, 0);
+                                                       __builtin_bit_cast(bf16x8_t, lo), o[c], 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
+                                                       __builtin_bit_cast(bf16x8_t, hi[ks]), o[c], 0, 0, 0);
     });
   };
 
