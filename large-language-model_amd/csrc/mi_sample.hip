@@ -334,10 +334,10 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int row, Sampl
   auto all = [](float, int) { return true; };
 
   // Bins, even in the distance from the maximum, over what weighs anything; halves of the values, whose
-  // difference cannot overflow.
-  const float reach = min((float)((0.5 * mxd - 0.5 * (double)mn) * c), 0.5f * (float)(p.shift + 2));
-  const float per =
-      c > 0.0 && reach > 0.0f ? (float)min((double)(SMP_BINS - 1) / (double)reach * c, 3e38) : 0.0f;
+  // difference cannot overflow.  64 bits until the division: with a temperature of 1e38 a reach in 32 is a
+  // denormal of few bits, and the row's tail would lie past the last bin.
+  const double reach = min((0.5 * mxd - 0.5 * (double)mn) * c, 0.5 * (double)(p.shift + 2));
+  const float per = c > 0.0 && reach > 0.0 ? (float)min((double)(SMP_BINS - 1) / reach * c, 3e38) : 0.0f;
   const float half_mx = 0.5f * mx;
   auto bin_of = [&](float v) __attribute__((always_inline)) {
     return (int)fminf(fmaf(-0.5f, v, half_mx) * per, (float)SMP_BINS);  // SMP_BINS: weighs nothing
