@@ -1011,9 +1011,10 @@ size_t mi_paged_attn_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_
                                     int64_t max_q_len, int64_t max_kv_len) {
   if (n_heads < 1 || n_kv < 1 || n_heads % n_kv || head_dim < 1 || n_seqs < 1 || total_q < 1) return 0;
   if (n_seqs > INT32_MAX || total_q > INT32_MAX / n_heads) return 0;  // refused by the call
-  // CUs of the current device; without one, those of an MI355X
+  // CUs of the current device, whose table the first of all calls fills in; without one, those of an MI355X
+  const int cus = host_device() == MI_OK ? host_cus() : 256;
   const PaPlan plan = pa_plan(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len,
-                              total_q == n_seqs && max_q_len == 1, host_cus());
+                              total_q == n_seqs && max_q_len == 1, cus);
   return (size_t)std::max(plan.bytes(total_q, n_heads, head_dim), plan.share_bytes(n_seqs, n_heads, head_dim));
 }
 
