@@ -507,7 +507,8 @@ typedef struct mi_sampling {
  * 2^-(62 - b), at most 2^-50, b the bits of vocab - 1 (2^-46 for 65536 entries), so sums do not
  * depend on their order and a token of less than half of that is never drawn.  NaN logits weigh
  * nothing; a +inf logit takes all; a row without a logit above -inf gets token -1 and share 0.
- * Any alignment of whole elements and any row pitch; vocab at most 2^24.
+ * Any alignment of whole elements and any row pitch ld >= vocab, or 0: all rows pick from one, each
+ * with its own u and settings.  vocab at most 2^24.
  */
 int mi_sample(void* stream, const void* logits, int32_t dtype, int64_t ld, int64_t rows, int64_t vocab,
               const mi_sampling* how, const float* u, int32_t* tokens, float* probs);

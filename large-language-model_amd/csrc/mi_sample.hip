@@ -1131,7 +1131,7 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
     return host_fail(MI_ERR_SHAPE, "rows=%lld exceeds 2^31-1 or vocab=%lld exceeds 2^24", (long long)rows,
                      (long long)vocab);
   if (!logits || !how || !u || !tokens) return host_fail(MI_ERR_NULL, "logits, how, u or tokens is NULL");
-  if (rows > 1 && ld < vocab)
+  if (rows > 1 && ld != 0 && ld < vocab)
     return host_fail(MI_ERR_LD, "ld=%lld < vocab=%lld", (long long)ld, (long long)vocab);
   if ((uintptr_t)logits % (dtype == MI_BF16 ? 2 : 4) || ((uintptr_t)u & 3) || ((uintptr_t)tokens & 3) ||
       ((uintptr_t)probs & 3) || ((uintptr_t)how->temperature & 3) || ((uintptr_t)how->top_k & 3) ||

@@ -1384,8 +1384,9 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
 # ---- sampling ---------------------------------------------------------------------
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, prob=None, sync=None):
-    """One token for each row of logits [rows, V] (bf16 or fp32, any row stride; mi_sample) from the
-    uniform numbers u (fp32 [rows], in [0, 1)). temperature, top_k, top_p, min_p: a number for all
+    """One token for each row of logits [rows, V] (bf16 or fp32, any row stride of V or more, or 0 as
+    of logits.expand(rows, V): several tokens from one row; mi_sample) from the uniform numbers u
+    (fp32 [rows], in [0, 1)). temperature, top_k, top_p, min_p: a number for all
     rows or a tensor [rows] (fp32, top_k int32); temperature <= 0 takes the largest logit, top_k <= 0,
     top_p >= 1 and min_p <= 0 are off. Filters apply in the order top-k, top-p of what is left,
     min-p; equal logits go by index, lowest first. Returns tokens (int32 [rows], into `out` if
