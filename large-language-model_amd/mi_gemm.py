@@ -1362,6 +1362,8 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
         o_t, o_h = _heads_of("out", out, N, n_heads, d)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, n_heads) or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 [{N}, {n_heads}] tensor")
+    if workspace is not None and not isinstance(workspace, str) and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous: its bytes are those of its elements")
     stream = _stream_of(q, k_cache, v_cache, pages, kv_len, q_start, out, lse,
                         None if isinstance(workspace, str) else workspace)
     mq = 1 if q_start is None else N if max_q_len is None else int(max_q_len)
