@@ -1426,7 +1426,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     u_at, out_at = of_rows("u", u, f32), of_rows("out", out, i32)
     if prob is not None:
         prob_at = of_rows("prob", prob, f32)
-    how = _PACK_SAMPLING(t_at, k_at, p_at, m_at, temperature, int(top_k), top_p, min_p)
+    top_k = min(max(int(top_k), 0), 1 << 30)  # more than any vocabulary has is off, as 0 and less are
+    how = _PACK_SAMPLING(t_at, k_at, p_at, m_at, temperature, top_k, top_p, min_p)
     st = load_library().mi_sample(_stream_of(*tensors), logits.data_ptr(), _dt(logits), ld if rows > 1 else V, rows, V,
                                   how, u_at, out_at, prob_at)
     _done("mi_sample", st, sync)
