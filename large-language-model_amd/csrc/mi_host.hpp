@@ -13,6 +13,9 @@ int host_error(int code, const char* text);  // stores mi_last_error's text, ret
 int host_device();                           // MI_OK if the current device is a gfx950
 int host_cus();                              // CUs of the current device
 
+// Workgroups of `threads` that a launch may have: its threads are counted in 32 bits.
+inline int64_t host_most_groups(int threads) { return UINT32_MAX / (uint32_t)threads; }
+
 inline int host_fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;

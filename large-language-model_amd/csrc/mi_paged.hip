@@ -1046,6 +1046,9 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   if (st != MI_OK) return st;
   PaPlan plan = pa_plan(n_heads, cache->n_kv, d, seqs->n_seqs, rows, max_q_len, max_kv_len, !seqs->q_start, host_cus());
   if (seqs->n_seqs * (seqs->max_pages * cache->page_size / PF_BLOCK + 1) > INT32_MAX) plan.share = 0;  // its sums
+  // The joins have a workgroup for each row and head.  Only a max_q_len far below the sequences' rows cuts so many.
+  const int64_t most = host_most_groups(256);
+  if (rows * n_heads > most) plan.pieces = 1, plan.share = 0;
   // as many pieces as the workspace holds
   const int64_t piece_bytes = rows * n_heads * (d + 1) * 4;
   if (!workspace) plan.pieces = 1;
@@ -1090,7 +1093,9 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
     return e == hipSuccess ? MI_OK : host_fail(MI_ERR_HIP, "paged_attn launch: %s", hipGetErrorString(e));
   }
   const int64_t grid = plan.tiles * p.n_kv * plan.pieces;
-  if (grid > INT32_MAX) return host_fail(MI_ERR_SHAPE, "too many row tiles");
+  if (grid > most)
+    return host_fail(MI_ERR_SHAPE, "%lld row tiles of %lld KV heads: more than %lld workgroups", (long long)plan.tiles,
+                     (long long)cache->n_kv, (long long)most);
   if (plan.few) {
     if (d <= 64) paged_attn_few_kernel<64><<<(unsigned)grid, 64 * PF_WAVES, 0, (hipStream_t)stream>>>(p);
     else paged_attn_few_kernel<128><<<(unsigned)grid, 64 * PF_WAVES, 0, (hipStream_t)stream>>>(p);

@@ -49,6 +49,7 @@ struct RopeParams {
   int64_t pos_ld, pos0;
   int tokens, T;        // T: tokens of a sequence (dense)
   int per_wg;           // tokens of a workgroup
+  int64_t first;        // the launch's first token
   PagedView pv;
 };
 
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(RopeParams p) {
   __shared__ int64_t tok_pos[ROPE_MAX_TOKENS], tok_off[ROPE_MAX_TOKENS];
   __shared__ int tok_b[ROPE_MAX_TOKENS], tok_t[ROPE_MAX_TOKENS];
   const int tid = threadIdx.x;
-  const int64_t tok0 = (int64_t)blockIdx.x * p.per_wg;
+  const int64_t tok0 = p.first + (int64_t)blockIdx.x * p.per_wg;
   const int n_tok = (int)min((int64_t)p.per_wg, p.tokens - tok0);
 
   if constexpr (PAGED) {
@@ -235,11 +236,17 @@ bool rope_vec_fits(const RopeParams& p, int vec, int es, int64_t batch, int64_t 
 }
 
 template <typename T, int VEC>
-hipError_t rope_launch(const RopeParams& p, bool paged, hipStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)p.tokens + p.per_wg - 1) / p.per_wg);
-  if (paged) rope_kernel<T, VEC, true><<<grid, ROPE_THREADS, 0, st>>>(p);
-  else rope_kernel<T, VEC, false><<<grid, ROPE_THREADS, 0, st>>>(p);
-  return hipGetLastError();
+hipError_t rope_launch(RopeParams p, bool paged, hipStream_t st) {
+  const int64_t groups = ((int64_t)p.tokens + p.per_wg - 1) / p.per_wg, most = host_most_groups(ROPE_THREADS);
+  hipError_t e = hipSuccess;
+  for (int64_t g = 0; g < groups && e == hipSuccess; g += most) {
+    const unsigned grid = (unsigned)(groups - g < most ? groups - g : most);
+    p.first = g * p.per_wg;
+    if (paged) rope_kernel<T, VEC, true><<<grid, ROPE_THREADS, 0, st>>>(p);
+    else rope_kernel<T, VEC, false><<<grid, ROPE_THREADS, 0, st>>>(p);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 // Fills in the workgroup's share and launches; heads: of each part.

@@ -1140,16 +1140,11 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
   const int st = host_device();
   if (st != MI_OK) return st;
   SampleParams p;
-  p.logits = logits;
   p.ld = ld;
   p.vocab = (int)vocab;
   int bits = 0;
   while ((int64_t{1} << bits) < vocab) ++bits;
   p.shift = 62 - bits < 50 ? 62 - bits : 50;
-  p.u = u;
-  p.tokens = tokens;
-  p.probs = probs;
-  p.how = *how;
   const bool bf16 = dtype == MI_BF16;
   // Whether any row may gain by counts; each decides for itself.
   const bool counted = bf16 && vocab >= SMC_FROM &&
@@ -1163,7 +1158,20 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
   auto kernel = halved ? sample_kernel<512, false> : sample_kernel<1024, false>;
   if (counted) kernel = halved ? sample_counts_kernel<512> : sample_counts_kernel<1024>;
   else if (bf16) kernel = halved ? sample_kernel<512, true> : sample_kernel<1024, true>;
-  kernel<<<(unsigned)rows, threads, 0, (hipStream_t)stream>>>(p);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipSuccess;
+  const int64_t most = host_most_groups(threads);
+  for (int64_t r = 0; r < rows && e == hipSuccess; r += most) {
+    p.logits = (const char*)logits + r * ld * (bf16 ? 2 : 4);
+    p.u = u + r;
+    p.tokens = tokens + r;
+    p.probs = probs ? probs + r : nullptr;
+    p.how = *how;
+    if (how->temperature) p.how.temperature += r;
+    if (how->top_k) p.how.top_k += r;
+    if (how->top_p) p.how.top_p += r;
+    if (how->min_p) p.how.min_p += r;
+    kernel<<<(unsigned)(rows - r < most ? rows - r : most), threads, 0, (hipStream_t)stream>>>(p);
+    e = hipGetLastError();
+  }
   return e == hipSuccess ? MI_OK : host_fail(MI_ERR_HIP, "sample launch: %s", hipGetErrorString(e));
 }
