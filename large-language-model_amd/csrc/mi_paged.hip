@@ -969,15 +969,22 @@ struct PaPlan {
   }
 };
 
-// Decode (graph replays; 16 / 4 heads of 128): one piece up to 512 keys (256 keys 8.6 us, in two pieces
-// and a join 10.5); else a workgroup for each CU, of 128 keys at least (one sequence of 32768: 23.9 us,
-// in twice as many pieces 29); where those pieces are long and the sequences several, even shares (64 of
-// up to 8000: 115 us in that many pieces, 79 in shares; 64 of up to 1000: 19 and 24).
+// Decode (graph replays, us; 16 / 4 heads of 128): one piece up to 512 keys (256 keys 8.6, in two pieces
+// and a join 10.5; 512 alike, 10.8 and 10.6 in four); else a workgroup for each CU, of 128 keys at least (one
+// sequence of 32768: 22.4, in twice as many pieces 25.4; of 2048: 11.0, in half as many 12.2).
+// Even shares instead where the sequences are several and long, 1024 keys a piece and 2048 at least. Lengths that
+// differ gain (lengths up to the one given, pieces / shares), alike ones lose less than that:
+//    sequences x keys   64 x 1500    64 x 2000    64 x 8000   256 x 1500  256 x 2000  16 x 4000    16 x 8000
+//              uneven   23.8/23.7    29.2/27.1   103.4/61.8   51.8/57.1   77.2/78.9   22.3/22.8    33.0/28.5
+//                even   34.0/39.3    43.1/47.8   180.0/188    137/142     179/185     28.7/29.9    45.6/49.1
 // Many rows: pieces of 512 keys at least until there are two workgroups for each CU, which fit at once; four
-// where the sequences are eight or more, of which some are short (4 chunks of up to 1024 rows over 4095
-// keys: 59 us, with four 65; 3 of 500 over 9000: 81 and 88; 16 of up to 333 over 2500: 55 with two, 49; 32 of
-// 64 over 6000: 71 and 62).  Shorter ones cost more in joins (8 of 700 over 1400: 50 us of 256, 40).
-// Where that leaves CUs empty, 256 or 128 (16 of 16 rows over 2000: 19 us, 24 of 512; 8 rows over 4000: 12.5, 20).
+// where the sequences are eight or more, of which some are short. With two / four, uneven lengths and even:
+//    sequences, rows over keys   6, 64/6000  8, 64/6000  32, 64/6000  6, 700/1400  10, 700/1400  4, 1024/4095  10, 1024/4095
+//                       uneven   39.6/38.5   39.5/38.0   83.7/64.0    38.6/38.9    45.4/39.4     75.3/81.0     109.8/97.7
+//                         even   59.5/63.4   68.9/71.2   228.7/203.9  77.7/92.8    109.3/140.4   182.8/196.4   449.3/449.7
+// Where that leaves CUs empty, pieces of 256 or 128 keys. One sequence, rows over keys, with 128 / 256 / 512:
+// 8 over 4000 13.1/15.1/21.0, 17 over 2000 13.6/16.1/22.5 (128 taken), 64 over 4000 26.4/22.1/24.9 (128 taken, 4 us
+// too many), 4 sequences of 64 over 2000 32.9/27.3/26.4 (256 taken).
 PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t total_q, int64_t max_q, int64_t max_kv,
                bool one_each, int cus) {
   PaPlan pl;
@@ -994,7 +1001,7 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   const int64_t most = (max_kv + pl.min_piece - 1) / pl.min_piece;
   pl.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, PA_PIECES}));
   // two workgroups on a CU, three of 64 components
-  pl.share = one_each && g <= PF_ROWS && n_seqs > 1 && n_seqs <= PF_SEQS && max_kv > 1024 * (int64_t)pl.pieces
+  pl.share = one_each && g <= PF_ROWS && n_seqs > 1 && n_seqs <= PF_SEQS && max_kv > 1024 * (int64_t)std::max(pl.pieces, 2)
                  ? (int)std::max<int64_t>(1, std::min<int64_t>((d <= 64 ? 3 : 2) * (int64_t)cus / n_kv, PF_SHARES))
                  : 0;
   return pl;

@@ -74,3 +74,18 @@ def test_bytes_without_a_device(mi):
     for bad in ((16, 3, 128, 4, 4, 1, 100), (0, 1, 128, 4, 4, 1, 100), (16, 4, 0, 4, 4, 1, 100), (16, 4, 128, 4, 0, 1, 100),
                 (16, 4, 128, 1, 1 << 31, 1, 100), (1 << 16, 1, 128, 1, 1 << 15, 1 << 15, 100)):
         assert f(*bad) == 0, bad
+
+
+def test_where_even_shares_begin(mi):
+    """1024 keys for each piece that a sequence would be cut into, 2048 at least."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible")
+    f = mi.paged_attn_workspace_size
+    parts = lambda share, S: 2 * share * 16 * 129 * 4 + (S + 1) * 4  # noqa: E731
+    for S, pieces in ((64, 1), (256, 1), (32, 2), (16, 4)):
+        border = 1024 * max(pieces, 2)
+        assert f(16, 4, 128, S, S, 1, border) == (pieces * S * 16 * 129 * 4 if pieces > 1 else 0)
+        assert f(16, 4, 128, S, S, 1, border + 1) == max(parts(128, S), pieces * S * 16 * 129 * 4 if pieces > 1 else 0)
+    assert f(16, 4, 128, 1, 1, 1, 10 ** 6) == 64 * 16 * 129 * 4  # one sequence: pieces
