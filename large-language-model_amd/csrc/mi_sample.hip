@@ -37,7 +37,13 @@ namespace {
 constexpr int SMP_BINS = 1024;
 constexpr int SMP_LIST = 1024;        // tokens of a bin that are ranked in LDS
 constexpr int SMP_FEW = 256;          // tokens that are handled in LDS altogether
-constexpr int SMP_FEW_K = SMP_FEW * 5 / 8;  // the largest top-k for which that is tried
+// The largest top-k that the lanes' maxima are asked for.  Their bound lets a few dozen tokens more than top-k through,
+// and where those do not fit the list the histogram follows all the same.  With 0 / 160 / 255 here (us, top-p 0.9):
+//    rows of logits           top-k 50        160             180             200             220
+//      64 of 32001, fp32      16.0/12.8/12.8  19.5/16.5/16.5  19.9/20.2/17.1  21.1/21.4/18.3  21.7/22.0/27.6
+//     512 of 32000, fp32      34.1/25.8/25.7  39.4/31.6/31.6  40.5/40.9/33.2  41.7/42.1/47.3  42.7/43.2/52.5
+//      64 of 5000, fp32       10.4/9.7/9.7    13.5/12.9/13.0  14.0/14.2/13.5  15.2/15.5/14.8  15.7/16.0/19.4
+constexpr int SMP_FEW_K = SMP_FEW * 5 / 8;
 constexpr int SMP_GATHER = 4;         // logits that a lane weighs at a time: its waits for each overlap
 
 struct SampleParams {
