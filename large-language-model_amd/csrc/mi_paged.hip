@@ -140,6 +140,50 @@ struct PaLds {
   }
 };
 
+// N fragments of V: two transposing reads of 8 bytes each, at[c] + OFF and 4 rows further on.  Inline asm: the builtin
+// would also wait for the loads into LDS that are in flight.  The wait for all of them ends the asm, so that
+// the compiler sees no register before it holds its data.
+template <int N, int OFF, int ROW>
+__device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint32_t (&at)[N]) {
+  static_assert(N == 2 || N == 4 || N == 8, "written out for these");
+  u32x2_t w[2 * N];
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (N == 2)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
+        : "v"(st + at[0]), "v"(st + at[1]), "i"(OFF), "i"(OFF + 4 * ROW));
+  else if constexpr (N == 4)
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
+        : "v"(st + at[0]), "v"(st + at[1]), "v"(st + at[2]), "v"(st + at[3]), "i"(OFF), "i"(OFF + 4 * ROW));
+  else
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %16 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %2, %17 offset:%24\n\tds_read_b64_tr_b16 %3, %17 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %4, %18 offset:%24\n\tds_read_b64_tr_b16 %5, %18 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %6, %19 offset:%24\n\tds_read_b64_tr_b16 %7, %19 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %8, %20 offset:%24\n\tds_read_b64_tr_b16 %9, %20 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %10, %21 offset:%24\n\tds_read_b64_tr_b16 %11, %21 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %12, %22 offset:%24\n\tds_read_b64_tr_b16 %13, %22 offset:%25\n\t"
+        "ds_read_b64_tr_b16 %14, %23 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
+          "=&v"(w[8]), "=&v"(w[9]), "=&v"(w[10]), "=&v"(w[11]), "=&v"(w[12]), "=&v"(w[13]), "=&v"(w[14]), "=&v"(w[15])
+        : "v"(st + at[0]), "v"(st + at[1]), "v"(st + at[2]), "v"(st + at[3]), "v"(st + at[4]), "v"(st + at[5]),
+          "v"(st + at[6]), "v"(st + at[7]), "i"(OFF), "i"(OFF + 4 * ROW));
+#endif
+#pragma unroll
+  for (int c = 0; c < N; ++c) v[c] = u32x4_t{w[2 * c][0], w[2 * c][1], w[2 * c + 1][0], w[2 * c + 1][1]};
+}
+
 // Few rows (decode): 16 rows of one (sequence, KV head) for a workgroup, bound by the keys and values that
 // it streams.  Every wave takes 32-key blocks of its own, so nothing waits at a barrier until the waves'
 // sums are joined at the end: K of the next block comes into registers, where the product wants it, V of
@@ -354,21 +398,8 @@ __device__ __forceinline__ void pf_segment(const AttnParams& p, PfShared<D>& lds
         lo[i] = pack_bf16x2(e0 - bf16_bits_to_f32(hi[i] & 0xffffu), e1 - __uint_as_float(hi[i] & 0xffff0000u));
       }
       u32x4_t vf[ND];
-#pragma unroll
-      for (int c = 0; c < ND; ++c)
-        static_for<2>([&](auto t_c) __attribute__((always_inline)) {
-          constexpr int tt = decltype(t_c)::value;
-          u32x2_t w2 = {0u, 0u};
-#if defined(__HIP_DEVICE_COMPILE__)
-          // inline asm: the builtin would also wait for the loads into LDS that are in flight
-          asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(w2) : "v"(st + v_rd[c]), "i"(4 * tt * L::ROW));
-#endif
-          vf[c][2 * tt] = w2[0];
-          vf[c][2 * tt + 1] = w2[1];
-        });
-      // the results are valid after lgkmcnt(0), which the compiler does not know of
-      __builtin_amdgcn_s_waitcnt(0xC07F);
-      __builtin_amdgcn_sched_barrier(0);
+      read_v<ND, 0, L::ROW>(vf, st, v_rd);
+      __builtin_amdgcn_sched_barrier(0);  // nothing that the next block asks for comes before
       // V has been read: its place takes the block after next
       fetch(base + 2 * STEP, stage);
       seen_now = seen_next;
@@ -627,21 +658,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     static_for<4>([&](auto ks_c) __attribute__((always_inline)) {
       constexpr int ks = decltype(ks_c)::value;
       u32x4_t vf[NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        static_for<2>([&](auto t_c) __attribute__((always_inline)) {
-          constexpr int tt = decltype(t_c)::value;
-          u32x2_t w2 = {0u, 0u};
-#if defined(__HIP_DEVICE_COMPILE__)
-          // inline asm: the builtin would also wait for the loads into LDS that are in flight
-          asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
-                       : "=v"(w2)
-                       : "v"(st + v_rd[c]), "i"((16 * ks + 4 * tt) * L::ROW));
-#endif
-          vf[c][2 * tt] = w2[0];
-          vf[c][2 * tt + 1] = w2[1];
-        });
-      }
       u32x4_t lo;
       {
         constexpr int kb = ks >> 1, base = 8 * (ks & 1);
@@ -650,8 +666,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
           lo[w2] = pack_bf16x2(sc[kb][base + 2 * w2] - bf16_bits_to_f32(hi[ks][w2] & 0xffffu),
                                sc[kb][base + 2 * w2 + 1] - __uint_as_float(hi[ks][w2] & 0xffff0000u));
       }
-      // the results are valid after lgkmcnt(0), which the compiler does not know of
-      __builtin_amdgcn_s_waitcnt(0xC07F);
+      read_v<NC, 16 * ks * L::ROW, L::ROW>(vf, st, v_rd);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
