@@ -1019,6 +1019,8 @@ PaPlan pa_plan(int64_t n_heads, int64_t n_kv, int64_t d, int64_t n_seqs, int64_t
   pl.share = one_each && g <= PF_ROWS && n_seqs > 1 && n_seqs <= PF_SEQS && max_kv > 1024 * (int64_t)std::max(pl.pieces, 2)
                  ? (int)std::max<int64_t>(1, std::min<int64_t>((d <= 64 ? 3 : 2) * (int64_t)cus / n_kv, PF_SHARES))
                  : 0;
+  // The joins have a workgroup for each row and head.  Only a max_q_len far below the sequences' rows cuts so many.
+  if (total_q * n_heads > host_most_groups(256)) pl.pieces = 1, pl.share = 0;
   return pl;
 }
 
@@ -1068,9 +1070,6 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
   if (st != MI_OK) return st;
   PaPlan plan = pa_plan(n_heads, cache->n_kv, d, seqs->n_seqs, rows, max_q_len, max_kv_len, !seqs->q_start, host_cus());
   if (seqs->n_seqs * (seqs->max_pages * cache->page_size / PF_BLOCK + 1) > INT32_MAX) plan.share = 0;  // its sums
-  // The joins have a workgroup for each row and head.  Only a max_q_len far below the sequences' rows cuts so many.
-  const int64_t most = host_most_groups(256);
-  if (rows * n_heads > most) plan.pieces = 1, plan.share = 0;
   // as many pieces as the workspace holds
   const int64_t piece_bytes = rows * n_heads * (d + 1) * 4;
   if (!workspace) plan.pieces = 1;
@@ -1114,7 +1113,7 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
     }
     return e == hipSuccess ? MI_OK : host_fail(MI_ERR_HIP, "paged_attn launch: %s", hipGetErrorString(e));
   }
-  const int64_t grid = plan.tiles * p.n_kv * plan.pieces;
+  const int64_t grid = plan.tiles * p.n_kv * plan.pieces, most = host_most_groups(256);
   if (grid > most)
     return host_fail(MI_ERR_SHAPE, "%lld row tiles of %lld KV heads: more than %lld workgroups", (long long)plan.tiles,
                      (long long)cache->n_kv, (long long)most);

@@ -89,3 +89,10 @@ def test_where_even_shares_begin(mi):
         assert f(16, 4, 128, S, S, 1, border) == (pieces * S * 16 * 129 * 4 if pieces > 1 else 0)
         assert f(16, 4, 128, S, S, 1, border + 1) == max(parts(128, S), pieces * S * 16 * 129 * 4 if pieces > 1 else 0)
     assert f(16, 4, 128, 1, 1, 1, 10 ** 6) == 64 * 16 * 129 * 4  # one sequence: pieces
+
+
+def test_rows_that_no_join_could_be_launched_for(mi):
+    """The call does not cut them, whatever max_q_len says, and asks for no room to."""
+    f = mi.paged_attn_workspace_size
+    assert f(16, 4, 128, 1, 1 << 20, 1, 1 << 20) == 0
+    assert f(16, 4, 128, 1, (1 << 20) - 1, 1, 1 << 20) > 0
