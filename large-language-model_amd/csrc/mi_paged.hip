@@ -6,18 +6,19 @@
 //
 // Bound by reading the keys once for a KV head's group where rows are few, by the matrix cores where they
 // are many.  Few rows (decode) have kernels of their own below: 64 sequences of up to 8000 keys, 372 MB in
-// 79 us (4.7 TB/s; equal lengths reach 5.3 to 5.9, plain reads 6.0); one of 2048 keys takes 11 us, two
-// launches.  Many: 4096 rows over 8192 keys in 242 us (850 TFLOP/s), 4 chunks of up to 1024 rows over 4095
-// in 60 (509).  What keeps these from the rate of a large product is LDS: each of four waves reads all of a
-// block's K and V, 128 KB, beside a chain of product, maximum, exponentials and product; computing the next
-// block's scores under the exponentials instead only took registers (66 -> 72 us).
+// 78 us (4.8 TB/s; equal lengths reach 5.3 to 5.9, plain reads 6.0); one of 2048 keys takes 11 us, two
+// launches.  Many: 4096 rows over 8192 keys in 317 us (650 TFLOP/s of the formula's operations, half as many
+// again are done), 4 chunks of up to 1024 rows over 4095 in 73 (420).  There the matrix cores are busy for 53 and
+// 44 % of the busy CUs' clocks, LDS for 18 and 15 %, and waits for LDS are 3 and 2 % of the waves' cycles: what is
+// left is each wave's chain of product, maximum, exponentials and product, with two waves on a SIMD to hide it.
+// Computing the next block's scores under the exponentials instead only took registers (66 -> 72 us).
 //
 // A workgroup owns 128 rows of one (sequence, KV head), the group's query heads of a token side by side,
 // so one pass over K and V serves all of them; it streams 64-key blocks through a two-stage LDS ring.
 // P goes into its product with V as the sum of two bf16, in every kernel: what is left out is 2^-16 of a weight,
-// so an output is as exact as its own rounding, whichever rows share its tile.  Rounded to one bf16 the weights
-// of many rows cost a product less, 65 us in place of 79 (4 chunks of up to 1024 rows over 4095 keys) and 259 of
-// 335 (4096 over 8192), but outputs are off by up to 2^-8 of sum p |v| more than those of decode.
+// so an output is as exact as its own rounding, whichever rows share its tile.  Many rows pay 21 % for the second
+// product (4 chunks of up to 1024 rows over 4095 keys) and 29 % (4096 over 8192); with one bf16 their outputs were
+// off by up to 2^-8 of sum p |v| more than those of decode.
 // Blocks are gathered row by row from the pages, straight into LDS.  Keys beyond the sequence, in bad
 // pages or past head_dim are read from zeros: what a page holds past the sequence may be anything.
 #include <hip/hip_runtime.h>
@@ -489,8 +490,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
 
   // this lane's row; rows past the sequence's last one repeat it and are not stored
   const int n_packed = min(t.n * p.group - t.first, PA_ROWS);
-  // Decode rows beside prompts, and the ends of those: all four waves at one row tile (a prompt of 500 and 63
-  // rows over 4000 keys each: 114 us, 121 without; with 12 heads of 64 and 30 uneven rows 38 and 41.5).
+  // Decode rows beside prompts, and the ends of those: all four waves at one row tile (chunks of 500 and 63 rows over
+  // 4000 keys: 44.9 us, 47.9 without; one of 500 and 63 single rows: 132.8, 129.8; 30 of up to 97 rows, 12 heads of
+  // 64: 52.4, 53.0).
   if (n_packed <= PF_ROWS) {
     pf_segment<D>(p, lds.few, t, kvh, k_begin, k_end, whole,
                   [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
@@ -777,7 +779,7 @@ __device__ __forceinline__ int pa_pieces_of(const AttnParams& p, PaTile t, int r
 
 // One new token for each sequence: the keys of all sequences, in blocks of PF_BLOCK, are one line that the
 // workgroups of a KV head share evenly, so that sequences of any lengths keep all CUs busy to the end
-// (64 sequences of 500 to 8000 keys, 372 MB: 79 us, in pieces 92 at best).  A workgroup's share lies
+// (64 sequences of 500 to 8000 keys, 372 MB: 78 us, in pieces 88 at best).  A workgroup's share lies
 // in one sequence or runs over several; only its first and its last may be cut.
 constexpr int PF_BLOCK = PF_KEYS * PF_WAVES;
 constexpr int PF_SEQS = 1024;   // sequences whose lengths a workgroup sums up
@@ -994,9 +996,9 @@ struct PaPlan {
 //                even   34.0/39.3    43.1/47.8   180.0/188    137/142     179/185     28.7/29.9    45.6/49.1
 // Many rows: pieces of 512 keys at least until there are two workgroups for each CU, which fit at once; four
 // where the sequences are eight or more, of which some are short. With two / four, uneven lengths and even:
-//    sequences, rows over keys   6, 64/6000  8, 64/6000  32, 64/6000  6, 700/1400  10, 700/1400  4, 1024/4095  10, 1024/4095
-//                       uneven   39.6/38.5   39.5/38.0   83.7/64.0    38.6/38.9    45.4/39.4     75.3/81.0     109.8/97.7
-//                         even   59.5/63.4   68.9/71.2   228.7/203.9  77.7/92.8    109.3/140.4   182.8/196.4   449.3/449.7
+//    sequences: rows/keys  6: 64/6000  8: 64/6000  32: 64/6000  6: 700/1400  10: 700/1400  4: 1024/4095  10: 1024/4095
+//                 uneven   39.6/38.5   39.5/38.0   83.7/64.0    38.6/38.9    45.4/39.4     75.3/81.0     109.8/97.7
+//                   even   59.5/63.4   68.9/71.2   228.7/203.9  77.7/92.8    109.3/140.4   182.8/196.4   449.3/449.7
 // Where that leaves CUs empty, pieces of 256 or 128 keys. One sequence, rows over keys, with 128 / 256 / 512:
 // 8 over 4000 13.1/15.1/21.0, 17 over 2000 13.6/16.1/22.5 (128 taken), 64 over 4000 26.4/22.1/24.9 (128 taken, 4 us
 // too many), 4 sequences of 64 over 2000 32.9/27.3/26.4 (256 taken).

@@ -743,10 +743,13 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleParams p) {
 // their bits, 32768 counters of 16 bits in LDS, and listed in order with their counts, so only the
 // distinct ones are weighed and all three borders lie in running sums over the list.  The second pass
 // takes each token's weight from LDS by its bits.  The answers are those of the kernel above, to the bit.
-// Normal logits, top-p 0.9, without / with it (us):
-//             8192       16384      32000      131072 logits
-//    64 rows  16.6/15.7  22.7/17.8  35.4/23.9  113/60
-//   512 rows  22.7/19.4  34.0/25.4  60.0/38.8  240/119    (4096 logits: 15.4/16.5)
+// Normal logits of standard deviation 2.5, top-p 0.9, without / with it (us):
+//             4096       8192       16384      32000      131072 logits
+//    64 rows  13.9/14.7  15.0/15.3  20.7/18.1  33.3/23.4  102/59
+//   512 rows  15.1/17.1  20.9/19.9  31.6/25.6  54.8/39.2  213/117
+// Where a row is so flat that more distinct logits are kept than there is room for weights, it takes both: 64 rows of
+// 32000 with top-p 0.9, deviations of 0.5, 1, 1.5 and 4: 36.2/48.2, 36.6/47.6, 35.6/23.6, 28.8/23.4; with top-p 0.99, 1,
+// 2 and 2.5: 35.3/46.7, 36.5/47.8, 35.3/23.6.
 // LDS and vector instructions bound it: of a row's 17 us alone 4 go to the counting, 4 to the second
 // pass, 7 to the list and its sums.  80 KB of LDS leave room for two blocks of 512 threads on a CU.
 constexpr int SMC_LIST = 3584;          // distinct logits of a row
@@ -1097,8 +1100,8 @@ __device__ __forceinline__ bool sample_counted(const SampleParams& p, int row, f
   return true;
 }
 
-// Whether a border is looked for among many tokens.  (64 rows of 32000: top-k 200 21.6 us without counts,
-// 25.6 with; top-k 1000 27.6 and 23.2; min-p alone 20.1 and 24.6.)
+// Whether a border is looked for among many tokens.  (64 rows of 32000, without counts and with: top-k 200 21.0 and
+// 22.6 us, 260 24.9 and 22.6, 1000 26.6 and 23.1; min-p alone 19.5 and 29.1.)
 __host__ __device__ __forceinline__ bool counts_pay(int top_k, float top_p, int vocab) {
   return top_k > 0 && top_k < vocab ? top_k > SMP_FEW : top_p < 1.0f;
 }
@@ -1157,7 +1160,8 @@ extern "C" int mi_sample(void* stream, const void* logits, int32_t dtype, int64_
                        (how->temperature || how->temperature_all > 0.0f) &&
                        (how->top_k || how->top_p || counts_pay(how->top_k_all, how->top_p_all, (int)vocab));
   // More rows than CUs: half the threads, so that two rows share a CU and one's waits are under the
-  // other's work (512 rows of 32000 bf16 logits, top-p, by weights: 65 us with 1024 threads, 60 with 512)
+  // other's work (bf16 rows of 32000, top-p, by weights, with 1024 / 512 threads: 256 rows 37.6/44.4 us, 257
+  // 65.0/54.4, 512 72.7/63.3)
   const bool halved = rows > host_cus();
   const int threads = halved ? 512 : 1024, per_layer = threads * (bf16 ? 8 : 4);
   p.layers = (int)((vocab + per_layer - 1) / per_layer);
