@@ -473,8 +473,8 @@ int mi_kv_append(void* stream, const void* q, int64_t q_t, int64_t q_h, void* q_
  * parts, NULL: no split).  Results do not depend on timing.  Scores, sums and parts are fp32, and the
  * weights enter their product with V as the sum of two bf16 (2^-16 of each is left out), decode rows and
  * prompt rows alike: which rows share a call changes the order of sums, and so now and then the
- * output's rounding, no more.  A call of 2^24 workgroups or more (a row tile of each sequence and KV
- * head, and one for every 128 rows and heads) is refused.
+ * output's rounding, no more.  A call of 2^24 workgroups or more (a tile for each sequence and KV head,
+ * and for every 128 of total_q * n_heads, 16 where max_q_len is small) is refused.
  */
 int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h, float* lse,
                   int64_t n_heads, const mi_paged_cache* cache, const mi_paged_seqs* seqs, int64_t max_q_len,

@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][base + 2 * w2 + 1], sl2, nmc));
         sum += e0 + e1;
         hi[ks][w2] = pack_bf16x2(e0, e1);
-        sc[kb][base + 2 * w2] = e0;  // for what hi leaves, taken while V is read
+        sc[kb][base + 2 * w2] = e0;  // for what hi leaves
         sc[kb][base + 2 * w2 + 1] = e1;
       }
     }
