@@ -57,28 +57,46 @@ __device__ __forceinline__ int wave_first_false(int n, F below) {
   return lo;
 }
 
-// Checks cache and seqs of an entry point; MI_OK or an error with its text.
-inline int check_paged(const mi_paged_cache* c, const mi_paged_seqs* s) {
-  if (!c || !s) return host_fail(MI_ERR_NULL, "cache or seqs is NULL");
-  if (s->n_seqs < 0 || s->total_q < 0 || s->max_pages < 0 || c->num_pages < 0 || c->n_kv < 0 || c->head_dim < 0)
+// Checks the sizes and tables of an entry point's cache and seqs; MI_OK or an error with its text.  any: whether there
+// are tokens at all.
+inline int check_pages(int64_t num_pages, int64_t page_size, int64_t n_kv, int64_t head_dim, const mi_paged_seqs* s,
+                       bool& any) {
+  any = false;
+  if (s->n_seqs < 0 || s->total_q < 0 || s->max_pages < 0 || num_pages < 0 || n_kv < 0 || head_dim < 0)
     return host_fail(MI_ERR_SHAPE, "negative size");
-  if (s->n_seqs > INT32_MAX || s->total_q > INT32_MAX || s->max_pages > INT32_MAX || c->num_pages > INT32_MAX ||
-      c->n_kv > INT32_MAX)
+  if (s->n_seqs > INT32_MAX || s->total_q > INT32_MAX || s->max_pages > INT32_MAX || num_pages > INT32_MAX ||
+      n_kv > INT32_MAX)
     return host_fail(MI_ERR_SHAPE, "size exceeds 2^31-1");
-  if (c->page_size < 1 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)))
-    return host_fail(MI_ERR_SHAPE, "page_size=%lld is not a power of two up to 2^20", (long long)c->page_size);
+  if (page_size < 1 || page_size > (1 << 20) || (page_size & (page_size - 1)))
+    return host_fail(MI_ERR_SHAPE, "page_size=%lld is not a power of two up to 2^20", (long long)page_size);
   if (!s->q_start && s->total_q != s->n_seqs)
     return host_fail(MI_ERR_SHAPE, "total_q=%lld for %lld sequences without q_start", (long long)s->total_q,
                      (long long)s->n_seqs);
-  if (s->max_pages * c->page_size > INT32_MAX - 4096)
+  if (s->max_pages * page_size > INT32_MAX - 4096)
     return host_fail(MI_ERR_SHAPE, "max_pages * page_size = %lld exceeds 2^31 - 4096",
-                     (long long)(s->max_pages * c->page_size));
+                     (long long)(s->max_pages * page_size));
   if (s->pages_ld < s->max_pages)
     return host_fail(MI_ERR_LD, "pages_ld=%lld < max_pages=%lld", (long long)s->pages_ld, (long long)s->max_pages);
   if (s->n_seqs == 0 || s->total_q == 0) return MI_OK;
   if (!s->kv_len || (s->max_pages > 0 && !s->pages)) return host_fail(MI_ERR_NULL, "kv_len or pages is NULL");
   if (((uintptr_t)s->q_start | (uintptr_t)s->kv_len | (uintptr_t)s->pages) & 3)
     return host_fail(MI_ERR_UNSUPPORTED, "q_start, kv_len and pages must be aligned to their element size");
+  any = true;
+  return MI_OK;
+}
+
+// Whether rows of `row` elements or bytes, that far apart, could share memory.
+inline bool rows_overlap(int64_t num_pages, int64_t page_size, int64_t n_kv, int64_t row, int64_t page_stride,
+                         int64_t head_stride, int64_t slot_stride) {
+  return (page_size > 1 && slot_stride < row) || (n_kv > 1 && head_stride < row) || (num_pages > 1 && page_stride < row);
+}
+
+// Checks cache and seqs of an entry point; MI_OK or an error with its text.
+inline int check_paged(const mi_paged_cache* c, const mi_paged_seqs* s) {
+  if (!c || !s) return host_fail(MI_ERR_NULL, "cache or seqs is NULL");
+  bool any;
+  const int st = check_pages(c->num_pages, c->page_size, c->n_kv, c->head_dim, s, any);
+  if (st != MI_OK || !any) return st;
   if (c->num_pages > 0 && (!c->k || !c->v)) return host_fail(MI_ERR_NULL, "cache k or v is NULL");
   if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
     return host_fail(MI_ERR_UNSUPPORTED, "cache k and v must be 16-byte aligned");
@@ -86,8 +104,7 @@ inline int check_paged(const mi_paged_cache* c, const mi_paged_seqs* s) {
     return host_fail(MI_ERR_UNSUPPORTED, "head_dim %lld: a multiple of 8 is needed", (long long)c->head_dim);
   if ((c->page_stride | c->head_stride | c->slot_stride) % 8)
     return host_fail(MI_ERR_UNSUPPORTED, "cache strides must be multiples of 8 elements");
-  if ((c->page_size > 1 && c->slot_stride < c->head_dim) || (c->n_kv > 1 && c->head_stride < c->head_dim) ||
-      (c->num_pages > 1 && c->page_stride < c->head_dim))
+  if (rows_overlap(c->num_pages, c->page_size, c->n_kv, c->head_dim, c->page_stride, c->head_stride, c->slot_stride))
     return host_fail(MI_ERR_LD, "a cache stride is shorter than a row of %lld", (long long)c->head_dim);
   return MI_OK;
 }
