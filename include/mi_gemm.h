@@ -483,6 +483,73 @@ int mi_paged_attn(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O
 size_t mi_paged_attn_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t n_seqs, int64_t total_q,
                                     int64_t max_q_len, int64_t max_kv_len);
 
+/* How a mi_quant_cache holds a component. */
+typedef enum mi_kv_format {
+  MI_KV_E4M3 = 0, /* 8 bits: sign, 4 bits of exponent, 3 of fraction, up to 448             */
+  MI_KV_E2M1 = 1  /* 4 bits: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives; component 2i in
+                     the low half of byte i, 2i+1 in the high half                          */
+} mi_kv_format;
+
+/*
+ * A paged cache of K and V in 8 or 4 bits.  32 neighbouring components of a head of a token are a
+ * group that shares a power of two: with m their largest magnitude, e is the least integer with
+ * m <= L * 2^e, at least -100, where L is 464 (e4m3) or 7 (e2m1), so that the largest, too, is off by
+ * half a step at most; the group's scale byte is e + 127 and each code is x / 2^e rounded to the
+ * nearest number of the type, ties to even, at most 448 or 6.  A group with an infinity, a NaN or a
+ * magnitude of 2^127 or more has scale byte 255, codes 0, and reads back as NaN.  Every value read
+ * back is exact in bf16.  Pages as in mi_paged_cache: the codes of head h of slot i of page p are the
+ * head_dim (e4m3) or head_dim / 2 (e2m1) bytes at k + p*page_stride + h*head_stride + i*slot_stride, their
+ * scale bytes the head_dim / 32 at k_scale + p*scale_page_stride + h*scale_head_stride + i*scale_slot_stride,
+ * and v alike.  head_dim is a multiple of 32; k and v are 16-byte aligned and the strides of codes
+ * multiples of 16 bytes; scale bytes may lie anywhere.
+ */
+typedef struct mi_quant_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t num_pages;
+  int64_t page_size; /* a power of two */
+  int64_t n_kv, head_dim;
+  int64_t page_stride, head_stride, slot_stride;                   /* bytes */
+  int64_t scale_page_stride, scale_head_stride, scale_slot_stride; /* bytes */
+  int32_t format;   /* mi_kv_format */
+  int32_t reserved; /* 0 */
+} mi_quant_cache;
+
+/*
+ * mi_kv_append into a cache of 8 or 4 bits: K is rotated in 64 bits and quantised as it is written (rounded
+ * once, to its code), V quantised, Q rotated in 32 bits and rounded to bf16.  Arguments as there; head_dim
+ * at most 1024.
+ */
+int mi_kv_append_quant(void* stream, const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h,
+                       int64_t n_heads, const void* k, int64_t k_t, int64_t k_h, const void* v, int64_t v_t, int64_t v_h,
+                       const mi_quant_cache* cache, const mi_paged_seqs* seqs, const mi_rotary* rotary);
+
+/*
+ * The tokens of seqs, which mi_kv_append_quant names as its new ones (the last q_start[s+1] - q_start[s] of
+ * kv_len[s]; all of a sequence's where they are as many), read back: K and V [total_q, n_kv, head_dim] of
+ * dtype MI_BF16 or MI_F32 (exact in both), element strides k_t, v_t between tokens and k_h, v_h between heads,
+ * components contiguous.  k or v may be NULL: not read.  A token that no page holds is written as zeros; rows
+ * behind the last sequence are left as they are.
+ */
+int mi_kv_read_quant(void* stream, void* k, int64_t k_t, int64_t k_h, void* v, int64_t v_t, int64_t v_h, int32_t dtype,
+                     const mi_quant_cache* cache, const mi_paged_seqs* seqs);
+
+/*
+ * mi_paged_attn over a cache of 8 or 4 bits: its results are those of mi_paged_attn over the values that
+ * the cache stands for.  Arguments, workspace and refusals as there; head_dim 32, 64, 96 or 128.  A group that
+ * reads back as NaN makes the output NaN of every row that sees it (of V: in that group's components), and may do
+ * so in the sequence's rows before it.
+ */
+int mi_paged_attn_quant(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h,
+                        float* lse, int64_t n_heads, const mi_quant_cache* cache, const mi_paged_seqs* seqs,
+                        int64_t max_q_len, int64_t max_kv_len, int32_t causal, float scale, void* workspace,
+                        size_t workspace_bytes);
+
+size_t mi_paged_attn_quant_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t n_seqs,
+                                          int64_t total_q, int64_t max_q_len, int64_t max_kv_len);
+
 /*
  * How mi_sample picks.  A device pointer gives every row its own value ([rows]); where it is
  * NULL the value beside it holds for all rows.

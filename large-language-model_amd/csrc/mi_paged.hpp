@@ -1,5 +1,6 @@
 // mi_paged.hpp -- device view of a paged K/V cache and of the sequences of one call, shared by
-// the append (mi_rope.hip) and the attention (mi_paged.hip).
+// the append (mi_rope.hip), the attention (mi_paged.hip) and their forms for a cache of 8 or 4 bits
+// (mi_kv_quant.hip, mi_paged_quant.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -13,7 +14,7 @@ struct PagedView {
   const int32_t* kv_len;
   const int32_t* pages;
   int64_t pages_ld;
-  int64_t page_stride, head_stride, slot_stride;  // elements
+  int64_t page_stride, head_stride, slot_stride;  // elements (bytes of codes in a cache of 8 or 4 bits)
   int n_seqs, total_q, max_pages, num_pages, page_shift;
 };
 
@@ -109,7 +110,35 @@ inline int check_paged(const mi_paged_cache* c, const mi_paged_seqs* s) {
   return MI_OK;
 }
 
-inline PagedView paged_view(const mi_paged_cache* c, const mi_paged_seqs* s) {
+// The same for a cache of 8 or 4 bits.
+inline int check_quant(const mi_quant_cache* c, const mi_paged_seqs* s) {
+  if (!c || !s) return host_fail(MI_ERR_NULL, "cache or seqs is NULL");
+  if (c->format != MI_KV_E4M3 && c->format != MI_KV_E2M1) return host_fail(MI_ERR_DTYPE, "format %d", c->format);
+  if (c->reserved != 0) return host_fail(MI_ERR_SHAPE, "reserved must be 0");
+  bool any;
+  const int st = check_pages(c->num_pages, c->page_size, c->n_kv, c->head_dim, s, any);
+  if (st != MI_OK || !any) return st;
+  if (c->num_pages > 0 && (!c->k || !c->v || !c->k_scale || !c->v_scale))
+    return host_fail(MI_ERR_NULL, "cache k, v or a scale is NULL");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15)
+    return host_fail(MI_ERR_UNSUPPORTED, "cache k and v must be 16-byte aligned");
+  if (c->head_dim < 32 || c->head_dim % 32)
+    return host_fail(MI_ERR_UNSUPPORTED, "head_dim %lld: a multiple of 32 is needed", (long long)c->head_dim);
+  if ((c->num_pages > 1 && c->page_stride % 16) || (c->n_kv > 1 && c->head_stride % 16) ||
+      (c->page_size > 1 && c->slot_stride % 16))
+    return host_fail(MI_ERR_UNSUPPORTED, "strides of the codes must be multiples of 16 bytes");
+  const int64_t row = c->format == MI_KV_E2M1 ? c->head_dim / 2 : c->head_dim, groups = c->head_dim / 32;
+  if (rows_overlap(c->num_pages, c->page_size, c->n_kv, row, c->page_stride, c->head_stride, c->slot_stride))
+    return host_fail(MI_ERR_LD, "a stride of the codes is shorter than a row of %lld bytes", (long long)row);
+  if (rows_overlap(c->num_pages, c->page_size, c->n_kv, groups, c->scale_page_stride, c->scale_head_stride,
+                   c->scale_slot_stride))
+    return host_fail(MI_ERR_LD, "a stride of the scales is shorter than a row of %lld bytes", (long long)groups);
+  return MI_OK;
+}
+
+// Cache: mi_paged_cache, strides in elements, or mi_quant_cache, those of the codes in bytes.
+template <class Cache>
+inline PagedView paged_view(const Cache* c, const mi_paged_seqs* s) {
   PagedView v;
   v.q_start = s->q_start;
   v.kv_len = s->kv_len;

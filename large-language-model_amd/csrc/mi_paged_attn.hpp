@@ -1,4 +1,5 @@
-// mi_paged_attn.hpp -- what the attention over a paged cache needs whatever the cache holds: tiles of rows, pieces and even shares of the keys, a
+// mi_paged_attn.hpp -- what the attention over a paged cache has in common whatever the cache holds
+// (mi_paged.hip: bf16, mi_paged_quant.hip: 8 or 4 bits): tiles of rows, pieces and even shares of the keys, a
 // 64-key block of many rows in LDS, the join of few rows' waves, the joins of parts, and the host's plan.
 #pragma once
 #include <hip/hip_runtime.h>

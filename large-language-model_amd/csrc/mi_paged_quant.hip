@@ -1,0 +1,399 @@
+// mi_paged_quant.hip -- attention of new tokens over a paged K/V cache of 8 or 4 bits, gfx950.
+//
+// The formula, the tiles, pieces, shares and joins are those of the cache in bf16 (mi_paged.hip, mi_paged_attn.hpp);
+// here the keys and values come as codes and a power of two for 32 of them.  The conversion gives two bf16 at once
+// and multiplies on the way, both exactly, so scores and sums are those of a bf16 cache that holds the values
+// which the codes stand for.
+//
+// A quarter of a row (head_dim / 4 components, within one group) is what a lane loads and converts.
+#include <hip/hip_runtime.h>
+
+#include "mi_kv_quant.hpp"
+#include "mi_paged_attn.hpp"
+
+namespace mig {
+namespace {
+
+struct QuantParams : AttnParams {
+  const uint8_t *ks, *vs;
+  int64_t scale_page, scale_head, scale_slot;
+};
+
+// A quarter of a row of up to D components: its codes, and how they become bf16.
+template <int D, int BITS>
+struct Quarter {
+  static constexpr int COMPS = D / 4, BYTES = COMPS * BITS / 8, EIGHTS = COMPS / 8;
+  uint32_t w[BYTES / 4];
+  uint32_t scale;  // the byte
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
+    if constexpr (BYTES == 8) *(u32x2_t*)w = *(const u32x2_t*)codes;
+    else
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) ((u32x4_t*)w)[i] = ((const u32x4_t*)codes)[i];
+    scale = *scales;
+  }
+  __device__ __forceinline__ u32x4_t eight(int i) const { return kv_eight<BITS>(w + i * (BITS / 4), kv_power(scale)); }
+};
+
+// Codes and scale bytes of keys that no row sees, and of components past head_dim: zeros times 2^-127.
+__device__ __align__(16) uint32_t pq_zero[8];
+
+// Few rows: V of a 32-key block of a wave, converted, rows of D components whose 16-byte chunks are moved so that
+// the writes of two rows' quarters, and the transposing reads, lie in different banks.
+template <int D>
+struct PqLds {
+  static constexpr int ROW = D * 2;
+  static constexpr int V_BYTES = PF_KEYS * ROW;
+  static constexpr int SUM_BYTES = PF_ROWS * PF_PITCH<D> * 4;
+  static constexpr int BYTES = V_BYTES > SUM_BYTES ? V_BYTES : SUM_BYTES;
+  __device__ static __forceinline__ int v_pos(int r, int c) {
+    if constexpr (D == 128) return c ^ ((r & 3) << 2) ^ (((r >> 3) & 1) << 1) ^ (r & 1);
+    else return c ^ (((r >> 1) & 1) << 2) ^ (((r >> 3) & 1) << 1);
+  }
+};
+
+template <int D>
+struct PqShared {
+  __attribute__((aligned(16))) char v[PF_WAVES * PqLds<D>::BYTES];
+  int table[PF_TABLE];
+  PfWaves waves;
+};
+
+// Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
+// part, at part_at(row of the sequence, head).  Every wave takes 32-key blocks of its own, whose codes come into
+// registers DEPTH blocks ahead.
+template <int D, int BITS, class PartAt>
+__device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& lds, const PaTile& t, int kvh, int k_begin,
+                                           int k_end, bool whole, PartAt part_at) {
+  using L = PqLds<D>;
+  using Q4 = Quarter<D, BITS>;
+  constexpr int NS = D / 32, ND = D / 16, DEPTH = BITS == 4 ? 3 : 2;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int g = lane >> 4, l16 = lane & 15;
+  const uint32_t vlds = lds_addr(lds.v) + (uint32_t)(wave * L::BYTES);
+
+  const int n_packed = min(t.n * p.group - t.first, PF_ROWS);
+  const int pr = t.first + min(l16, n_packed - 1);
+  const int token = pr / p.group, head = kvh * p.group + pr - token * p.group;
+  const int lim = t.limit(p, token), lim_lo = t.limit(p, t.first / p.group);
+
+  // lane (g, l16) holds the components of quarter g of K's row and of Q's: product s takes eight of each quarter
+  u32x4_t qf[NS];
+  {
+    const uint16_t* qr = p.q + (int64_t)(t.q0 + token) * p.q_t + (int64_t)head * p.q_h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int c = Q4::COMPS * g + 8 * s;
+      qf[s] = c < p.d ? *(const u32x4_t*)(qr + c) : u32x4_t{0, 0, 0, 0};
+    }
+  }
+
+  const int shift = p.pv.page_shift;
+  const int64_t slot_stride = p.pv.slot_stride;
+  const uint8_t* kbase = (const uint8_t*)p.k + kvh * p.pv.head_stride;
+  const uint8_t* vbase = (const uint8_t*)p.v + kvh * p.pv.head_stride;
+  const uint8_t* ksbase = p.ks + kvh * p.scale_head;
+  const uint8_t* vsbase = p.vs + kvh * p.scale_head;
+  int first_page = 0, k_stop = 0;  // the table holds the pages of the keys before k_stop
+
+  // Tile i of the scores: row r reads key 8 (r / 4) + 4i + r % 4, so that the eight scores of a lane are, in
+  // order, the run of keys that the second operand of P V takes.  V: row 16u + lane / 4, quarter lane % 4.
+  const int k_row = 8 * (l16 >> 2) + (l16 & 3), v_row = lane >> 2, v_q = lane & 3;
+  const bool k_in = Q4::COMPS * g < p.d, v_in = Q4::COMPS * v_q < p.d;  // d is a multiple of 32: whole quarters
+  const int k_code = Q4::BYTES * g, k_scale = Q4::COMPS * g / KV_GROUP;
+  const int v_code = Q4::BYTES * v_q, v_scale = Q4::COMPS * v_q / KV_GROUP;
+  struct Block {
+    Q4 k[2], v[2];
+    uint32_t seen;  // its keys that exist
+  } ring[DEPTH];
+  auto fetch = [&](Block& b, int base) __attribute__((always_inline)) {
+    const int last = k_stop - 1, pos = base + (lane & 31);
+    const int page = lds.table[(min(pos, last) >> shift) - first_page];
+    const bool there = pos < k_stop && (uint32_t)page < (uint32_t)p.pv.num_pages;
+    const int slot = pos & ((1 << shift) - 1);
+    const int64_t off = there ? page * p.pv.page_stride + slot * slot_stride : -1;
+    const int64_t soff = page * p.scale_page + slot * p.scale_slot;
+    b.seen = (uint32_t)__ballot(there);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t o = __shfl(off, k_row + 4 * i, 64), so = __shfl(soff, k_row + 4 * i, 64);
+      const bool ok = o >= 0 && k_in;
+      b.k[i].load(ok ? kbase + o + k_code : (const uint8_t*)pq_zero, ok ? ksbase + so + k_scale : (const uint8_t*)pq_zero);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t o = __shfl(off, 16 * u + v_row, 64), so = __shfl(soff, 16 * u + v_row, 64);
+      const bool ok = o >= 0 && v_in;
+      b.v[u].load(ok ? vbase + o + v_code : (const uint8_t*)pq_zero, ok ? vsbase + so + v_scale : (const uint8_t*)pq_zero);
+    }
+  };
+
+  uint32_t v_rd[ND], v_wr[2][Q4::EIGHTS];
+#pragma unroll
+  for (int c = 0; c < ND; ++c) {
+    const int r = 8 * g + (l16 >> 2), col = 16 * c + 4 * (l16 & 3);
+    v_rd[c] = (uint32_t)(r * L::ROW + 16 * L::v_pos(r, col >> 3) + (col & 7) * 2);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < Q4::EIGHTS; ++j) {
+      const int r = 16 * u + v_row;
+      v_wr[u][j] = (uint32_t)(r * L::ROW + 16 * L::v_pos(r, Q4::EIGHTS * v_q + j));
+    }
+
+  f32x4_t o[ND];
+#pragma unroll
+  for (int c = 0; c < ND; ++c) o[c] = f32x4_t{0, 0, 0, 0};
+  float m_run = -INFINITY, l_run = 0.0f;
+  const float sl2 = p.scale_log2;
+
+  auto work = [&](const Block& b, int base) __attribute__((always_inline)) {
+    f32x4_t sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b.k[i].eight(s)),
+                                                       __builtin_bit_cast(bf16x8_t, qf[s]), sc[i], 0, 0, 0);
+    // V goes through LDS to its transposing reads
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < Q4::EIGHTS; ++j) *(lds_u32x4_t*)(uintptr_t)(vlds + v_wr[u][j]) = b.v[u].eight(j);
+    // sc[t][e] is key 8g + 4t + e of row l16
+    if (base + PF_KEYS > lim_lo || b.seen != ~0u) {
+      const int room = lim - base;
+      const uint32_t bits = (room >= 32 ? b.seen : room <= 0 ? 0u : b.seen & ((1u << room) - 1)) >> (8 * g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sc[i >> 2][i & 3] = (bits >> i) & 1 ? sc[i >> 2][i & 3] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_old = m_run;
+    const bool fresh = m_old == -INFINITY, raise = !fresh && (mx - m_old) * sl2 > PA_TAU;
+    const float m_ref = fresh || raise ? mx : m_old;
+    if (__any(raise)) {
+      const float alpha = raise ? __builtin_amdgcn_exp2f((m_old - m_ref) * sl2) : 1.0f;
+      l_run *= alpha;
+#pragma unroll
+      for (int c = 0; c < ND; ++c) o[c] *= alpha;
+    }
+    m_run = m_ref;
+    const float nmc = m_ref == -INFINITY ? 0.0f : -m_ref * sl2;
+    u32x4_t hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 1][2 * (i & 1)], sl2, nmc));
+      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 1][2 * (i & 1) + 1], sl2, nmc));
+      l_run += e0 + e1;
+      hi[i] = pack_bf16x2(e0, e1);
+      lo[i] = pack_bf16x2(e0 - bf16_bits_to_f32(hi[i] & 0xffffu), e1 - __uint_as_float(hi[i] & 0xffff0000u));
+    }
+    // LDS serves a wave in order: the reads follow the writes
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4_t vf[ND];
+    read_v<ND, 0, L::ROW>(vf, vlds, v_rd);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < ND; ++c) {
+      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
+                                                    __builtin_bit_cast(bf16x8_t, lo), o[c], 0, 0, 0);
+      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
+                                                    __builtin_bit_cast(bf16x8_t, hi), o[c], 0, 0, 0);
+    }
+  };
+
+  constexpr int STEP = PF_KEYS * PF_WAVES;
+  // keys whose pages the table holds, wherever in a page they begin
+  const int k_span = (int)min((int64_t)(PF_TABLE - 1) << shift, (int64_t)1 << 30) / STEP * STEP;
+  for (int k_first = k_begin; k_first < k_end; k_first = k_stop) {
+    if (k_first > k_begin) __syncthreads();  // everyone is done with the table
+    k_stop = k_first + min(k_span, k_end - k_first);
+    first_page = k_first >> shift;
+    const int n_pages = ((k_stop - 1) >> shift) - first_page + 1;
+    for (int i = threadIdx.x; i < n_pages; i += 64 * PF_WAVES)
+      lds.table[i] = p.pv.pages[(int64_t)t.s * p.pv.pages_ld + first_page + i];
+    __syncthreads();
+    int base = k_first + PF_KEYS * wave;
+    static_for<DEPTH>([&](auto i) __attribute__((always_inline)) {
+      if (base + STEP * i < k_stop) fetch(ring[i], base + STEP * i);
+    });
+    while (base < k_stop)
+      static_for<DEPTH>([&](auto i) __attribute__((always_inline)) {
+        if (base >= k_stop) return;
+        work(ring[i], base);
+        if (base + STEP * DEPTH < k_stop) fetch(ring[i], base + STEP * DEPTH);
+        base += STEP;
+      });
+  }
+  __syncthreads();  // V's place takes the waves' sums
+  pf_join_waves<D>(p, lds.v, L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at);
+}
+
+// Many rows: a workgroup converts each 64-key block once, into LDS as the cache in bf16 would have it, and its waves
+// multiply from there.
+template <int D, int BITS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) paged_attn_quant_kernel(QuantParams p) {
+  using L = PaLds<D>;
+  using Q4 = Quarter<D, BITS>;
+  constexpr int STAGE = 2 * L::BYTES;
+  __shared__ union {
+    __attribute__((aligned(16))) char ring[2 * STAGE];
+    PqShared<D> few;
+  } lds;
+  const uint32_t lds0 = lds_addr(lds.ring);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+
+  // KV heads innermost, the last tiles, which see the most keys, first (as in mi_paged.hip)
+  const int rest = uniform(blockIdx.x / p.n_kv), kvh = uniform(blockIdx.x - rest * p.n_kv);
+  const int piece = uniform(rest / p.tiles), x = uniform(p.tiles - 1 - (rest - piece * p.tiles));
+  const PaTile t = pa_tile(p, x);
+  if (t.s < 0) return;
+  const int end = t.end(p), plen = pa_piece(p, end);
+  if (piece > 0 && (int64_t)piece * plen >= end) return;
+  const int k_begin = piece * plen, k_end = k_begin + min(plen, end - k_begin);
+  const bool whole = plen >= end;
+
+  const int n_packed = min(t.n * p.group - t.first, PA_ROWS);
+  if (n_packed <= PF_ROWS) {
+    pq_segment<D, BITS>(p, lds.few, t, kvh, k_begin, k_end, whole,
+                        [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
+    return;
+  }
+  const bool wave_has_rows = 32 * wave < n_packed;
+  PaRows<D> rows;
+  rows.begin(p, t, kvh, wave, n_packed);
+
+  // wave w brings rows 16w .. 16w+15 of a block, a lane a quarter of row 16w + lane / 4
+  const int row = 16 * wave + (lane >> 2), quarter = lane & 3;
+  const bool in = Q4::COMPS * quarter < p.d;
+  const int code_at = Q4::BYTES * quarter, scale_at = Q4::COMPS * quarter / KV_GROUP;
+  const uint8_t* kbase = (const uint8_t*)p.k + kvh * p.pv.head_stride + code_at;
+  const uint8_t* vbase = (const uint8_t*)p.v + kvh * p.pv.head_stride + code_at;
+  const uint8_t* ksbase = p.ks + kvh * p.scale_head + scale_at;
+  const uint8_t* vsbase = p.vs + kvh * p.scale_head + scale_at;
+  uint32_t k_wr[Q4::EIGHTS], v_wr[Q4::EIGHTS];
+#pragma unroll
+  for (int j = 0; j < Q4::EIGHTS; ++j) {
+    k_wr[j] = (uint32_t)(row * L::ROW + 16 * L::k_pos(row, Q4::EIGHTS * quarter + j));
+    v_wr[j] = (uint32_t)(L::BYTES + row * L::ROW + 16 * L::v_pos(row, Q4::EIGHTS * quarter + j));
+  }
+  int page_next = -1;      // page of key `lane` of the next block to be asked for, read a block ahead of its use
+  uint64_t seen_next = 0;  // keys of the block asked for last that exist
+  Q4 kq, vq;
+  auto look_up = [&](int base) __attribute__((always_inline)) {
+    const int pos = base + lane;
+    page_next = pos < k_end ? p.pv.pages[(int64_t)t.s * p.pv.pages_ld + (pos >> p.pv.page_shift)] : -1;
+  };
+  auto fetch = [&](int base) __attribute__((always_inline)) {
+    seen_next = __ballot((uint32_t)page_next < (uint32_t)p.pv.num_pages);
+    const int page = __shfl(page_next, row, 64), slot = (base + row) & ((1 << p.pv.page_shift) - 1);
+    const bool ok = in && (uint32_t)page < (uint32_t)p.pv.num_pages;
+    const int64_t off = page * p.pv.page_stride + slot * p.pv.slot_stride;
+    const int64_t soff = page * p.scale_page + slot * p.scale_slot;
+    const uint8_t* zero = (const uint8_t*)pq_zero;
+    kq.load(ok ? kbase + off : zero, ok ? ksbase + soff : zero);
+    vq.load(ok ? vbase + off : zero, ok ? vsbase + soff : zero);
+  };
+
+  const int n_blocks = uniform((k_end - k_begin + PA_KEYS - 1) / PA_KEYS);
+  if (n_blocks > 0) {
+    look_up(k_begin);
+    fetch(k_begin);
+    look_up(k_begin + PA_KEYS);
+  }
+  for (int j = 0; j < n_blocks; ++j) {
+    const uint64_t seen = seen_next;
+    const int base = k_begin + j * PA_KEYS;
+    const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
+#pragma unroll
+    for (int i = 0; i < Q4::EIGHTS; ++i) {
+      *(lds_u32x4_t*)(uintptr_t)(st + k_wr[i]) = kq.eight(i);
+      *(lds_u32x4_t*)(uintptr_t)(st + v_wr[i]) = vq.eight(i);
+    }
+    if (j + 1 < n_blocks) {
+      fetch(base + PA_KEYS);
+      look_up(base + 2 * PA_KEYS);
+    }
+    lds_ring_barrier();  // everyone's share of block j is in place, and block j - 1 has been read
+    if (wave_has_rows) rows.block(st, base, seen);
+  }
+  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole);
+}
+
+// A tile's keys in pieces, each a workgroup's; the order of the workgroups as in mi_paged.hip.
+template <int D, int BITS>
+__global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
+    paged_attn_quant_few_kernel(QuantParams p) {
+  __shared__ PqShared<D> lds;
+  const int inner = p.n_kv * p.pieces, x = uniform(blockIdx.x / inner);
+  const int at_inner = uniform((int)((blockIdx.x % inner + (uint32_t)x % p.pieces * p.n_kv) % inner));
+  const int kvh = uniform(at_inner % p.n_kv), piece = uniform(at_inner / p.n_kv);
+  const PaTile t = pa_tile(p, x);
+  if (t.s < 0) return;
+  const int end = t.end(p), plen = pa_piece(p, end);
+  if (piece > 0 && (int64_t)piece * plen >= end) return;
+  const int k_begin = piece * plen;
+  pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_begin + min(plen, end - k_begin), plen >= end,
+                      [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
+}
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
+    paged_attn_quant_share_kernel(QuantParams p) {
+  __shared__ PqShared<D> lds;
+  __shared__ PfPrefix prefix;
+  const int kvh = uniform(blockIdx.x % p.n_kv);
+  pf_over_share(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
+                [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
+                  pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
+                });
+}
+
+template <int D, int BITS>
+int pq_launch(const QuantParams& p, const PaPlan& plan, hipStream_t hs) {
+  return pa_launch(
+      p, plan, hs, [&](unsigned wgs) { paged_attn_quant_share_kernel<D, BITS><<<wgs, 64 * PF_WAVES, 0, hs>>>(p); },
+      [&](unsigned wgs) { paged_attn_quant_few_kernel<D, BITS><<<wgs, 64 * PF_WAVES, 0, hs>>>(p); },
+      [&](unsigned wgs) { paged_attn_quant_kernel<D, BITS><<<wgs, 256, 0, hs>>>(p); });
+}
+
+}  // namespace
+}  // namespace mig
+
+using namespace mig;
+
+extern "C" {
+
+size_t mi_paged_attn_quant_workspace_size(int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t n_seqs,
+                                          int64_t total_q, int64_t max_q_len, int64_t max_kv_len) {
+  return pa_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len);
+}
+
+int mi_paged_attn_quant(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h,
+                        float* lse, int64_t n_heads, const mi_quant_cache* cache, const mi_paged_seqs* seqs,
+                        int64_t max_q_len, int64_t max_kv_len, int32_t causal, float scale, void* workspace,
+                        size_t workspace_bytes) {
+  int st = check_quant(cache, seqs);
+  if (st != MI_OK) return st;
+  QuantParams p;
+  PaPlan plan;
+  bool launch;
+  st = pa_prepare(p, plan, launch, Q, q_t, q_h, O, o_t, o_h, lse, n_heads, cache->n_kv, cache->head_dim, cache->page_size,
+                  seqs, paged_view(cache, seqs), max_q_len, max_kv_len, causal, scale, workspace, workspace_bytes);
+  if (st != MI_OK || !launch) return st;
+  p.k = cache->k, p.v = cache->v;
+  p.ks = (const uint8_t*)cache->k_scale, p.vs = (const uint8_t*)cache->v_scale;
+  p.scale_page = cache->scale_page_stride, p.scale_head = cache->scale_head_stride, p.scale_slot = cache->scale_slot_stride;
+  hipStream_t hs = (hipStream_t)stream;
+  if (cache->format == MI_KV_E2M1) return cache->head_dim <= 64 ? pq_launch<64, 4>(p, plan, hs) : pq_launch<128, 4>(p, plan, hs);
+  return cache->head_dim <= 64 ? pq_launch<64, 8>(p, plan, hs) : pq_launch<128, 8>(p, plan, hs);
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// mi_rope.hpp -- pieces of the rotation that its kernels share.
+// mi_rope.hpp -- pieces of the rotation that its kernels share (mi_rope.hip, mi_kv_quant.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>

@@ -24,6 +24,7 @@ import functools
 import math
 import os
 import struct
+from typing import NamedTuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmi_gemm.so")
@@ -42,9 +43,11 @@ C_SYMBOLS = (
     "mi_profiler_reset", "mi_gemm_noalloc", "mi_flash_attn_fwd_scaled", "mi_flash_attn_bwd_scaled",
     "mi_convert_matrices", "mi_rmsnorm_fold_weight", "mi_lm_head_xent",
     "mi_lm_head_xent_workspace_size", "mi_rope", "mi_kv_append", "mi_paged_attn",
-    "mi_paged_attn_workspace_size", "mi_sample",
+    "mi_paged_attn_workspace_size", "mi_sample", "mi_kv_append_quant", "mi_kv_read_quant",
+    "mi_paged_attn_quant", "mi_paged_attn_quant_workspace_size",
 )
 MI_ATTN_O_BHTD, MI_ATTN_O_BTHD = 0, 1
+MI_KV_E4M3, MI_KV_E2M1 = 0, 1
 
 
 class MiError(RuntimeError):
@@ -116,6 +119,17 @@ class MiPagedSeqs(ctypes.Structure):
         ("n_seqs", ctypes.c_int64), ("total_q", ctypes.c_int64), ("q_start", ctypes.c_void_p),
         ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("max_pages", ctypes.c_int64),
         ("pages_ld", ctypes.c_int64),
+    ]
+
+
+class MiQuantCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+        ("n_kv", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64),
+        ("scale_page_stride", ctypes.c_int64), ("scale_head_stride", ctypes.c_int64),
+        ("scale_slot_stride", ctypes.c_int64), ("format", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -223,6 +237,14 @@ def load_library():
                                 ctypes.c_size_t]
     L.mi_paged_attn_workspace_size.restype = ctypes.c_size_t
     L.mi_paged_attn_workspace_size.argtypes = [i64] * 7
+    L.mi_kv_append_quant.restype = ctypes.c_int
+    L.mi_kv_append_quant.argtypes = L.mi_kv_append.argtypes
+    L.mi_kv_read_quant.restype = ctypes.c_int
+    L.mi_kv_read_quant.argtypes = [vp, vp, i64, i64, vp, i64, i64, i32, vp, vp]
+    L.mi_paged_attn_quant.restype = ctypes.c_int
+    L.mi_paged_attn_quant.argtypes = L.mi_paged_attn.argtypes
+    L.mi_paged_attn_quant_workspace_size.restype = ctypes.c_size_t
+    L.mi_paged_attn_quant_workspace_size.argtypes = [i64] * 7
     L.mi_sample.restype = ctypes.c_int
     L.mi_sample.argtypes = [vp, vp, i32, i64, i64, i64, vp, vp, vp, vp]
     L.mi_profiler_enable.restype = ctypes.c_int
@@ -1089,6 +1111,7 @@ _PACK_PART = struct.Struct("@PPqqqqqqqii").pack     # mi_rope_part
 _PACK_ROTARY = struct.Struct("@PqifPqq").pack       # mi_rotary
 _PACK_CACHE = struct.Struct("@PPqqqqqqq").pack      # mi_paged_cache
 _PACK_SEQS = struct.Struct("@qqPPPqq").pack         # mi_paged_seqs
+_PACK_QUANT = struct.Struct("@PPPPqqqqqqqqqqii").pack  # mi_quant_cache
 _PACK_SAMPLING = struct.Struct("@PPPPfiff").pack    # mi_sampling
 
 
@@ -1262,7 +1285,14 @@ def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
     sp, sh, ss, sc = strides
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16 or (sc != 1 and d > 1):
         raise ValueError("the caches must be bf16 with contiguous components")
-    i32, table, rows_at = torch.int32, pages.shape, pages.stride()
+    cache = _PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), num, size, n_kv, d, sp, sh, ss)
+    seqs, n, width = _tables(pages, kv_len, q_start, rows)
+    return cache, seqs, (n_kv, size, d, n, width)
+
+
+def _tables(pages, kv_len, q_start, rows):
+    """mi_paged_seqs, packed, of int32 device tables; sequences; table width."""
+    i32, table, rows_at = _torch().int32, pages.shape, pages.stride()
     if pages.dtype != i32 or len(table) != 2 or (rows_at[1] != 1 and table[1] > 1):
         raise ValueError("pages must be int32, 2-D, with a contiguous last dimension")
     if kv_len.dtype != i32 or kv_len.dim() != 1 or not kv_len.is_contiguous():
@@ -1275,10 +1305,9 @@ def _paged(k_cache, v_cache, pages, kv_len, q_start, rows):
             raise ValueError(f"{rows} rows for {n} sequences: q_start is needed")
     elif q_start.dtype != i32 or q_start.dim() != 1 or not q_start.is_contiguous() or q_start.numel() != n + 1:
         raise ValueError(f"q_start must be int32, 1-D, contiguous, with {n + 1} entries")
-    cache = _PACK_CACHE(k_cache.data_ptr(), v_cache.data_ptr(), num, size, n_kv, d, sp, sh, ss)
     seqs = _PACK_SEQS(n, rows, 0 if q_start is None else q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
                       width, rows_at[0] if n > 1 else width)
-    return cache, seqs, (n_kv, size, d, n, width)
+    return seqs, n, width
 
 
 def _heads_of(name, t, rows, heads, d):
@@ -1303,6 +1332,13 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
     cache, seqs, of = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
     if of[0] != n_kv or of[2] != d:
         raise ValueError(f"the cache has {of[0]} heads of {of[2]}, k has {n_kv} of {d}")
+    return _append("mi_kv_append", k, v, cache, seqs, (k_cache, v_cache, pages, kv_len, q_start), q, q_out, inv_freq,
+                   positions, interleaved, scale, sync)
+
+
+def _append(name, k, v, cache, seqs, tensors, q, q_out, inv_freq, positions, interleaved, scale, sync):
+    """The call of mi_kv_append and mi_kv_append_quant, whose cache and sequences are packed."""
+    N, n_kv, d = k.shape
     k_t, k_h = _heads_of("k", k, N, n_kv, d)
     v_t, v_h = _heads_of("v", v, N, n_kv, d)
     n_heads = q_t = q_h = o_t = o_h = q_at = o_at = 0
@@ -1316,15 +1352,15 @@ def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out
         else:
             o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
-    stream = _stream_of(k, v, k_cache, v_cache, pages, kv_len, q_start, q, q_out, inv_freq, positions)
+    stream = _stream_of(k, v, *tensors, q, q_out, inv_freq, positions)
     rotary = None
     if inv_freq is not None:
         rotary = _rotary(inv_freq, positions, 1, N, 0, interleaved, scale)
     elif positions is not None:
         raise ValueError("positions without inv_freq")
-    st = load_library().mi_kv_append(stream, q_at, q_t, q_h, o_at, o_t, o_h, n_heads, k.data_ptr(), k_t, k_h,
-                                     v.data_ptr(), v_t, v_h, cache, seqs, rotary)
-    _done("mi_kv_append", st, sync)
+    st = getattr(load_library(), name)(stream, q_at, q_t, q_h, o_at, o_t, o_h, n_heads, k.data_ptr(), k_t, k_h,
+                                       v.data_ptr(), v_t, v_h, cache, seqs, rotary)
+    _done(name, st, sync)
     return q_out
 
 
@@ -1348,13 +1384,22 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
     max_kv_len: most cached tokens, as far as the host knows (else what the page table holds); both
     only shape the launch. workspace: "auto" allocates it, None never splits a sequence, or a device
     tensor of paged_attn_workspace_size bytes, which calls that may overlap must not share."""
-    torch = _torch()
     if q.dim() != 3:
         raise ValueError("q is [tokens, nH, d]")
     N, n_heads, d = q.shape
     cache, seqs, (n_kv, page, cd, n, width) = _paged(k_cache, v_cache, pages, kv_len, q_start, N)
     if d != cd:
         raise ValueError(f"the cache has heads of {cd}, q of {d}")
+    return _attend("mi_paged_attn", _attn_bytes, q, cache, seqs, n_kv, n, page * width, (k_cache, v_cache, pages, kv_len),
+                   q_start, max_q_len, max_kv_len, out, lse, causal, scale, workspace, sync)
+
+
+def _attend(name, bytes_of, q, cache, seqs, n_kv, n, room, tensors, q_start, max_q_len, max_kv_len, out, lse, causal, scale,
+            workspace, sync):
+    """The call of mi_paged_attn and mi_paged_attn_quant, whose cache and sequences are packed; room: tokens that a row
+    of the page table holds."""
+    torch = _torch()
+    N, n_heads, d = q.shape
     q_t, q_h = _heads_of("q", q, N, n_heads, d)
     if out is None:
         out, o_t, o_h = q.new_empty((N, n_heads, d)), n_heads * d, d
@@ -1364,23 +1409,138 @@ def paged_attn(q, k_cache, v_cache, pages, kv_len, q_start=None, max_q_len=None,
         raise ValueError(f"lse must be a contiguous fp32 [{N}, {n_heads}] tensor")
     if workspace is not None and not isinstance(workspace, str) and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous: its bytes are those of its elements")
-    stream = _stream_of(q, k_cache, v_cache, pages, kv_len, q_start, out, lse,
+    stream = _stream_of(q, *tensors, q_start, out, lse,
                         None if isinstance(workspace, str) else workspace)
     mq = 1 if q_start is None else N if max_q_len is None else int(max_q_len)
-    mk = page * width if max_kv_len is None else int(max_kv_len)
+    mk = room if max_kv_len is None else int(max_kv_len)
     at = size = 0
     if isinstance(workspace, str):
-        size = _attn_bytes(n_heads, n_kv, d, n, N, mq, mk, q.get_device())
+        size = bytes_of(n_heads, n_kv, d, n, N, mq, mk, q.get_device())
         workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     elif workspace is not None:
         size = workspace.numel() * workspace.element_size()
     if workspace is not None:
         at = workspace.data_ptr()
-    st = load_library().mi_paged_attn(stream, q.data_ptr(), q_t, q_h, out.data_ptr(), o_t, o_h,
+    st = getattr(load_library(), name)(stream, q.data_ptr(), q_t, q_h, out.data_ptr(), o_t, o_h,
                          None if lse is None else lse.data_ptr(), n_heads, cache, seqs, mq, mk, 1 if causal else 0,
                          1.0 / math.sqrt(d) if scale is None else scale, at, size)
-    _done("mi_paged_attn", st, sync)
+    _done(name, st, sync)
     return out
+
+
+# ---- a paged cache of 8 or 4 bits -----------------------------------------------------
+
+class QuantCache(NamedTuple):
+    """A paged cache of 8 or 4 bits (mi_quant_cache): codes k, v, uint8 [pages, nKV, page size, d] (e4m3) or
+    [pages, nKV, page size, d / 2] (e2m1, two components a byte), and the scale bytes of their groups of 32
+    components, k_scale, v_scale, uint8 [pages, nKV, page size, d / 32]; any strides with contiguous rows, those of
+    codes whole 16 bytes. quant_cache allocates one."""
+    k: "torch.Tensor"
+    v: "torch.Tensor"
+    k_scale: "torch.Tensor"
+    v_scale: "torch.Tensor"
+
+
+def quant_cache(num_pages, n_kv, page_size, head_dim, bits=8, device="cuda") -> QuantCache:
+    """An empty QuantCache of 8 (e4m3) or 4 bits (e2m1); head_dim a multiple of 32."""
+    if bits not in (8, 4) or head_dim < 32 or head_dim % 32:
+        raise ValueError(f"{bits} bits, heads of {head_dim}: 8 or 4 bits and a multiple of 32 are needed")
+    torch = _torch()
+    zeros = [torch.zeros((num_pages, n_kv, page_size, n), dtype=torch.uint8, device=device)
+             for n in (head_dim * bits // 8, head_dim // 32) for _ in "kv"]
+    return QuantCache(*zeros)
+
+
+def _quant(cache, pages, kv_len, q_start, rows):
+    """mi_quant_cache and mi_paged_seqs, packed; and (nKV, page size, d, sequences, table width)."""
+    k, v, ks, vs = cache
+    shape, groups, u8 = k.shape, ks.shape, _torch().uint8
+    strides, scale_strides = k.stride(), ks.stride()
+    if len(shape) != 4 or v.shape != shape or v.stride() != strides or len(groups) != 4 or vs.shape != groups or \
+            vs.stride() != scale_strides or groups[:3] != shape[:3]:
+        raise ValueError("codes are [pages, nKV, page size, bytes], scales [pages, nKV, page size, d / 32], of K and V "
+                         "with one shape and strides")
+    num, n_kv, size, n_bytes = shape
+    d = 32 * groups[3]
+    if n_bytes not in (d, d // 2):
+        raise ValueError(f"{n_bytes} bytes of codes for {groups[3]} groups of 32: {d} (8 bits) or {d // 2} (4) are needed")
+    if any(t.dtype != u8 for t in cache) or (n_bytes > 1 and strides[3] != 1) or (groups[3] > 1 and scale_strides[3] != 1):
+        raise ValueError("codes and scales must be uint8 with contiguous rows")
+    packed = _PACK_QUANT(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), num, size, n_kv, d, *strides[:3],
+                         *scale_strides[:3], MI_KV_E4M3 if n_bytes == d else MI_KV_E2M1, 0)
+    seqs, n, width = _tables(pages, kv_len, q_start, rows)
+    return packed, seqs, (n_kv, size, d, n, width)
+
+
+def kv_append_quant(k, v, cache, pages, kv_len, q_start=None, q=None, q_out=None, inv_freq=None, positions=None,
+                    interleaved=False, scale=1.0, sync=None):
+    """kv_append into a QuantCache (mi_kv_append_quant): K is rotated in 64 bits and rounded once, to the cache's
+    numbers, as it is written, V rounded alike. The other arguments and the result (q_out) as there."""
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v are [tokens, nKV, d]")
+    N, n_kv, d = k.shape
+    packed, seqs, of = _quant(cache, pages, kv_len, q_start, N)
+    if of[0] != n_kv or of[2] != d:
+        raise ValueError(f"the cache has {of[0]} heads of {of[2]}, k has {n_kv} of {d}")
+    return _append("mi_kv_append_quant", k, v, packed, seqs, (*cache, pages, kv_len, q_start), q, q_out, inv_freq, positions,
+                   interleaved, scale, sync)
+
+
+def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_out=None, parts="kv", dtype=None, sync=None):
+    """The tokens that kv_append_quant with these tables has written, read back (mi_kv_read_quant): the last
+    q_start[s + 1] - q_start[s] tokens of sequence s (None: its last one), K and V [rows, nKV, d] of dtype bf16
+    (the default) or fp32, exact in both. rows: how many there are, q_start's last entry (a row behind it is left as it
+    is; k_out or v_out say it, too). Tokens that no page holds are zeros. parts "k" or "v" reads one of the two.
+    Returns (K, V), None for the one not read."""
+    torch = _torch()
+    if parts not in ("kv", "k", "v"):
+        raise ValueError(f"parts {parts!r}: kv, k or v")
+    outs = [t if name in parts else None for name, t in zip("kv", (k_out, v_out))]
+    if rows is None:
+        rows = next((t.shape[0] for t in outs if t is not None), kv_len.numel() if q_start is None else None)
+    if rows is None:
+        raise ValueError("rows, k_out or v_out is needed with q_start")
+    packed, seqs, (n_kv, _, d, _, _) = _quant(cache, pages, kv_len, q_start, rows)
+    args, dt = [], dtype or next((t.dtype for t in outs if t is not None), torch.bfloat16)
+    for i, name in enumerate("kv"):
+        if name not in parts:
+            args += [None, 0, 0]
+            continue
+        if outs[i] is None:
+            outs[i] = torch.empty((rows, n_kv, d), dtype=dt, device=cache.k.device)
+        st, sh, sc = outs[i].stride() if outs[i].dim() == 3 else (0, 0, 0)
+        if outs[i].dtype != dt or outs[i].shape != (rows, n_kv, d) or (sc != 1 and d > 1):
+            raise ValueError(f"{name}_out must be {dt} [{rows}, {n_kv}, {d}] with contiguous components")
+        args += [outs[i].data_ptr(), st, sh]
+    stream = _stream_of(*cache, pages, kv_len, q_start, *outs)
+    _done("mi_kv_read_quant", load_library().mi_kv_read_quant(stream, *args, _dt(outs[0] if outs[0] is not None else outs[1]),
+                                                              packed, seqs), sync)
+    return tuple(outs)
+
+
+def paged_attn_quant_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len) -> int:
+    """Bytes of workspace paged_attn_quant uses (mi_paged_attn_quant_workspace_size)."""
+    return load_library().mi_paged_attn_quant_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_quant_bytes(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len, device):
+    return paged_attn_quant_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len)
+
+
+def paged_attn_quant(q, cache, pages, kv_len, q_start=None, max_q_len=None, max_kv_len=None, out=None, lse=None, causal=True,
+                     scale=None, workspace="auto", sync=None):
+    """paged_attn over a QuantCache (mi_paged_attn_quant), heads of 32, 64, 96 or 128: what paged_attn gives over the
+    values that the cache stands for. Arguments and result as there, workspace of paged_attn_quant_workspace_size
+    bytes."""
+    if q.dim() != 3:
+        raise ValueError("q is [tokens, nH, d]")
+    N, n_heads, d = q.shape
+    packed, seqs, (n_kv, page, cd, n, width) = _quant(cache, pages, kv_len, q_start, N)
+    if d != cd:
+        raise ValueError(f"the cache has heads of {cd}, q of {d}")
+    return _attend("mi_paged_attn_quant", _attn_quant_bytes, q, packed, seqs, n_kv, n, page * width, (*cache, pages, kv_len),
+                   q_start, max_q_len, max_kv_len, out, lse, causal, scale, workspace, sync)
 
 
 # ---- sampling ---------------------------------------------------------------------
