@@ -131,12 +131,12 @@ __device__ __forceinline__ void write_group(const float (&y)[8], uint8_t* dst, u
   const int from_m = (int)(m >> 23) - (int)BELOW + ((m & 0x7fffffu) > TOP ? 1 : 0);
   const bool none = m >= 0x7f000000u;
   const uint32_t byte = none ? 255u : (uint32_t)max(from_m, 27);
-  const float inv = none ? 0.0f : __uint_as_float((254u - byte) << 23);
+  [[maybe_unused]] const float inv = none ? 0.0f : __uint_as_float((254u - byte) << 23);
   uint32_t w[BITS / 4] = {};
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    float a = none ? 0.0f : y[e] * inv, b = none ? 0.0f : y[e + 1] * inv;
 #if defined(__HIP_DEVICE_COMPILE__)
+    float a = none ? 0.0f : y[e] * inv, b = none ? 0.0f : y[e + 1] * inv;
     if constexpr (BITS == 4) {
       if (e == 0) w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], a, b, 1.0f, 0);
       if (e == 2) w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], a, b, 1.0f, 1);

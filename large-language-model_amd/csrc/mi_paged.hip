@@ -226,7 +226,7 @@ __device__ __forceinline__ void pf_segment(const AttnParams& p, PfShared<D>& lds
         lo[i] = pack_bf16x2(e0 - bf16_bits_to_f32(hi[i] & 0xffffu), e1 - __uint_as_float(hi[i] & 0xffff0000u));
       }
       u32x4_t vf[ND];
-      read_v<ND, 0, L::ROW>(vf, st, v_rd);
+      read_v<ND, 0, 4 * L::ROW>(vf, st, v_rd);
       __builtin_amdgcn_sched_barrier(0);  // nothing that the next block asks for comes before
       // V has been read: its place takes the block after next
       fetch(base + 2 * STEP, stage);

@@ -122,10 +122,10 @@ struct PaLds {
   }
 };
 
-// N fragments of V: two transposing reads of 8 bytes each, at[c] + OFF and 4 rows further on.  Inline asm: the builtin
+// N fragments of V: two transposing reads of 8 bytes each, at[c] + OFF and NEXT bytes further on.  Inline asm: the builtin
 // would also wait for the loads into LDS that are in flight.  The wait for all of them ends the asm, so that
 // the compiler sees no register before it holds its data.
-template <int N, int OFF, int ROW>
+template <int N, int OFF, int NEXT>
 __device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint32_t (&at)[N]) {
   static_assert(N == 2 || N == 4 || N == 8, "written out for these");
   u32x2_t w[2 * N];
@@ -136,7 +136,7 @@ __device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint3
         "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
-        : "v"(st + at[0]), "v"(st + at[1]), "i"(OFF), "i"(OFF + 4 * ROW));
+        : "v"(st + at[0]), "v"(st + at[1]), "i"(OFF), "i"(OFF + NEXT));
   else if constexpr (N == 4)
     asm volatile(
         "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
@@ -145,7 +145,7 @@ __device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint3
         "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7])
-        : "v"(st + at[0]), "v"(st + at[1]), "v"(st + at[2]), "v"(st + at[3]), "i"(OFF), "i"(OFF + 4 * ROW));
+        : "v"(st + at[0]), "v"(st + at[1]), "v"(st + at[2]), "v"(st + at[3]), "i"(OFF), "i"(OFF + NEXT));
   else
     asm volatile(
         "ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %16 offset:%25\n\t"
@@ -160,7 +160,7 @@ __device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint3
         : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(w[4]), "=&v"(w[5]), "=&v"(w[6]), "=&v"(w[7]),
           "=&v"(w[8]), "=&v"(w[9]), "=&v"(w[10]), "=&v"(w[11]), "=&v"(w[12]), "=&v"(w[13]), "=&v"(w[14]), "=&v"(w[15])
         : "v"(st + at[0]), "v"(st + at[1]), "v"(st + at[2]), "v"(st + at[3]), "v"(st + at[4]), "v"(st + at[5]),
-          "v"(st + at[6]), "v"(st + at[7]), "i"(OFF), "i"(OFF + 4 * ROW));
+          "v"(st + at[6]), "v"(st + at[7]), "i"(OFF), "i"(OFF + NEXT));
 #endif
 #pragma unroll
   for (int c = 0; c < N; ++c) v[c] = u32x4_t{w[2 * c][0], w[2 * c][1], w[2 * c + 1][0], w[2 * c + 1][1]};
@@ -295,7 +295,7 @@ struct PaRows {
           lo[w2] = pack_bf16x2(sc[kb][base + 2 * w2] - bf16_bits_to_f32(hi[ks][w2] & 0xffffu),
                                sc[kb][base + 2 * w2 + 1] - __uint_as_float(hi[ks][w2] & 0xffff0000u));
       }
-      read_v<NC, 16 * ks * L::ROW, L::ROW>(vf, st, v_rd);
+      read_v<NC, 16 * ks * L::ROW, 4 * L::ROW>(vf, st, v_rd);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < NC; ++c)

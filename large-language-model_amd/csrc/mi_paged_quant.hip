@@ -25,12 +25,15 @@ struct Quarter {
   static constexpr int COMPS = D / 4, BYTES = COMPS * BITS / 8, EIGHTS = COMPS / 8;
   uint32_t w[BYTES / 4];
   uint32_t scale;  // the byte
+  // by global loads whatever the compiler knows of the addresses: flat ones would count as LDS accesses, too
   __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
-    if constexpr (BYTES == 8) *(u32x2_t*)w = *(const u32x2_t*)codes;
+#define MIG_GLOBAL(T, p) ((const __attribute__((address_space(1))) T*)(uintptr_t)(p))
+    if constexpr (BYTES == 8) *(u32x2_t*)w = *MIG_GLOBAL(u32x2_t, codes);
     else
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) ((u32x4_t*)w)[i] = ((const u32x4_t*)codes)[i];
-    scale = *scales;
+      for (int i = 0; i < BYTES / 16; ++i) ((u32x4_t*)w)[i] = MIG_GLOBAL(u32x4_t, codes)[i];
+    scale = *MIG_GLOBAL(uint8_t, scales);
+#undef MIG_GLOBAL
   }
   __device__ __forceinline__ u32x4_t eight(int i) const { return kv_eight<BITS>(w + i * (BITS / 4), kv_power(scale)); }
 };
@@ -39,7 +42,8 @@ struct Quarter {
 __device__ __align__(16) uint32_t pq_zero[8];
 
 // Few rows: V of a 32-key block of a wave, converted, rows of D components whose 16-byte chunks are moved so that
-// the writes of two rows' quarters, and the transposing reads, lie in different banks.
+// nothing collides: a write's lanes have 128 bytes a clock, the quarters of two rows (32 banks), a transposing
+// read's 256, 32 bytes of each of eight rows (64 banks).  Rows 8 apart have one order.
 template <int D>
 struct PqLds {
   static constexpr int ROW = D * 2;
@@ -47,8 +51,8 @@ struct PqLds {
   static constexpr int SUM_BYTES = PF_ROWS * PF_PITCH<D> * 4;
   static constexpr int BYTES = V_BYTES > SUM_BYTES ? V_BYTES : SUM_BYTES;
   __device__ static __forceinline__ int v_pos(int r, int c) {
-    if constexpr (D == 128) return c ^ ((r & 3) << 2) ^ (((r >> 3) & 1) << 1) ^ (r & 1);
-    else return c ^ (((r >> 1) & 1) << 2) ^ (((r >> 3) & 1) << 1);
+    if constexpr (D == 128) return c ^ ((r & 7) << 1) ^ (c >> 3);
+    else return c ^ (r & 7);
   }
 };
 
@@ -67,9 +71,10 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
                                            int k_end, bool whole, PartAt part_at) {
   using L = PqLds<D>;
   using Q4 = Quarter<D, BITS>;
-  constexpr int NS = D / 32, ND = D / 16, DEPTH = BITS == 4 ? 3 : 2;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int g = lane >> 4, l16 = lane & 15;
+  constexpr int NS = D / 32, ND = D / 16, DEPTH = BITS == 4 ? 3 : 2, STEP = PF_KEYS * PF_WAVES;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // or what a segment needs at its ends would be kept in registers from one to the next
+  const int wave = uniform(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
   const uint32_t vlds = lds_addr(lds.v) + (uint32_t)(wave * L::BYTES);
 
   const int n_packed = min(t.n * p.group - t.first, PF_ROWS);
@@ -96,59 +101,107 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
   const uint8_t* vsbase = p.vs + kvh * p.scale_head;
   int first_page = 0, k_stop = 0;  // the table holds the pages of the keys before k_stop
 
-  // Tile i of the scores: row r reads key 8 (r / 4) + 4i + r % 4, so that the eight scores of a lane are, in
-  // order, the run of keys that the second operand of P V takes.  V: row 16u + lane / 4, quarter lane % 4.
-  const int k_row = 8 * (l16 >> 2) + (l16 & 3), v_row = lane >> 2, v_q = lane & 3;
+  // Tile i of the scores: row r reads key 16i + r, so the eight scores of a lane are the keys 4g + e and 16 + 4g + e,
+  // e = 0 .. 3, and the second operand of P V takes these.  V: row 16u + lane / 4, quarter lane % 4.
+  const int v_row = lane >> 2, v_q = lane & 3;
   const bool k_in = Q4::COMPS * g < p.d, v_in = Q4::COMPS * v_q < p.d;  // d is a multiple of 32: whole quarters
   const int k_code = Q4::BYTES * g, k_scale = Q4::COMPS * g / KV_GROUP;
   const int v_code = Q4::BYTES * v_q, v_scale = Q4::COMPS * v_q / KV_GROUP;
+  // Whole blocks whose halves lie in one page each: scalar bases, of products of 32 bits each, and these offsets.
+  const int64_t most32 = INT32_MAX;
+  const bool even = shift >= 4 && p.d == D && p.pv.page_stride <= most32 && slot_stride << shift <= most32 &&
+                    p.scale_page <= most32 && p.scale_slot << shift <= most32;
+  const uint32_t page32 = (uint32_t)p.pv.page_stride, slot32 = (uint32_t)slot_stride;
+  const uint32_t spage32 = (uint32_t)p.scale_page, sslot32 = (uint32_t)p.scale_slot;
+  const uint32_t k_off = l16 * slot32 + k_code, ks_off = l16 * sslot32 + k_scale;
+  const uint32_t v_off = v_row * slot32 + v_code, vs_off = v_row * sslot32 + v_scale;
+  const int mask = (1 << shift) - 1;
   struct Block {
     Q4 k[2], v[2];
     uint32_t seen;  // its keys that exist
   } ring[DEPTH];
+  int page_lo, page_hi;  // of the halves of the block to be asked for next, read a block ahead of their use
+  auto look_up = [&](int base) __attribute__((always_inline)) {
+    page_lo = lds.table[(min(base, k_stop - 1) >> shift) - first_page];
+    page_hi = lds.table[(min(base + 16, k_stop - 1) >> shift) - first_page];
+  };
+  // Asks for the block at `base`, whose pages have been looked up.  A block past the end is asked for from zeros,
+  // so that every step has the same loads on their way and waits for no more than its own.
   auto fetch = [&](Block& b, int base) __attribute__((always_inline)) {
-    const int last = k_stop - 1, pos = base + (lane & 31);
-    const int page = lds.table[(min(pos, last) >> shift) - first_page];
-    const bool there = pos < k_stop && (uint32_t)page < (uint32_t)p.pv.num_pages;
-    const int slot = pos & ((1 << shift) - 1);
-    const int64_t off = there ? page * p.pv.page_stride + slot * slot_stride : -1;
-    const int64_t soff = page * p.scale_page + slot * p.scale_slot;
-    b.seen = (uint32_t)__ballot(there);
+    const uint32_t p0 = (uint32_t)uniform(page_lo), p1 = (uint32_t)uniform(page_hi);
+    const uint8_t *kp[2], *ksp[2], *vp[2], *vsp[2];
+    uint32_t seen = ~0u;
+    if (even && base + PF_KEYS <= k_stop && p0 < (uint32_t)p.pv.num_pages && p1 < (uint32_t)p.pv.num_pages) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t page = i ? p1 : p0, slot = (base + 16 * i) & mask;
+        const uint64_t at = (uint64_t)page * page32 + slot * slot32, sat = (uint64_t)page * spage32 + slot * sslot32;
+        kp[i] = kbase + at + k_off, ksp[i] = ksbase + sat + ks_off;
+        vp[i] = vbase + at + v_off, vsp[i] = vsbase + sat + vs_off;
+      }
+    } else if (base >= k_stop) {
+      seen = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kp[i] = ksp[i] = vp[i] = vsp[i] = (const uint8_t*)pq_zero;
+    } else {
+      const int pos = base + (lane & 31);
+      const int page = lds.table[(min(pos, k_stop - 1) >> shift) - first_page];
+      const bool there = pos < k_stop && (uint32_t)page < (uint32_t)p.pv.num_pages;
+      const int slot = pos & mask;
+      const int64_t off = there ? page * p.pv.page_stride + slot * slot_stride : -1;
+      const int64_t soff = page * p.scale_page + slot * p.scale_slot;
+      seen = (uint32_t)__ballot(there);
+      const uint8_t* zero = (const uint8_t*)pq_zero;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t ko = __shfl(off, 16 * i + l16, 64), kso = __shfl(soff, 16 * i + l16, 64);
+        const int64_t vo = __shfl(off, 16 * i + v_row, 64), vso = __shfl(soff, 16 * i + v_row, 64);
+        const bool k_ok = ko >= 0 && k_in, v_ok = vo >= 0 && v_in;
+        kp[i] = k_ok ? kbase + ko + k_code : zero, ksp[i] = k_ok ? ksbase + kso + k_scale : zero;
+        vp[i] = v_ok ? vbase + vo + v_code : zero, vsp[i] = v_ok ? vsbase + vso + v_scale : zero;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t o = __shfl(off, k_row + 4 * i, 64), so = __shfl(soff, k_row + 4 * i, 64);
-      const bool ok = o >= 0 && k_in;
-      b.k[i].load(ok ? kbase + o + k_code : (const uint8_t*)pq_zero, ok ? ksbase + so + k_scale : (const uint8_t*)pq_zero);
+      b.k[i].load(kp[i], ksp[i]);
+      b.v[i].load(vp[i], vsp[i]);
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t o = __shfl(off, 16 * u + v_row, 64), so = __shfl(soff, 16 * u + v_row, 64);
-      const bool ok = o >= 0 && v_in;
-      b.v[u].load(ok ? vbase + o + v_code : (const uint8_t*)pq_zero, ok ? vsbase + so + v_scale : (const uint8_t*)pq_zero);
-    }
+    b.seen = seen;
+    look_up(base + STEP);
   };
 
-  uint32_t v_rd[ND], v_wr[2][Q4::EIGHTS];
+  uint32_t v_rd[ND], v_wr[Q4::EIGHTS];
 #pragma unroll
   for (int c = 0; c < ND; ++c) {
-    const int r = 8 * g + (l16 >> 2), col = 16 * c + 4 * (l16 & 3);
-    v_rd[c] = (uint32_t)(r * L::ROW + 16 * L::v_pos(r, col >> 3) + (col & 7) * 2);
+    const int r = 4 * g + (l16 >> 2), col = 16 * c + 4 * (l16 & 3);
+    v_rd[c] = vlds + (uint32_t)(r * L::ROW + 16 * L::v_pos(r, col >> 3) + (col & 7) * 2);
   }
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int j = 0; j < Q4::EIGHTS; ++j) {
-      const int r = 16 * u + v_row;
-      v_wr[u][j] = (uint32_t)(r * L::ROW + 16 * L::v_pos(r, Q4::EIGHTS * v_q + j));
-    }
+  for (int j = 0; j < Q4::EIGHTS; ++j)
+    v_wr[j] = vlds + (uint32_t)(v_row * L::ROW + 16 * L::v_pos(v_row, Q4::EIGHTS * v_q + j));
 
   f32x4_t o[ND];
 #pragma unroll
   for (int c = 0; c < ND; ++c) o[c] = f32x4_t{0, 0, 0, 0};
-  float m_run = -INFINITY, l_run = 0.0f;
-  const float sl2 = p.scale_log2;
+  // the row's reference maximum, what a score has to exceed to move it, and -m_run in log2 units
+  float m_run = -INFINITY, l_run = 0.0f, m_lim = -INFINITY, nmc = 0.0f;
+  const float sl2 = p.scale_log2, tau = PA_TAU / sl2;
 
+  // V's fragment c, channels 16c + l16 by the keys that sc has, from where its block was written
+  auto v_frag = [&](int c) __attribute__((always_inline)) {
+    typedef short i16x4_t __attribute__((__vector_size__(4 * sizeof(short))));
+    typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+    const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uintptr_t)(v_rd[c])));
+    const u32x2_t hi = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uintptr_t)(v_rd[c] + 16 * L::ROW)));
+    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
   auto work = [&](const Block& b, int base) __attribute__((always_inline)) {
+    // V goes through LDS, which serves a wave in order, to its transposing reads
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < Q4::EIGHTS; ++j) *(lds_u32x4_t*)(uintptr_t)(v_wr[j] + u * 16 * L::ROW) = b.v[u].eight(j);
     f32x4_t sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -156,34 +209,35 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
       for (int i = 0; i < 2; ++i)
         sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b.k[i].eight(s)),
                                                        __builtin_bit_cast(bf16x8_t, qf[s]), sc[i], 0, 0, 0);
-    // V goes through LDS to its transposing reads
+    u32x4_t vf[ND / 2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int j = 0; j < Q4::EIGHTS; ++j) *(lds_u32x4_t*)(uintptr_t)(vlds + v_wr[u][j]) = b.v[u].eight(j);
-    // sc[t][e] is key 8g + 4t + e of row l16
+    for (int c = 0; c < ND / 2; ++c) vf[c] = v_frag(c);
+    // sc[t][e] is key 16t + 4g + e of row l16
     if (base + PF_KEYS > lim_lo || b.seen != ~0u) {
       const int room = lim - base;
-      const uint32_t bits = (room >= 32 ? b.seen : room <= 0 ? 0u : b.seen & ((1u << room) - 1)) >> (8 * g);
+      const uint32_t bits = (room >= 32 ? b.seen : room <= 0 ? 0u : b.seen & ((1u << room) - 1)) >> (4 * g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sc[i >> 2][i & 3] = (bits >> i) & 1 ? sc[i >> 2][i & 3] : -INFINITY;
+      for (int i = 0; i < 8; ++i)
+        sc[i >> 2][i & 3] = (bits >> (16 * (i >> 2) + (i & 3))) & 1 ? sc[i >> 2][i & 3] : -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float m_old = m_run;
-    const bool fresh = m_old == -INFINITY, raise = !fresh && (mx - m_old) * sl2 > PA_TAU;
-    const float m_ref = fresh || raise ? mx : m_old;
-    if (__any(raise)) {
-      const float alpha = raise ? __builtin_amdgcn_exp2f((m_old - m_ref) * sl2) : 1.0f;
+    // Lanes l16 + 16g share a row and its reference maximum.  It is moved, and the lanes' maxima looked at
+    // together, only where one of them has a first score or one that exceeds it by PA_TAU.
+    if (__any(mx > m_lim)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const bool raise = mx > m_lim;
+      const float m_ref = raise ? mx : m_run;
+      const float alpha = raise && m_run != -INFINITY ? __builtin_amdgcn_exp2f((m_run - m_ref) * sl2) : 1.0f;
       l_run *= alpha;
 #pragma unroll
       for (int c = 0; c < ND; ++c) o[c] *= alpha;
+      m_run = m_ref;
+      m_lim = m_run == -INFINITY ? -INFINITY : m_run + tau;
+      nmc = m_run == -INFINITY ? 0.0f : -m_run * sl2;
     }
-    m_run = m_ref;
-    const float nmc = m_ref == -INFINITY ? 0.0f : -m_ref * sl2;
     u32x4_t hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -193,23 +247,19 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
       hi[i] = pack_bf16x2(e0, e1);
       lo[i] = pack_bf16x2(e0 - bf16_bits_to_f32(hi[i] & 0xffffu), e1 - __uint_as_float(hi[i] & 0xffff0000u));
     }
-    // LDS serves a wave in order: the reads follow the writes
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4_t vf[ND];
-    read_v<ND, 0, L::ROW>(vf, vlds, v_rd);
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int c = 0; c < ND; ++c) {
-      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
-                                                    __builtin_bit_cast(bf16x8_t, lo), o[c], 0, 0, 0);
-      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
-                                                    __builtin_bit_cast(bf16x8_t, hi), o[c], 0, 0, 0);
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < ND / 2; ++i) {
+        const int c = h * ND / 2 + i;
+        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[i]),
+                                                      __builtin_bit_cast(bf16x8_t, lo), o[c], 0, 0, 0);
+        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[i]),
+                                                      __builtin_bit_cast(bf16x8_t, hi), o[c], 0, 0, 0);
+        if (h == 0) vf[i] = v_frag(ND / 2 + i);
+      }
   };
 
-  constexpr int STEP = PF_KEYS * PF_WAVES;
   // keys whose pages the table holds, wherever in a page they begin
   const int k_span = (int)min((int64_t)(PF_TABLE - 1) << shift, (int64_t)1 << 30) / STEP * STEP;
   for (int k_first = k_begin; k_first < k_end; k_first = k_stop) {
@@ -221,16 +271,19 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
       lds.table[i] = p.pv.pages[(int64_t)t.s * p.pv.pages_ld + first_page + i];
     __syncthreads();
     int base = k_first + PF_KEYS * wave;
-    static_for<DEPTH>([&](auto i) __attribute__((always_inline)) {
-      if (base + STEP * i < k_stop) fetch(ring[i], base + STEP * i);
-    });
-    while (base < k_stop)
-      static_for<DEPTH>([&](auto i) __attribute__((always_inline)) {
-        if (base >= k_stop) return;
-        work(ring[i], base);
-        if (base + STEP * DEPTH < k_stop) fetch(ring[i], base + STEP * DEPTH);
-        base += STEP;
-      });
+    if (base >= k_stop) continue;
+    look_up(base);
+    static_for<DEPTH>([&](auto i) __attribute__((always_inline)) { fetch(ring[i], base + STEP * i); });
+    auto step = [&](Block& b) __attribute__((always_inline)) {
+      work(b, base);
+      fetch(b, base + STEP * DEPTH);
+      base += STEP;
+      return base < k_stop;
+    };
+    static_assert(DEPTH >= 2 && DEPTH <= 4, "written out for these");
+    while (step(ring[0]) && step(ring[1]) && (DEPTH < 3 || step(ring[DEPTH < 3 ? 0 : 2])) &&
+           (DEPTH < 4 || step(ring[DEPTH < 4 ? 0 : 3]))) {
+    }
   }
   __syncthreads();  // V's place takes the waves' sums
   pf_join_waves<D>(p, lds.v, L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at);
