@@ -1310,12 +1310,16 @@ def _tables(pages, kv_len, q_start, rows):
     return seqs, n, width
 
 
-def _heads_of(name, t, rows, heads, d):
-    """Strides of a bf16 [rows, heads, d] tensor."""
-    st, sh, sc = t.stride() if t.dim() == 3 else (0, 0, 0)
-    if t.dtype != _torch().bfloat16 or t.shape != (rows, heads, d) or (sc != 1 and d > 1):
-        raise ValueError(f"{name} must be bf16 [{rows}, {heads}, {d}] with contiguous components")
-    return st, sh
+def _heads_of(name, t, rows, heads, d, dtype=None):
+    """Strides of a [rows, heads, d] tensor, bf16 if no dtype is given."""
+    if dtype is None:
+        dtype = _torch().bfloat16
+    if t.shape == (rows, heads, d) and t.dtype == dtype:
+        st, sh, sc = t.stride()
+        if sc == 1 or d <= 1:
+            return st, sh
+    what = str(dtype).replace("torch.", "").replace("bfloat16", "bf16")
+    raise ValueError(f"{name} must be {what} [{rows}, {heads}, {d}] with contiguous components")
 
 
 def kv_append(k, v, k_cache, v_cache, pages, kv_len, q_start=None, q=None, q_out=None, inv_freq=None,
@@ -1348,7 +1352,7 @@ def _append(name, k, v, cache, seqs, tensors, q, q_out, inv_freq, positions, int
         n_heads = q.shape[1] if q.dim() == 3 else 0
         q_t, q_h = _heads_of("q", q, N, n_heads, d)
         if q_out is None:
-            q_out, o_t, o_h = q.new_empty((N, n_heads, d)), n_heads * d, d
+            q_out, o_t, o_h = q.new_empty(N, n_heads, d), n_heads * d, d
         else:
             o_t, o_h = _heads_of("q_out", q_out, N, n_heads, d)
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
@@ -1402,7 +1406,7 @@ def _attend(name, bytes_of, q, cache, seqs, n_kv, n, room, tensors, q_start, max
     N, n_heads, d = q.shape
     q_t, q_h = _heads_of("q", q, N, n_heads, d)
     if out is None:
-        out, o_t, o_h = q.new_empty((N, n_heads, d)), n_heads * d, d
+        out, o_t, o_h = q.new_empty(N, n_heads, d), n_heads * d, d
     else:
         o_t, o_h = _heads_of("out", out, N, n_heads, d)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, n_heads) or not lse.is_contiguous()):
@@ -1454,20 +1458,23 @@ def quant_cache(num_pages, n_kv, page_size, head_dim, bits=8, device="cuda") -> 
 def _quant(cache, pages, kv_len, q_start, rows):
     """mi_quant_cache and mi_paged_seqs, packed; and (nKV, page size, d, sequences, table width)."""
     k, v, ks, vs = cache
-    shape, groups, u8 = k.shape, ks.shape, _torch().uint8
-    strides, scale_strides = k.stride(), ks.stride()
-    if len(shape) != 4 or v.shape != shape or v.stride() != strides or len(groups) != 4 or vs.shape != groups or \
-            vs.stride() != scale_strides or groups[:3] != shape[:3]:
+    shape, groups = k.shape, ks.shape
+    at, scale_at = k.stride(), ks.stride()
+    if len(shape) != 4 or len(groups) != 4 or v.shape != shape or vs.shape != groups or groups[:3] != shape[:3] or \
+            v.stride() != at or vs.stride() != scale_at:
         raise ValueError("codes are [pages, nKV, page size, bytes], scales [pages, nKV, page size, d / 32], of K and V "
                          "with one shape and strides")
     num, n_kv, size, n_bytes = shape
-    d = 32 * groups[3]
-    if n_bytes not in (d, d // 2):
-        raise ValueError(f"{n_bytes} bytes of codes for {groups[3]} groups of 32: {d} (8 bits) or {d // 2} (4) are needed")
-    if any(t.dtype != u8 for t in cache) or (n_bytes > 1 and strides[3] != 1) or (groups[3] > 1 and scale_strides[3] != 1):
+    n_groups = groups[3]
+    d = 32 * n_groups
+    if n_bytes != d and 2 * n_bytes != d:
+        raise ValueError(f"{n_bytes} bytes of codes for {n_groups} groups of 32: {d} (8 bits) or {d // 2} (4) are needed")
+    u8 = _torch().uint8
+    if k.dtype != u8 or v.dtype != u8 or ks.dtype != u8 or vs.dtype != u8 or (at[3] != 1 and n_bytes > 1) or \
+            (scale_at[3] != 1 and n_groups > 1):
         raise ValueError("codes and scales must be uint8 with contiguous rows")
-    packed = _PACK_QUANT(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), num, size, n_kv, d, *strides[:3],
-                         *scale_strides[:3], MI_KV_E4M3 if n_bytes == d else MI_KV_E2M1, 0)
+    packed = _PACK_QUANT(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), num, size, n_kv, d, at[0], at[1], at[2],
+                         scale_at[0], scale_at[1], scale_at[2], MI_KV_E4M3 if n_bytes == d else MI_KV_E2M1, 0)
     seqs, n, width = _tables(pages, kv_len, q_start, rows)
     return packed, seqs, (n_kv, size, d, n, width)
 
@@ -1492,30 +1499,37 @@ def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_o
     (the default) or fp32, exact in both. rows: how many there are, q_start's last entry (a row behind it is left as it
     is; k_out or v_out say it, too). Tokens that no page holds are zeros. parts "k" or "v" reads one of the two.
     Returns (K, V), None for the one not read."""
-    torch = _torch()
     if parts not in ("kv", "k", "v"):
         raise ValueError(f"parts {parts!r}: kv, k or v")
-    outs = [t if name in parts else None for name, t in zip("kv", (k_out, v_out))]
+    if parts != "kv":
+        k_out, v_out = (None, v_out) if parts == "v" else (k_out, None)
+    given = k_out if k_out is not None else v_out
     if rows is None:
-        rows = next((t.shape[0] for t in outs if t is not None), kv_len.numel() if q_start is None else None)
-    if rows is None:
-        raise ValueError("rows, k_out or v_out is needed with q_start")
+        if given is None and q_start is not None:
+            raise ValueError("rows, k_out or v_out is needed with q_start")
+        rows = kv_len.numel() if given is None else given.shape[0]
     packed, seqs, (n_kv, _, d, _, _) = _quant(cache, pages, kv_len, q_start, rows)
-    args, dt = [], dtype or next((t.dtype for t in outs if t is not None), torch.bfloat16)
-    for i, name in enumerate("kv"):
-        if name not in parts:
-            args += [None, 0, 0]
-            continue
-        if outs[i] is None:
-            outs[i] = torch.empty((rows, n_kv, d), dtype=dt, device=cache.k.device)
-        st, sh, sc = outs[i].stride() if outs[i].dim() == 3 else (0, 0, 0)
-        if outs[i].dtype != dt or outs[i].shape != (rows, n_kv, d) or (sc != 1 and d > 1):
-            raise ValueError(f"{name}_out must be {dt} [{rows}, {n_kv}, {d}] with contiguous components")
-        args += [outs[i].data_ptr(), st, sh]
-    stream = _stream_of(*cache, pages, kv_len, q_start, *outs)
-    _done("mi_kv_read_quant", load_library().mi_kv_read_quant(stream, *args, _dt(outs[0] if outs[0] is not None else outs[1]),
-                                                              packed, seqs), sync)
-    return tuple(outs)
+    if dtype is None:
+        dtype = _torch().bfloat16 if given is None else given.dtype
+    code = MI_F32 if dtype == _torch().float32 else MI_BF16 if dtype == _torch().bfloat16 else None
+    if code is None:
+        raise ValueError(f"dtype {dtype}: bf16 and fp32 are possible")
+    k_at = k_t = k_h = v_at = v_t = v_h = 0
+    if parts != "v":
+        if k_out is None:
+            k_out, k_t, k_h = cache.k.new_empty((rows, n_kv, d), dtype=dtype), n_kv * d, d
+        else:
+            k_t, k_h = _heads_of("k_out", k_out, rows, n_kv, d, dtype)
+        k_at = k_out.data_ptr()
+    if parts != "k":
+        if v_out is None:
+            v_out, v_t, v_h = cache.k.new_empty((rows, n_kv, d), dtype=dtype), n_kv * d, d
+        else:
+            v_t, v_h = _heads_of("v_out", v_out, rows, n_kv, d, dtype)
+        v_at = v_out.data_ptr()
+    stream = _stream_of(*cache, pages, kv_len, q_start, k_out, v_out)
+    _done("mi_kv_read_quant", load_library().mi_kv_read_quant(stream, k_at, k_t, k_h, v_at, v_t, v_h, code, packed, seqs), sync)
+    return k_out, v_out
 
 
 def paged_attn_quant_workspace_size(n_heads, n_kv, head_dim, n_seqs, total_q, max_q_len, max_kv_len) -> int:
