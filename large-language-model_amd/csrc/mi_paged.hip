@@ -378,10 +378,10 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
   __shared__ PfShared<D> lds;
   __shared__ PfPrefix prefix;
   const int kvh = uniform(blockIdx.x % p.n_kv);
-  pf_over_share(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
-                [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
-                  pf_segment<D>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
-                });
+  pf_over_share<0>(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
+                   [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
+                     pf_segment<D>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
+                   });
 }
 
 }  // namespace

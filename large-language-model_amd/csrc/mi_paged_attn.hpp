@@ -466,8 +466,9 @@ struct PfPrefix {
 };
 
 // Workgroup w of KV head kvh over its share: segment(tile, first key, last key, whole, part_at) for each sequence
-// in it, all threads together.
-template <class Segment>
+// in it, all threads together.  A sequence's keys come after EXTRA blocks of none, for what a workgroup spends on going
+// over to it; a share that ends among these has none of its keys.
+template <int EXTRA, class Segment>
 __device__ __forceinline__ void pf_over_share(const AttnParams& p, PfPrefix& lds, uint32_t w, Segment segment) {
   uint32_t* prefix = lds.prefix;
   uint32_t* wave_sum = lds.wave_sum;
@@ -478,6 +479,7 @@ __device__ __forceinline__ void pf_over_share(const AttnParams& p, PfPrefix& lds
   for (int i = 0; i < EACH; ++i) {
     const int s = EACH * tid + i;
     n[i] = s < S ? (uint32_t)(min(max(p.pv.kv_len[s], 0), p.cap) + PF_BLOCK - 1) / PF_BLOCK : 0;
+    n[i] += n[i] ? EXTRA : 0;
     sum += n[i];
   }
   uint32_t before = sum;
@@ -517,7 +519,8 @@ __device__ __forceinline__ void pf_over_share(const AttnParams& p, PfPrefix& lds
     t.len = uniform(p.pv.kv_len[s]);
     const int len = t.limit(p, 0);
     const uint32_t last = min(stop, next);
-    const int k_begin = (int)(b - first) * PF_BLOCK, k_end = last == next ? len : (int)(last - first) * PF_BLOCK;
+    const int k_begin = max((int)(b - first) - EXTRA, 0) * PF_BLOCK;
+    const int k_end = last == next ? len : max((int)(last - first) - EXTRA, 0) * PF_BLOCK;
     segment(t, k_begin, k_end, b == first && last == next,
             [&](int, int head) { return (int64_t)(2 * w + k) * p.n_heads + head; });
     b = last;

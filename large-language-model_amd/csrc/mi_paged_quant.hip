@@ -397,16 +397,19 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
                       [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
 }
 
+// The first blocks of a sequence arrive 4 us after the last sum of the one before, in which a workgroup does 300 keys:
+// counted as 256, the workgroups end together (64 sequences of 500 to 8000 keys: 30.5 us, not counted 32.0; 512 as 256).
+constexpr int PQ_EXTRA = 256 / PF_BLOCK;
 template <int D, int BITS>
 __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
     paged_attn_quant_share_kernel(QuantParams p) {
   __shared__ PqShared<D> lds;
   __shared__ PfPrefix prefix;
   const int kvh = uniform(blockIdx.x % p.n_kv);
-  pf_over_share(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
-                [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
-                  pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
-                });
+  pf_over_share<PQ_EXTRA>(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
+                          [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
+                            pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
+                          });
 }
 
 template <int D, int BITS>
