@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     return;
   }
   const bool wave_has_rows = 32 * wave < n_packed;
-  PaRows<D> rows;
+  PaRows<D, true> rows;
   rows.begin(p, t, kvh, wave, n_packed);
 
   // DMA: wave w brings rows 16w .. 16w+15 of a block; in load u lane l brings a chunk of row

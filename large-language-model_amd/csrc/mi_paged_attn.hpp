@@ -122,6 +122,12 @@ struct PaLds {
   }
 };
 
+__device__ __forceinline__ u32x2_t read_tr16(uint32_t at) {
+  typedef short i16x4_t __attribute__((__vector_size__(4 * sizeof(short))));
+  typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uintptr_t)at));
+}
+
 // N fragments of V: two transposing reads of 8 bytes each, at[c] + OFF and NEXT bytes further on.  Inline asm: the builtin
 // would also wait for the loads into LDS that are in flight.  The wait for all of them ends the asm, so that
 // the compiler sees no register before it holds its data.
@@ -166,8 +172,10 @@ __device__ __forceinline__ void read_v(u32x4_t (&v)[N], uint32_t st, const uint3
   for (int c = 0; c < N; ++c) v[c] = u32x4_t{w[2 * c][0], w[2 * c][1], w[2 * c + 1][0], w[2 * c + 1][1]};
 }
 
-// The rows of a wave, 32 of a tile of PA_ROWS, with their running sums.
-template <int D>
+// The rows of a wave, 32 of a tile of PA_ROWS, with their running sums.  STREAMED: the blocks come by loads into LDS, which
+// are in flight meanwhile, so V's fragments are read in inline asm; else the compiler's reads bring them a step
+// ahead, and the waves that multiply go first.
+template <int D, bool STREAMED>
 struct PaRows {
   using L = PaLds<D>;
   static constexpr int NS = D / 16, NC = D / 32;
@@ -212,6 +220,14 @@ struct PaRows {
     sl2 = p.scale_log2;
   }
 
+  __device__ __forceinline__ void fragments(u32x4_t (&v)[NC], uint32_t st) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const u32x2_t a = read_tr16(st + v_rd[c]), b = read_tr16(st + v_rd[c] + 4 * L::ROW);
+      v[c] = u32x4_t{a[0], a[1], b[0], b[1]};
+    }
+  }
+
   // The 64-key block at LDS address st, K and behind it V, of keys base .. base + 63, of which `seen` exist.
   __device__ __forceinline__ void block(uint32_t st, int base, uint64_t seen) {
     if (base >= lim_hi) return;
@@ -223,6 +239,7 @@ struct PaRows {
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[kb][e] = 0.0f;
+    if constexpr (!STREAMED) __builtin_amdgcn_s_setprio(1);
     u32x4_t kf[NS][2];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -236,6 +253,7 @@ struct PaRows {
       for (int kb = 0; kb < 2; ++kb)
         sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, kf[s][kb]),
                                                         __builtin_bit_cast(bf16x8_t, qf[s]), sc[kb], 0, 0, 0);
+    if constexpr (!STREAMED) __builtin_amdgcn_s_setprio(0);
     // sc[kb][4q + e] is key 32kb + 8*h32 + 16(q>>1) + 4(q&1) + e
     if (masked) {
 #pragma unroll
@@ -284,9 +302,14 @@ struct PaRows {
       }
     }
     l_run += sum;
+    u32x4_t v[STREAMED ? 1 : 2][NC];
+    if constexpr (!STREAMED) {
+      __builtin_amdgcn_s_setprio(1);
+      fragments(v[0], st);
+    }
     static_for<4>([&](auto ks_c) __attribute__((always_inline)) {
       constexpr int ks = decltype(ks_c)::value;
-      u32x4_t vf[NC];
+      u32x4_t(&vf)[NC] = v[STREAMED ? 0 : ks & 1];
       u32x4_t lo;
       {
         constexpr int kb = ks >> 1, base = 8 * (ks & 1);
@@ -295,8 +318,12 @@ struct PaRows {
           lo[w2] = pack_bf16x2(sc[kb][base + 2 * w2] - bf16_bits_to_f32(hi[ks][w2] & 0xffffu),
                                sc[kb][base + 2 * w2 + 1] - __uint_as_float(hi[ks][w2] & 0xffff0000u));
       }
-      read_v<NC, 16 * ks * L::ROW, 4 * L::ROW>(vf, st, v_rd);
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (STREAMED) {
+        read_v<NC, 16 * ks * L::ROW, 4 * L::ROW>(vf, st, v_rd);
+        __builtin_amdgcn_sched_barrier(0);
+      } else if constexpr (ks < 3) {
+        fragments(v[(ks + 1) & 1], st + 16 * (ks + 1) * L::ROW);
+      }
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
@@ -306,6 +333,7 @@ struct PaRows {
         o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[c]),
                                                        __builtin_bit_cast(bf16x8_t, hi[ks]), o[c], 0, 0, 0);
     });
+    if constexpr (!STREAMED) __builtin_amdgcn_s_setprio(0);
   }
 
   // Writes O and lse, or the part of a piece.

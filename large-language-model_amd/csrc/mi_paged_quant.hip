@@ -189,11 +189,7 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
 
   // V's fragment c, channels 16c + l16 by the keys that sc has, from where its block was written
   auto v_frag = [&](int c) __attribute__((always_inline)) {
-    typedef short i16x4_t __attribute__((__vector_size__(4 * sizeof(short))));
-    typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
-    const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uintptr_t)(v_rd[c])));
-    const u32x2_t hi = __builtin_bit_cast(
-        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uintptr_t)(v_rd[c] + 16 * L::ROW)));
+    const u32x2_t lo = read_tr16(v_rd[c]), hi = read_tr16(v_rd[c] + 16 * L::ROW);
     return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
   };
   auto work = [&](const Block& b, int base) __attribute__((always_inline)) {
@@ -320,7 +316,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     return;
   }
   const bool wave_has_rows = 32 * wave < n_packed;
-  PaRows<D> rows;
+  PaRows<D, false> rows;
   rows.begin(p, t, kvh, wave, n_packed);
 
   // wave w brings rows 16w .. 16w+15 of a block, a lane a quarter of row 16w + lane / 4
