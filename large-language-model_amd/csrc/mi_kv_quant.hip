@@ -260,7 +260,10 @@ struct ReadParams {
   int64_t first;
 };
 
-// Eight components a lane.  T: uint16_t (bf16) or float; VEC: rows of the output are whole 16-byte vectors.
+// KR_COMPS components a lane, half a group: of half as many a lane's loads are 4 bytes (8 sequences of up
+// to 16000 tokens in 4 bits: 27.4 us, so 21.0), of a group the stores of a wave lie 64 bytes apart (31.8).  T: uint16_t
+// (bf16) or float; VEC: rows of the output are whole 16-byte vectors.
+constexpr int KR_COMPS = 16;
 template <int BITS, typename T, bool VEC>
 __global__ void __launch_bounds__(KQ_THREADS) kv_read_quant_kernel(ReadParams p) {
   __shared__ Tokens at;
@@ -268,41 +271,43 @@ __global__ void __launch_bounds__(KQ_THREADS) kv_read_quant_kernel(ReadParams p)
   const int n_tok = (int)min((int64_t)p.per_wg, p.tokens - tok0);
   look_up_tokens(p.pv, tok0, n_tok, at);
   __syncthreads();
-  const int runs = p.d / 8, units = n_tok * p.parts * p.n_kv * runs;
+  const int runs = p.d / KR_COMPS, units = n_tok * p.parts * p.n_kv * runs;
 #pragma unroll 4
   for (int u = threadIdx.x; u < units; u += KQ_THREADS) {
-    const int hh = u / runs, c0 = 8 * (u - hh * runs);
+    const int hh = u / runs, c0 = KR_COMPS * (u - hh * runs);
     const int k = hh / (p.parts * p.n_kv);
     int h = hh - k * p.parts * p.n_kv;
     const bool is_v = h >= p.n_kv || !p.k;
     if (h >= p.n_kv) h -= p.n_kv;
     const int page = at.page[k], slot = at.slot[k];
     if (page == -2) continue;
-    u32x4_t x = {0, 0, 0, 0};
+    u32x4_t x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     if (page >= 0) {
       const uint8_t* src = (is_v ? p.c.v : p.c.k) + page * p.pv.page_stride + h * p.pv.head_stride +
                            slot * p.pv.slot_stride + c0 * BITS / 8;
       const uint8_t* sc = (is_v ? p.c.vs : p.c.ks) + page * p.c.scale_page + h * p.c.scale_head + slot * p.c.scale_slot;
       const float s = kv_power(sc[c0 / KV_GROUP]);
-      uint32_t w[BITS / 4];
-      if constexpr (BITS == 4) w[0] = *(const uint32_t*)src;
-      else *(u32x2_t*)w = *(const u32x2_t*)src;
-      x = kv_eight<BITS>(w, s);
+      uint32_t w[BITS / 2];
+      if constexpr (BITS == 4) *(u32x2_t*)w = *(const u32x2_t*)src;
+      else *(u32x4_t*)w = *(const u32x4_t*)src;
+      x[0] = kv_eight<BITS>(w, s);
+      x[1] = kv_eight<BITS>(w + BITS / 4, s);
     }
     T* dst = (T*)(is_v ? p.v : p.k) + (is_v ? (tok0 + k) * p.v_t + h * p.v_h : (tok0 + k) * p.k_t + h * p.k_h) + c0;
     if constexpr (sizeof(T) == 2 && VEC) {
-      *(u32x4_t*)dst = x;
+      ((u32x4_t*)dst)[0] = x[0];
+      ((u32x4_t*)dst)[1] = x[1];
     } else if constexpr (VEC) {
-      f32x4_t lo, hi;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        (e < 4 ? lo : hi)[e & 3] = __uint_as_float(e & 1 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16);
-      ((f32x4_t*)dst)[0] = lo;
-      ((f32x4_t*)dst)[1] = hi;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = x[i / 2][i % 2 * 2], b = x[i / 2][i % 2 * 2 + 1];
+        ((f32x4_t*)dst)[i] = f32x4_t{__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u),
+                                     __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)};
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t bits = e & 1 ? x[e / 2] >> 16 : x[e / 2] & 0xffffu;
+      for (int e = 0; e < KR_COMPS; ++e) {
+        const uint32_t w = x[e / 8][e % 8 / 2], bits = e & 1 ? w >> 16 : w & 0xffffu;
         if constexpr (sizeof(T) == 2) dst[e] = (T)bits;
         else dst[e] = __uint_as_float(bits << 16);
       }
@@ -434,7 +439,7 @@ int mi_kv_read_quant(void* stream, void* k, int64_t k_t, int64_t k_h, void* v, i
     return !at || ((uintptr_t)at % 16 == 0 && (tokens <= 1 || t * es % 16 == 0) && (p.n_kv <= 1 || h * es % 16 == 0));
   };
   const bool vec = rows_fit(k, k_t, k_h) && rows_fit(v, v_t, v_h), four = cache->format == MI_KV_E2M1;
-  p.per_wg = tokens_of_group(tokens, (int64_t)p.parts * p.n_kv * (d / 8), 8, KR_MAX_TOKENS);
+  p.per_wg = tokens_of_group(tokens, (int64_t)p.parts * p.n_kv * (d / KR_COMPS), 4, KR_MAX_TOKENS);
   hipStream_t hs = (hipStream_t)stream;
   return launch_tokens(p, "kv_read_quant", [&](unsigned grid) {
     if (dtype == MI_BF16) {
