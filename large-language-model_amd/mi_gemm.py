@@ -1527,6 +1527,8 @@ def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_o
         else:
             v_t, v_h = _heads_of("v_out", v_out, rows, n_kv, d, dtype)
         v_at = v_out.data_ptr()
+        if v_at and v_at == k_at:
+            raise ValueError("k_out and v_out are the same memory")
     stream = _stream_of(*cache, pages, kv_len, q_start, k_out, v_out)
     _done("mi_kv_read_quant", load_library().mi_kv_read_quant(stream, k_at, k_t, k_h, v_at, v_t, v_h, code, packed, seqs), sync)
     return k_out, v_out

@@ -136,6 +136,21 @@ def test_one_sequence_cut_by_all_workgroups(mi, dev, bits, kv, nKV, d):
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("kv,nH,nKV,d", [([5, 600], 2, 1, 32), ([100] * 200, 4, 4, 64), ([1, 0, 129, 128, 127] * 31, 8, 2, 128)])
+def test_shares_of_short_sequences(mi, dev, bits, kv, nH, nKV, d):
+    """Far shorter than the host said: shares that begin or end before a sequence's first key, and have none."""
+    import torch
+
+    b = hold(mi, Batch([1] * len(kv), kv, 16, nH, nKV, d, seed=len(kv), one_each=True), bits)
+    ref = b.reference()
+    close(*run(mi, b, max_kv_len=1 << 16), ref, max(kv))
+    n = mi.paged_attn_quant_workspace_size(nH, nKV, d, len(kv), len(kv), 1, 1 << 16)
+    ws = torch.full((n + 16,), 255, dtype=torch.uint8, device="cuda")  # a part that no one wrote would be NaN
+    close(*run(mi, b, max_kv_len=1 << 16, workspace=ws[:n]), ref, max(kv))
+    assert (ws[n:] == 255).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("most", [0, 1, 3, 10 ** 6])
 @pytest.mark.parametrize("nH,nKV,d", [(8, 2, 128), (4, 4, 64)])
 def test_bounds_only_shape_the_launch(mi, dev, bits, most, nH, nKV, d):
@@ -400,6 +415,83 @@ def test_streams_and_graph(mi, dev, bits):
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(out, eager))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q,kv", [([1] * 5, [900, 64, 2000, 3, 33]), ([70, 3, 200], [90, 2500, 700])])
+def test_two_streams_at_once(mi, dev, bits, q, kv):
+    """Two calls in flight, each with parts of its own, and the same in a graph."""
+    import torch
+
+    b = hold(mi, Batch(q, kv, 16, 8, 2, 128, seed=4, one_each=max(q) == 1), bits)
+    qs = [b.q, make(b.q.shape, 77)]
+    how = dict(q_start=b.q_start, max_kv_len=max(kv), sync=False)
+    if b.q_start is not None:
+        how["max_q_len"] = max(q)
+
+    def call(x):
+        return mi.paged_attn_quant(x, b.c, b.pages, b.kv_len, **how)
+
+    want = [call(x).clone() for x in qs]
+    main, streams = torch.cuda.current_stream(), [torch.cuda.Stream() for _ in qs]
+
+    def both():
+        main = torch.cuda.current_stream()
+        out = []
+        for x, s in zip(qs, streams):
+            s.wait_stream(main)
+            with torch.cuda.stream(s):
+                out.append(call(x))
+        for s in streams:
+            main.wait_stream(s)
+        return out
+
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(both(), want))
+    main.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = both()
+    for seed in (8, 9):
+        for x in qs:
+            x.copy_(make(x.shape, seed))
+        want = [call(x).clone() for x in qs]
+        for t in out:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q,kv", [([1] * 4, [900, 64, 2000, 3]), ([3, 40, 150], [2100, 300, 200])])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_a_query_of_nan_stays_in_its_row(mi, dev, bits, q, kv, what):
+    import torch
+
+    b = hold(mi, Batch(q, kv, 16, 4, 2, 64, seed=6, one_each=max(q) == 1), bits)
+    want, wl = run(mi, b)
+    row = sum(q) // 2
+    b.q[row, 1, 5] = what
+    got, gl = run(mi, b)
+    assert torch.isnan(got[row, 1]).all()
+    others = torch.ones(got.shape[:2], dtype=torch.bool, device="cuda")
+    others[row, 1] = False
+    assert torch.equal(got[others], want[others]) and torch.equal(gl[others], wl[others])
+
+
+def test_tables_wider_than_their_pages(mi, dev):
+    """Views of a wider page table, and of longer tables of lengths."""
+    import torch
+
+    b = hold(mi, Batch([3, 1, 20], [50, 700, 64], 16, 4, 2, 64, seed=8), 4)
+    want, lse = run(mi, b)
+    wide = torch.full((3, b.pages.shape[1] + 5), 1 << 30, dtype=torch.int32, device="cuda")
+    wide[:, :b.pages.shape[1]] = b.pages
+    b.pages = wide[:, :b.pages.shape[1]]
+    b.kv_len = torch.cat([b.kv_len, b.kv_len])[:3]
+    got, lse2 = run(mi, b)
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
 
 
 def test_empty_calls(mi, dev):

@@ -79,6 +79,18 @@ def test_read(mi):
     assert read(mi, v_h=32) == 2 and "of v" in _msg(mi)
 
 
+def test_read_of_k_and_v_into_one_place(mi):
+    import torch
+
+    c = mi.quant_cache(6, 2, 16, 64, 4, device="cpu")
+    tables = torch.zeros(5, 3, dtype=torch.int32), torch.ones(5, dtype=torch.int32)
+    out = torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="same memory"):
+        mi.kv_read_quant(c, *tables, k_out=out[:, :2], v_out=out[:, :2])
+    with pytest.raises(ValueError, match="GPU"):
+        mi.kv_read_quant(c, *tables, k_out=out[:, :2], v_out=out[:, 2:])
+
+
 def test_attention(mi):
     assert attend(mi, nH=0) == 0
     assert attend(mi, mq=-1) == 1 and attend(mi, mk=-1) == 1
