@@ -539,8 +539,8 @@ int mi_kv_read_quant(void* stream, void* k, int64_t k_t, int64_t k_h, void* v, i
 /*
  * mi_paged_attn over a cache of 8 or 4 bits: its results are those of mi_paged_attn over the values that
  * the cache stands for.  Arguments, workspace and refusals as there; head_dim 32, 64, 96 or 128.  A group that
- * reads back as NaN makes the output NaN of every row that sees it (of V: in that group's components), and may do
- * so in the sequence's rows before it.
+ * reads back as NaN makes the output NaN of every row that sees it (of V: in that group's components) and of no
+ * other.
  */
 int mi_paged_attn_quant(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h,
                         float* lse, int64_t n_heads, const mi_quant_cache* cache, const mi_paged_seqs* seqs,

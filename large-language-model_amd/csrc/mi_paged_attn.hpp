@@ -336,9 +336,10 @@ struct PaRows {
     if constexpr (!STREAMED) __builtin_amdgcn_s_setprio(0);
   }
 
-  // Writes O and lse, or the part of a piece.
+  // Writes O and lse, or the part of a piece; nan(c): components 32c .. 32c + 31 of this lane's row are NaN.
+  template <class Nan>
   __device__ __forceinline__ void end(const AttnParams& p, const PaTile& t, int wave, int n_packed, int piece,
-                                      bool whole) {
+                                      bool whole, Nan nan) {
     if (32 * wave + l32 >= n_packed) return;
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
@@ -347,24 +348,28 @@ struct PaRows {
     if (whole) {
       uint16_t* out = p.o + row * p.o_t + (int64_t)head * p.o_h;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c) {
+        const float by = nan(c) ? NAN : inv;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (32 * c + 8 * q < p.d)
             *(u32x2_t*)(out + 32 * c + 8 * q + 4 * h32) =
-                u32x2_t{pack_bf16x2(o[c][4 * q] * inv, o[c][4 * q + 1] * inv),
-                        pack_bf16x2(o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv)};
+                u32x2_t{pack_bf16x2(o[c][4 * q] * by, o[c][4 * q + 1] * by),
+                        pack_bf16x2(o[c][4 * q + 2] * by, o[c][4 * q + 3] * by)};
+      }
       if (p.lse && h32 == 0) p.lse[row * p.n_heads + head] = lse2 * 0.69314718055994531f;
     } else {
       const int64_t at = ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head;
       float* out = p.part_o + at * p.d;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c) {
+        const float by = nan(c) ? NAN : inv;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (32 * c + 8 * q < p.d)
-            *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{o[c][4 * q] * inv, o[c][4 * q + 1] * inv,
-                                                                   o[c][4 * q + 2] * inv, o[c][4 * q + 3] * inv};
+            *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{o[c][4 * q] * by, o[c][4 * q + 1] * by,
+                                                                   o[c][4 * q + 2] * by, o[c][4 * q + 3] * by};
+      }
       if (h32 == 0) p.part_lse[at] = lse2;
     }
   }
@@ -390,14 +395,15 @@ constexpr int PF_PITCH = D + 4;  // floats of a row of a wave's sums: its 16-byt
 
 // Joins the sums of a workgroup's waves over one tile of few rows: o[c][e] is component 16c + 4g + e of row
 // l16, l_run a lane's share of its weights' sum. `ring`: LDS, `pitch` bytes for each wave, with nothing on its way to it.
-// O and lse are written if the keys are all of the tile's (whole), else the part at part_at(row, head).
+// O and lse are written if the keys are all of the tile's (whole), else the part at part_at(row, head); nan(token, c):
+// components 32c .. 32c + 31 of the token's row are NaN.
 struct PfWaves {
   float wm[PF_WAVES][PF_ROWS], wl[PF_WAVES][PF_ROWS];
 };
-template <int D, class PartAt>
+template <int D, class PartAt, class Nan>
 __device__ __forceinline__ void pf_join_waves(const AttnParams& p, char* ring, int pitch, PfWaves& lds, const PaTile& t,
                                               int kvh, int n_packed, const f32x4_t (&o)[D / 16], float m_run, float l_run,
-                                              bool whole, PartAt part_at) {
+                                              bool whole, PartAt part_at, Nan nan) {
   constexpr int ND = D / 16;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
   const float sl2 = p.scale_log2;
@@ -433,7 +439,7 @@ __device__ __forceinline__ void pf_join_waves(const AttnParams& p, char* ring, i
       for (int w = 0; w < PF_WAVES; ++w)
         s += f[w] * *(const f32x4_t*)((const float*)(ring + w * pitch) + r * PF_PITCH<D> + c);
       if (c >= p.d) continue;
-      s *= inv;
+      s *= nan(rt, c / 32) ? NAN : inv;
       if (whole)
         *(u32x2_t*)(p.o + row * p.o_t + (int64_t)rh * p.o_h + c) = u32x2_t{pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
       else

@@ -36,6 +36,38 @@ struct Quarter {
 #undef MIG_GLOBAL
   }
   __device__ __forceinline__ u32x4_t eight(int i) const { return kv_eight<BITS>(w + i * (BITS / 4), kv_power(scale)); }
+  // A group of NaN becomes zeros (its codes are); whether it was one.
+  __device__ __forceinline__ bool hide() {
+    const bool nan = scale == 255;
+    scale = nan ? 0 : scale;
+    return nan;
+  }
+};
+
+// Groups of NaN of V among keys that not every row of a tile sees.  A weight of 0 times NaN is NaN, so there they are
+// held as zeros; where any was, the keys [from, to) are looked at once more at the end for the first such key of each group,
+// and the rows that see one get their NaN.
+struct PqNan {
+  int first[4] = {INT32_MAX, INT32_MAX, INT32_MAX, INT32_MAX};
+  __device__ __forceinline__ void look(const QuantParams& p, const PaTile& t, int kvh, int from, int to) {
+    const uint8_t* scales = p.vs + kvh * p.scale_head;
+    for (int base = from; base < to; base += 64) {
+      const int key = base + (int)(threadIdx.x & 63), page = key < to ? page_of(p.pv, t.s, key) : -1;
+      const uint8_t* sc = scales + page * p.scale_page + (key & ((1 << p.pv.page_shift) - 1)) * p.scale_slot;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t nan = __ballot(page >= 0 && KV_GROUP * i < p.d && sc[i] == 255);
+        if (nan) first[i] = min(first[i], base + (int)__builtin_ctzll(nan));
+      }
+    }
+  }
+  // bit i: a row of `lim` keys sees a NaN of group i
+  __device__ __forceinline__ uint32_t seen(int lim) const {
+    uint32_t groups = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) groups |= lim > first[i] ? 1u << i : 0;
+    return groups;
+  }
 };
 
 // Codes and scale bytes of keys that no row sees, and of components past head_dim: zeros times 2^-127.
@@ -61,12 +93,14 @@ struct PqShared {
   __attribute__((aligned(16))) char v[PF_WAVES * PqLds<D>::BYTES];
   int table[PF_TABLE];
   PfWaves waves;
+  int hidden[PF_WAVES];  // of each: whether it held a group of NaN as zeros
 };
 
 // Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
 // part, at part_at(row of the sequence, head).  Every wave takes 32-key blocks of its own, whose codes come into
 // registers DEPTH blocks ahead.
-template <int D, int BITS, class PartAt>
+// ONE: the tile's rows are of one token.
+template <int D, int BITS, bool ONE, class PartAt>
 __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& lds, const PaTile& t, int kvh, int k_begin,
                                            int k_end, bool whole, PartAt part_at) {
   using L = PqLds<D>;
@@ -81,6 +115,8 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
   const int pr = t.first + min(l16, n_packed - 1);
   const int token = pr / p.group, head = kvh * p.group + pr - token * p.group;
   const int lim = t.limit(p, token), lim_lo = t.limit(p, t.first / p.group);
+  const bool uneven = !ONE && lim_lo < t.end(p);
+  if (!ONE) lds.hidden[wave] = 0;
 
   // lane (g, l16) holds the components of quarter g of K's row and of Q's: product s takes eight of each quarter
   u32x4_t qf[NS];
@@ -192,7 +228,11 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
     const u32x2_t lo = read_tr16(v_rd[c]), hi = read_tr16(v_rd[c] + 16 * L::ROW);
     return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
   };
-  auto work = [&](const Block& b, int base) __attribute__((always_inline)) {
+  auto work = [&](Block& b, int base) __attribute__((always_inline)) {
+    if (uneven && base + PF_KEYS > lim_lo) {
+      if (b.v[0].hide()) lds.hidden[wave] = 1;
+      if (b.v[1].hide()) lds.hidden[wave] = 1;
+    }
     // V goes through LDS, which serves a wave in order, to its transposing reads
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -281,8 +321,12 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
            (DEPTH < 4 || step(ring[DEPTH < 4 ? 0 : 3]))) {
     }
   }
+  PqNan nan;
   __syncthreads();  // V's place takes the waves' sums
-  pf_join_waves<D>(p, lds.v, L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at);
+  if (!ONE && (lds.hidden[0] | lds.hidden[1] | lds.hidden[2] | lds.hidden[3]))
+    nan.look(p, t, kvh, max(k_begin, lim_lo - PF_KEYS + 1), k_end);
+  pf_join_waves<D>(p, lds.v, L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at,
+                   [&](int token, int c) { return !ONE && (nan.seen(t.limit(p, token)) >> c) & 1; });
 }
 
 // Many rows: a workgroup converts each 64-key block once, into LDS as the cache in bf16 would have it, and its waves
@@ -296,6 +340,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     __attribute__((aligned(16))) char ring[2 * STAGE];
     PqShared<D> few;
   } lds;
+  __shared__ int hidden[4];  // of each wave: whether it held a group of NaN as zeros
   const uint32_t lds0 = lds_addr(lds.ring);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
 
@@ -311,7 +356,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
 
   const int n_packed = min(t.n * p.group - t.first, PA_ROWS);
   if (n_packed <= PF_ROWS) {
-    pq_segment<D, BITS>(p, lds.few, t, kvh, k_begin, k_end, whole,
+    pq_segment<D, BITS, false>(p, lds.few, t, kvh, k_begin, k_end, whole,
                         [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
     return;
   }
@@ -351,6 +396,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     vq.load(ok ? vbase + off : zero, ok ? vsbase + soff : zero);
   };
 
+  const int lim_lo = t.limit(p, t.first / p.group);
+  hidden[wave] = 0;
   const int n_blocks = uniform((k_end - k_begin + PA_KEYS - 1) / PA_KEYS);
   if (n_blocks > 0) {
     look_up(k_begin);
@@ -361,6 +408,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     const uint64_t seen = seen_next;
     const int base = k_begin + j * PA_KEYS;
     const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
+    if (lim_lo < end && base + PA_KEYS > lim_lo && vq.hide()) hidden[wave] = 1;
 #pragma unroll
     for (int i = 0; i < Q4::EIGHTS; ++i) {
       *(lds_u32x4_t*)(uintptr_t)(st + k_wr[i]) = kq.eight(i);
@@ -373,7 +421,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     lds_ring_barrier();  // everyone's share of block j is in place, and block j - 1 has been read
     if (wave_has_rows) rows.block(st, base, seen);
   }
-  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole);
+  PqNan nan;
+  if (n_blocks > 0 && (hidden[0] | hidden[1] | hidden[2] | hidden[3]))  // set before the last block's barrier
+    nan.look(p, t, kvh, max(k_begin, lim_lo - PA_KEYS + 1), k_end);
+  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole, [&](int c) { return (nan.seen(rows.lim) >> c) & 1; });
 }
 
 // A tile's keys in pieces, each a workgroup's; the order of the workgroups as in mi_paged.hip.
@@ -389,7 +440,7 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
   const int end = t.end(p), plen = pa_piece(p, end);
   if (piece > 0 && (int64_t)piece * plen >= end) return;
   const int k_begin = piece * plen;
-  pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_begin + min(plen, end - k_begin), plen >= end,
+  pq_segment<D, BITS, false>(p, lds, t, kvh, k_begin, k_begin + min(plen, end - k_begin), plen >= end,
                       [&](int row, int head) { return ((int64_t)piece * p.pv.total_q + row) * p.n_heads + head; });
 }
 
@@ -404,7 +455,7 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
   const int kvh = uniform(blockIdx.x % p.n_kv);
   pf_over_share<PQ_EXTRA>(p, prefix, uniform((int)(blockIdx.x / p.n_kv)),
                           [&](const PaTile& t, int k_begin, int k_end, bool whole, auto part_at) __attribute__((always_inline)) {
-                            pq_segment<D, BITS>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
+                            pq_segment<D, BITS, true>(p, lds, t, kvh, k_begin, k_end, whole, part_at);
                           });
 }
 

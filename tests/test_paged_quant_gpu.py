@@ -480,6 +480,40 @@ def test_a_query_of_nan_stays_in_its_row(mi, dev, bits, q, kv, what):
     assert torch.equal(got[others], want[others]) and torch.equal(gl[others], wl[others])
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("q,kv,nH,nKV,d", [([4, 3], [50, 600], 4, 2, 64), ([16], [16], 1, 1, 32), ([40, 150], [100, 200], 8, 2, 128),
+                                           ([300], [2500], 12, 12, 64), ([7], [3000], 4, 4, 96), ([129, 64], [129, 3000], 4, 2, 96),
+                                           ([17, 5], [33, 400], 20, 1, 128)])
+def test_nan_reaches_no_row_before_its_key(mi, dev, bits, q, kv, nH, nKV, d):
+    """Groups of NaN of new tokens: rows before the token are what they were, the others NaN (of V: in the group)."""
+    import torch
+
+    b = hold(mi, Batch(q, kv, 16, nH, nKV, d, seed=9), bits)
+    ways = [({}, *run(mi, b)), (dict(workspace=None), *run(mi, b, workspace=None))]
+    want = ways[0][1]
+    for part in ("v", "k"):
+        scale = b.c.v_scale if part == "v" else b.c.k_scale
+        marks, none = [], torch.zeros_like(want, dtype=torch.bool)
+        for s, (n, m) in enumerate(zip(q, kv)):
+            for i, j in enumerate(sorted({n // 3, n // 2, n - 1})):
+                at = m - n + j
+                h, group = i % nKV, (i + s) % (d // 32)
+                marks.append((int(b.table[s, at // 16]), h, at % 16, group))
+                comps = slice(32 * group, 32 * group + 32) if part == "v" else slice(None)
+                none[b.starts[s] + j:b.starts[s + 1], h * (nH // nKV):(h + 1) * (nH // nKV), comps] = True
+        was = [int(scale[x]) for x in marks]
+        for x in marks:
+            scale[x] = 255
+        for kw, o, l in ways:
+            got, lse = run(mi, b, **kw)
+            assert torch.equal(torch.isnan(got), none)
+            assert torch.equal(got[~none], o[~none])
+            gone = none.any(-1) if part == "k" else torch.zeros_like(none[..., 0])
+            assert torch.equal(torch.isnan(lse), gone) and torch.equal(lse[~gone], l[~gone])
+        for x, y in zip(marks, was):
+            scale[x] = y
+
+
 def test_tables_wider_than_their_pages(mi, dev):
     """Views of a wider page table, and of longer tables of lengths."""
     import torch
