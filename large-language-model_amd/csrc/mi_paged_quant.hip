@@ -6,6 +6,12 @@
 // which the codes stand for.
 //
 // A quarter of a row (head_dim / 4 components, within one group) is what a lane loads and converts.
+//
+// Few rows are bound by the loads of codes and scale bytes, many by their waves' chains of products and exponentials. On
+// an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with no arithmetic at all 5.5) and 5.9 in 8 bits; 64 sequences of
+// 500 to 8000 keys in 4 bits 28.5 us (in bf16 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095
+// keys 75 (69.5), of whose busy CUs' clocks the matrix cores have 41 % and vector instructions 50 %.
+// The plan's borders are those of the cache in bf16: others took the chunks to 72 at best, mixed rows from 34.4 to 34.5.
 #include <hip/hip_runtime.h>
 
 #include "mi_kv_quant.hpp"
@@ -98,14 +104,16 @@ struct PqShared {
 
 // Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
 // part, at part_at(row of the sequence, head).  Every wave takes 32-key blocks of its own, whose codes come into
-// registers DEPTH blocks ahead.
+// registers DEPTH blocks ahead: with one more the steady rate is the same, and a segment starts and ends later (64
+// sequences of 500 to 8000 keys in 4 bits 28.5 us, so 29.9; 16 in 8 bits 38.6 and 39.9). A load costs a CU some 30
+// clocks whatever its width, so a lane's are as wide as its codes.
 // ONE: the tile's rows are of one token.
 template <int D, int BITS, bool ONE, class PartAt>
 __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& lds, const PaTile& t, int kvh, int k_begin,
                                            int k_end, bool whole, PartAt part_at) {
   using L = PqLds<D>;
   using Q4 = Quarter<D, BITS>;
-  constexpr int NS = D / 32, ND = D / 16, DEPTH = BITS == 4 ? 3 : 2, STEP = PF_KEYS * PF_WAVES;
+  constexpr int NS = D / 32, ND = D / 16, DEPTH = 2, STEP = PF_KEYS * PF_WAVES;
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // or what a segment needs at its ends would be kept in registers from one to the next
   const int wave = uniform(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
@@ -316,9 +324,8 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
       base += STEP;
       return base < k_stop;
     };
-    static_assert(DEPTH >= 2 && DEPTH <= 4, "written out for these");
-    while (step(ring[0]) && step(ring[1]) && (DEPTH < 3 || step(ring[DEPTH < 3 ? 0 : 2])) &&
-           (DEPTH < 4 || step(ring[DEPTH < 4 ? 0 : 3]))) {
+    static_assert(DEPTH == 2, "written out for two");
+    while (step(ring[0]) && step(ring[1])) {
     }
   }
   PqNan nan;
