@@ -7,10 +7,11 @@
 //
 // A quarter of a row (head_dim / 4 components, within one group) is what a lane loads and converts.
 //
-// Few rows are bound by the loads of codes and scale bytes, many by their waves' chains of products and exponentials. On
-// an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with no arithmetic at all 5.5) and 5.9 in 8 bits; 64 sequences of
-// 500 to 8000 keys in 4 bits 28.5 us (in bf16 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095
-// keys 75 (69.5), of whose busy CUs' clocks the matrix cores have 41 % and vector instructions 50 %.
+// Few rows are bound by HBM where the keys are many, else by a wave's chain for a block (0.6 us with one wave a SIMD);
+// many by their waves' chains of products and exponentials.  On an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with
+// no arithmetic at all 5.5) and 5.7 to 5.9 in 8 bits; 64 sequences of 500 to 8000 keys in 4 bits 28.5 us (in bf16
+// 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095 keys 75 (69.5), of whose busy CUs' clocks the
+// matrix cores have 41 % and vector instructions 50 %.
 // The plan's borders are those of the cache in bf16: others took the chunks to 72 at best, mixed rows from 34.4 to 34.5.
 #include <hip/hip_runtime.h>
 
@@ -105,8 +106,8 @@ struct PqShared {
 // Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
 // part, at part_at(row of the sequence, head).  Every wave takes 32-key blocks of its own, whose codes come into
 // registers DEPTH blocks ahead: with one more the steady rate is the same, and a segment starts and ends later (64
-// sequences of 500 to 8000 keys in 4 bits 28.5 us, so 29.9; 16 in 8 bits 38.6 and 39.9). A load costs a CU some 30
-// clocks whatever its width, so a lane's are as wide as its codes.
+// sequences of 500 to 8000 keys in 4 bits 28.5 us, so 29.9; 16 in 8 bits 38.6 and 39.9).  One load for all scale
+// bytes of a block, given to the lanes by shuffles, was slower (30.6): it makes the chain longer.
 // ONE: the tile's rows are of one token.
 template <int D, int BITS, bool ONE, class PartAt>
 __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& lds, const PaTile& t, int kvh, int k_begin,

@@ -514,6 +514,34 @@ def test_nan_reaches_no_row_before_its_key(mi, dev, bits, q, kv, nH, nKV, d):
             scale[x] = y
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+def test_scales_anywhere_and_padded_codes(mi, dev, bits):
+    """Scale bytes at odd addresses with odd strides, codes with gaps: appended to, read back and attended over."""
+    import torch
+
+    b = hold(mi, Batch([3, 1, 150], [50, 700, 260], 16, 8, 2, 64, seed=12), bits)
+    want, lse = run(mi, b)
+    n, kv, P, nb = b.c.k.shape
+    c = []
+    for t in b.c[:2]:
+        x = torch.full((n, kv + 1, P + 1, nb + 16), 255, dtype=torch.uint8, device="cuda")[:, :kv, 1:, 16:]
+        c.append(x.copy_(t))
+    for t in b.c[2:]:
+        x = torch.full((n * (kv * P * 7 + 3) + 9,), 255, dtype=torch.uint8, device="cuda")
+        x = x.as_strided(t.shape, (kv * P * 7 + 3, P * 7, 7, 1), 5)
+        c.append(x.copy_(t))
+    plain, b.c = b.c, mi.QuantCache(*c)
+    got, lse2 = run(mi, b)
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    k, v = make((154, 2, 64), 1), make((154, 2, 64), 2)
+    for cache in (plain, b.c):
+        mi.kv_append_quant(k, v, cache, b.pages, b.kv_len, q_start=b.q_start)
+    for x, y in zip(plain, b.c):
+        assert torch.equal(x, y)
+    for x, y in zip(*(mi.kv_read_quant(cache, b.pages, b.kv_len, q_start=b.q_start, rows=154) for cache in (plain, b.c))):
+        assert torch.equal(x, y)
+
+
 def test_tables_wider_than_their_pages(mi, dev):
     """Views of a wider page table, and of longer tables of lengths."""
     import torch
