@@ -12,7 +12,14 @@
 // no arithmetic at all 5.5) and 5.7 to 5.9 in 8 bits; 64 sequences of 500 to 8000 keys in 4 bits 28.5 us (in bf16
 // 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095 keys 75 (69.5), of whose busy CUs' clocks the
 // matrix cores have 41 % and vector instructions 50 %.
-// The plan's borders are those of the cache in bf16: others took the chunks to 72 at best, mixed rows from 34.4 to 34.5.
+//
+// The plan's borders are those of the cache in bf16 (pa_plan), and hold here (us, 16 / 4 heads of 128, 4 bits). One piece
+// / pieces of 128 keys: 512 keys 8.5 / 9.7, 1024 keys 11.5 / 9.8.  Pieces / even shares, which the
+// last two columns take:
+//    sequences x keys   64 x 2000   256 x 2000   16 x 4000    16 x 8000    64 x 8000
+//              uneven   19.2/17.0   31.7/36.1    15.1/13.9    22.2/15.7    55.4/28.4
+//                even   20.3/22.9   50.2/54.4    16.5/16.4    23.3/22.8    57.7/51.7
+// Many rows: twice as many pieces or longer ones took the chunks to 72 at best, mixed rows from 34.4 to 34.5.
 #include <hip/hip_runtime.h>
 
 #include "mi_kv_quant.hpp"
