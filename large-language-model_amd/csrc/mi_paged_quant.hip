@@ -11,7 +11,7 @@
 // many by their waves' chains of products and exponentials.  On an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with
 // no arithmetic at all 5.5) and 5.7 to 5.9 in 8 bits; 64 sequences of 500 to 8000 keys in 4 bits 28.5 us (in bf16
 // 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095 keys 75 (69.5), of whose busy CUs' clocks the
-// matrix cores have 41 % and vector instructions 50 %.
+// matrix cores have 43 % and vector instructions 54 %.
 //
 // The plan's borders are those of the cache in bf16 (pa_plan), and hold here (us, 16 / 4 heads of 128, 4 bits). One piece
 // / pieces of 128 keys: 512 keys 8.5 / 9.7, 1024 keys 11.5 / 9.8.  Pieces / even shares, which the
