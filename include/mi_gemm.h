@@ -497,7 +497,8 @@ typedef enum mi_kv_format {
  * half a step at most; the group's scale byte is e + 127 and each code is x / 2^e rounded to the
  * nearest number of the type, ties to even, at most 448 or 6.  A group with an infinity, a NaN or a
  * magnitude of 2^127 or more has scale byte 255, codes 0, and reads back as NaN.  Every value read
- * back is exact in bf16.  Pages as in mi_paged_cache: the codes of head h of slot i of page p are the
+ * back is exact in bf16.  In a cache that something else has filled, any codes under byte 255 and the
+ * e4m3 codes 0x7f and 0xff under any byte read back as NaN.  Pages as in mi_paged_cache: the codes of head h of slot i of page p are the
  * head_dim (e4m3) or head_dim / 2 (e2m1) bytes at k + p*page_stride + h*head_stride + i*slot_stride, their
  * scale bytes the head_dim / 32 at k_scale + p*scale_page_stride + h*scale_head_stride + i*scale_slot_stride,
  * and v alike.  head_dim is a multiple of 32; k and v are 16-byte aligned and the strides of codes
@@ -538,9 +539,9 @@ int mi_kv_read_quant(void* stream, void* k, int64_t k_t, int64_t k_h, void* v, i
 
 /*
  * mi_paged_attn over a cache of 8 or 4 bits: its results are those of mi_paged_attn over the values that
- * the cache stands for.  Arguments, workspace and refusals as there; head_dim 32, 64, 96 or 128.  A group that
- * reads back as NaN makes the output NaN of every row that sees it (of V: in that group's components) and of no
- * other.
+ * the cache stands for.  Arguments, workspace and refusals as there; head_dim 32, 64, 96 or 128.  A component
+ * that reads back as NaN makes the output NaN of every row that sees its token (of V: in that component) and of
+ * no other row.
  */
 int mi_paged_attn_quant(void* stream, const void* Q, int64_t q_t, int64_t q_h, void* O, int64_t o_t, int64_t o_h,
                         float* lse, int64_t n_heads, const mi_quant_cache* cache, const mi_paged_seqs* seqs,

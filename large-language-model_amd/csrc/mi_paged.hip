@@ -243,7 +243,7 @@ __device__ __forceinline__ void pf_segment(const AttnParams& p, PfShared<D>& lds
   }  static_assert(PF_ROWS * PF_PITCH<D> * 4 <= 2 * L::BYTES, "a wave's sums fit its ring");
   wait_vmcnt<0>();  // nothing is on its way to the ring any more
   pf_join_waves<D>(p, lds.ring, 2 * L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at,
-                   [](int, int) { return false; });
+                   [](int, int) { return 0u; });
 }
 
 template <int D>
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     const uint32_t st = lds0 + (uint32_t)((j & 1) * STAGE);
     if (wave_has_rows) rows.block(st, base, seen);
   }
-  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole, [](int) { return false; });
+  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole, [](int) { return 0u; });
 }
 
 // A tile's keys in pieces, each a workgroup's.

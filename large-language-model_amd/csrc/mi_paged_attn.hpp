@@ -333,7 +333,7 @@ struct PaRows {
     if constexpr (!STREAMED) __builtin_amdgcn_s_setprio(0);
   }
 
-  // Writes O and lse, or the part of a piece; nan(c): components 32c .. 32c + 31 of this lane's row are NaN.
+  // Writes O and lse, or the part of a piece; bit i of nan(c): component 32c + i of this lane's row is NaN.
   template <class Nan>
   __device__ __forceinline__ void end(const AttnParams& p, const PaTile& t, int wave, int n_packed, int piece,
                                       bool whole, Nan nan) {
@@ -346,13 +346,13 @@ struct PaRows {
       uint16_t* out = p.o + row * p.o_t + (int64_t)head * p.o_h;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const float by = nan(c) ? NAN : inv;
+        const uint32_t gone = nan(c) >> (4 * h32);
+        auto at = [&](int q, int e) { return o[c][4 * q + e] * ((gone >> (8 * q + e)) & 1 ? NAN : inv); };
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (32 * c + 8 * q < p.d)
             *(u32x2_t*)(out + 32 * c + 8 * q + 4 * h32) =
-                u32x2_t{pack_bf16x2(o[c][4 * q] * by, o[c][4 * q + 1] * by),
-                        pack_bf16x2(o[c][4 * q + 2] * by, o[c][4 * q + 3] * by)};
+                u32x2_t{pack_bf16x2(at(q, 0), at(q, 1)), pack_bf16x2(at(q, 2), at(q, 3))};
       }
       if (p.lse && h32 == 0) p.lse[row * p.n_heads + head] = lse2 * 0.69314718055994531f;
     } else {
@@ -360,12 +360,12 @@ struct PaRows {
       float* out = p.part_o + at * p.d;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const float by = nan(c) ? NAN : inv;
+        const uint32_t gone = nan(c) >> (4 * h32);
+        auto at = [&](int q, int e) { return o[c][4 * q + e] * ((gone >> (8 * q + e)) & 1 ? NAN : inv); };
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (32 * c + 8 * q < p.d)
-            *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{o[c][4 * q] * by, o[c][4 * q + 1] * by,
-                                                                   o[c][4 * q + 2] * by, o[c][4 * q + 3] * by};
+            *(f32x4_t*)(out + 32 * c + 8 * q + 4 * h32) = f32x4_t{at(q, 0), at(q, 1), at(q, 2), at(q, 3)};
       }
       if (h32 == 0) p.part_lse[at] = lse2;
     }
@@ -392,8 +392,8 @@ constexpr int PF_PITCH = D + 4;  // floats of a row of a wave's sums: its 16-byt
 
 // Joins the sums of a workgroup's waves over one tile of few rows: o[c][e] is component 16c + 4g + e of row
 // l16, l_run a lane's share of its weights' sum. `ring`: LDS, `pitch` bytes for each wave, with nothing on its way to it.
-// O and lse are written if the keys are all of the tile's (whole), else the part at part_at(row, head); nan(token, c):
-// components 32c .. 32c + 31 of the token's row are NaN.
+// O and lse are written if the keys are all of the tile's (whole), else the part at part_at(row, head); bit i of
+// nan(token, c): component 32c + i of the token's row is NaN.
 struct PfWaves {
   float wm[PF_WAVES][PF_ROWS], wl[PF_WAVES][PF_ROWS];
 };
@@ -436,7 +436,9 @@ __device__ __forceinline__ void pf_join_waves(const AttnParams& p, char* ring, i
       for (int w = 0; w < PF_WAVES; ++w)
         s += f[w] * *(const f32x4_t*)((const float*)(ring + w * pitch) + r * PF_PITCH<D> + c);
       if (c >= p.d) continue;
-      s *= nan(rt, c / 32) ? NAN : inv;
+      const uint32_t gone = nan(rt, c / 32) >> (c % 32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] *= (gone >> e) & 1 ? NAN : inv;
       if (whole)
         *(u32x2_t*)(p.o + row * p.o_t + (int64_t)rh * p.o_h + c) = u32x2_t{pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3])};
       else

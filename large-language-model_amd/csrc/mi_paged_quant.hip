@@ -63,37 +63,68 @@ struct Quarter {
           w[(i | bit) * N + n] = is ? a : b;
         }
   }
-  // A group of NaN becomes zeros (its codes are); whether it was one.
+  // e4m3's codes of NaN, 0x7f and 0xff, in dword i: bit 7 of their bytes.
+  __device__ __forceinline__ uint32_t nan_codes(int i) const { return ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+  // Whether component c of the quarter reads back as NaN.
+  __device__ __forceinline__ bool nan(int c) const {
+    return scale == 255 || (BITS == 8 && (nan_codes(c / 4) >> (8 * (c & 3) + 7)) & 1);
+  }
+  // What reads back as NaN becomes zero (in a group of byte 255 the codes stay, times 2^-127); whether there was any.
   __device__ __forceinline__ bool hide() {
-    const bool nan = scale == 255;
-    scale = nan ? 0 : scale;
-    return nan;
+    bool any = scale == 255;
+    scale = any ? 0 : scale;
+    if constexpr (BITS == 8) {
+      uint32_t codes = 0;
+#pragma unroll
+      for (int i = 0; i < BYTES / 4; ++i) codes |= nan_codes(i);
+      if (codes) {
+        any = true;
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) {
+          const uint32_t m = nan_codes(i);
+          w[i] &= ~(m | (m - (m >> 7)));
+        }
+      }
+    }
+    return any;
   }
 };
 
-// Groups of NaN of V among keys that not every row of a tile sees.  A weight of 0 times NaN is NaN, so there they are
-// held as zeros; where any was, the keys [from, to) are looked at once more at the end for the first such key of each group,
-// and the rows that see one get their NaN.
+// NaN of V among keys that not every row of a tile sees.  A weight of 0 times NaN is NaN, so there it is held as zeros;
+// where any was, the workgroup looks at the keys [from, to) once more at the end for the first one at which each component
+// is NaN, and the rows that see it get their NaN.  The append writes NaN by whole groups; a cache that something else
+// has filled may hold codes of NaN, too.
+template <int D, int BITS>
 struct PqNan {
-  int first[4] = {INT32_MAX, INT32_MAX, INT32_MAX, INT32_MAX};
-  __device__ __forceinline__ void look(const QuantParams& p, const PaTile& t, int kvh, int from, int to) {
-    const uint8_t* scales = p.vs + kvh * p.scale_head;
-    for (int base = from; base < to; base += 64) {
-      const int key = base + (int)(threadIdx.x & 63), page = key < to ? page_of(p.pv, t.s, key) : -1;
-      const uint8_t* sc = scales + page * p.scale_page + (key & ((1 << p.pv.page_shift) - 1)) * p.scale_slot;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint64_t nan = __ballot(page >= 0 && KV_GROUP * i < p.d && sc[i] == 255);
-        if (nan) first[i] = min(first[i], base + (int)__builtin_ctzll(nan));
-      }
+  using Q4 = Quarter<D, BITS>;
+  const int* first;  // [D] in LDS
+  bool any = false;
+  __device__ __forceinline__ PqNan(const int* table) : first(table) {}
+  // All threads together; table: D entries of LDS that nothing reads any more once everyone has come here.
+  __device__ __forceinline__ void look(const QuantParams& p, const PaTile& t, int kvh, int from, int to, int* table) {
+    any = true;
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += blockDim.x) table[i] = INT32_MAX;
+    __syncthreads();
+    const int quarter = threadIdx.x & 3, c0 = Q4::COMPS * quarter;
+    for (int key = from + (int)(threadIdx.x >> 2); key < to; key += blockDim.x >> 2) {
+      const int page = page_of(p.pv, t.s, key), slot = key & ((1 << p.pv.page_shift) - 1);
+      if (page < 0 || c0 >= p.d) continue;
+      Q4 v;
+      v.load((const uint8_t*)p.v + kvh * p.pv.head_stride + page * p.pv.page_stride + slot * p.pv.slot_stride +
+                 Q4::BYTES * quarter,
+             p.vs + kvh * p.scale_head + page * p.scale_page + slot * p.scale_slot + c0 / KV_GROUP);
+      for (int c = 0; c < Q4::COMPS; ++c)
+        if (v.nan(c)) atomicMin(&table[c0 + c], key);
     }
+    __syncthreads();
   }
-  // bit i: a row of `lim` keys sees a NaN of group i
-  __device__ __forceinline__ uint32_t seen(int lim) const {
-    uint32_t groups = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) groups |= lim > first[i] ? 1u << i : 0;
-    return groups;
+  // bit i: a row of `lim` keys sees a NaN of component 32c + i
+  __device__ __forceinline__ uint32_t seen(int lim, int c) const {
+    uint32_t comps = 0;
+    if (any)
+      for (int i = 0; i < 32; ++i) comps |= lim > first[32 * c + i] ? 1u << i : 0;
+    return comps;
   }
 };
 
@@ -120,7 +151,7 @@ struct PqShared {
   __attribute__((aligned(16))) char v[PF_WAVES * PqLds<D>::BYTES];
   int table[PF_TABLE];
   PfWaves waves;
-  int hidden[PF_WAVES];  // of each: whether it held a group of NaN as zeros
+  int hidden[PF_WAVES];  // of each: whether it held a NaN as zero
 };
 
 // Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
@@ -349,12 +380,12 @@ __device__ __forceinline__ void pq_segment(const QuantParams& p, PqShared<D>& ld
     while (step(ring[0]) && step(ring[1])) {
     }
   }
-  PqNan nan;
+  PqNan<D, BITS> nan(lds.table);
   __syncthreads();  // V's place takes the waves' sums
   if (!ONE && (lds.hidden[0] | lds.hidden[1] | lds.hidden[2] | lds.hidden[3]))
-    nan.look(p, t, kvh, max(k_begin, lim_lo - PF_KEYS + 1), k_end);
+    nan.look(p, t, kvh, max(k_begin, lim_lo - PF_KEYS + 1), k_end, lds.table);
   pf_join_waves<D>(p, lds.v, L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at,
-                   [&](int token, int c) { return !ONE && (nan.seen(t.limit(p, token)) >> c) & 1; });
+                   [&](int token, int c) { return ONE ? 0u : nan.seen(t.limit(p, token), c); });
 }
 
 // Many rows: a workgroup converts each 64-key block once, into LDS as the cache in bf16 would have it, and its waves
@@ -368,7 +399,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     __attribute__((aligned(16))) char ring[2 * STAGE];
     PqShared<D> few;
   } lds;
-  __shared__ int hidden[4];  // of each wave: whether it held a group of NaN as zeros
+  __shared__ int hidden[4];  // of each wave: whether it held a NaN as zero
   const uint32_t lds0 = lds_addr(lds.ring);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
 
@@ -455,10 +486,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     lds_ring_barrier();  // everyone's share of block j is in place, and block j - 1 has been read
     if (wave_has_rows) rows.block(st, base, seen);
   }
-  PqNan nan;
+  PqNan<D, BITS> nan(lds.few.table);
   if (n_blocks > 0 && (hidden[0] | hidden[1] | hidden[2] | hidden[3]))  // set before the last block's barrier
-    nan.look(p, t, kvh, max(k_begin, lim_lo - PA_KEYS + 1), k_end);
-  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole, [&](int c) { return (nan.seen(rows.lim) >> c) & 1; });
+    nan.look(p, t, kvh, max(k_begin, lim_lo - PA_KEYS + 1), k_end, lds.few.table);
+  if (wave_has_rows) rows.end(p, t, wave, n_packed, piece, whole, [&](int c) { return nan.seen(rows.lim, c); });
 }
 
 // A tile's keys in pieces, each a workgroup's; the order of the workgroups as in mi_paged.hip.
