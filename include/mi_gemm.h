@@ -531,7 +531,8 @@ int mi_kv_append_quant(void* stream, const void* q, int64_t q_t, int64_t q_h, vo
  * The tokens of seqs, which mi_kv_append_quant names as its new ones (the last q_start[s+1] - q_start[s] of
  * kv_len[s]; all of a sequence's where they are as many), read back: K and V [total_q, n_kv, head_dim] of
  * dtype MI_BF16 or MI_F32 (exact in both), element strides k_t, v_t between tokens and k_h, v_h between heads,
- * components contiguous, in memory of their own.  k or v may be NULL: not read.  A token that no page holds is
+ * components contiguous, in memory of their own: where K and V share an element, either may be found in it.
+ * k or v may be NULL: not read.  A token that no page holds is
  * written as zeros; rows behind the last sequence are left as they are.
  */
 int mi_kv_read_quant(void* stream, void* k, int64_t k_t, int64_t k_h, void* v, int64_t v_t, int64_t v_h, int32_t dtype,

@@ -1493,11 +1493,33 @@ def kv_append_quant(k, v, cache, pages, kv_len, q_start=None, q=None, q_out=None
                    interleaved, scale, sync)
 
 
+def _rows_meet(apart, a, b, rows, heads, size):
+    """Whether two sets of rows x heads runs of `size` bytes, of strides a and b (of rows and of heads) and that far
+    apart, have a byte in common."""
+    if rows == 0 or heads == 0 or -((rows - 1) * b[0] + (heads - 1) * b[1] + size) >= apart or \
+            apart >= (rows - 1) * a[0] + (heads - 1) * a[1] + size:
+        return False
+    if a == b and a[0] > 0:  # r and h that bring |apart - r a[0] - h a[1]| below a run
+        for h in range(1 - heads, heads):
+            rest = apart - h * a[1]
+            r = rest // a[0]
+            if any(abs(rest - i * a[0]) < size and abs(i) < rows for i in (r, r + 1)):
+                return True
+        return False
+    torch = _torch()
+    starts = [(torch.arange(rows)[:, None] * t + torch.arange(heads) * h).flatten() for t, h in (a, b)]
+    held, others = starts[0].sort().values, starts[1] + apart
+    at = torch.searchsorted(held, others)
+    after, before = held[at.clamp(max=held.numel() - 1)], held[(at - 1).clamp(min=0)]
+    return bool((((after - others).abs() < size) | ((others - before).abs() < size)).any())
+
+
 def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_out=None, parts="kv", dtype=None, sync=None):
     """The tokens that kv_append_quant with these tables has written, read back (mi_kv_read_quant): the last
     q_start[s + 1] - q_start[s] tokens of sequence s (None: its last one), K and V [rows, nKV, d] of dtype bf16
     (the default) or fp32, exact in both. rows: how many there are, q_start's last entry (a row behind it is left as it
     is; k_out or v_out say it, too). Tokens that no page holds are zeros. parts "k" or "v" reads one of the two.
+    k_out and v_out may be views of one tensor that have no element in common.
     Returns (K, V), None for the one not read."""
     if parts not in ("kv", "k", "v"):
         raise ValueError(f"parts {parts!r}: kv, k or v")
@@ -1527,8 +1549,10 @@ def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_o
         else:
             v_t, v_h = _heads_of("v_out", v_out, rows, n_kv, d, dtype)
         v_at = v_out.data_ptr()
-        if v_at and v_at == k_at:
-            raise ValueError("k_out and v_out are the same memory")
+    if k_at and v_at:
+        es = k_out.element_size()
+        if _rows_meet(v_at - k_at, (k_t * es, k_h * es), (v_t * es, v_h * es), rows, n_kv, d * es):
+            raise ValueError("k_out and v_out have elements of the same memory")
     stream = _stream_of(*cache, pages, kv_len, q_start, k_out, v_out)
     _done("mi_kv_read_quant", load_library().mi_kv_read_quant(stream, k_at, k_t, k_h, v_at, v_t, v_h, code, packed, seqs), sync)
     return k_out, v_out
