@@ -1523,8 +1523,9 @@ def kv_read_quant(cache, pages, kv_len, q_start=None, rows=None, k_out=None, v_o
     Returns (K, V), None for the one not read."""
     if parts not in ("kv", "k", "v"):
         raise ValueError(f"parts {parts!r}: kv, k or v")
-    if parts != "kv":
-        k_out, v_out = (None, v_out) if parts == "v" else (k_out, None)
+    for name, out in (("k", k_out), ("v", v_out)):
+        if out is not None and name not in parts:
+            raise ValueError(f"{name}_out with parts {parts!r}: it would not be written")
     given = k_out if k_out is not None else v_out
     if rows is None:
         if given is None and q_start is not None:

@@ -73,3 +73,14 @@ def test_against_all_places(mi):
         both[want] += 1
         assert mi._rows_meet(at[1] - at[0], strides[0], strides[1], rows, heads, d) == want, (rows, heads, d, strides, at)
     assert min(both) > 300
+
+
+@pytest.mark.parametrize("parts,other", [("k", "v_out"), ("v", "k_out")])
+def test_a_tensor_for_the_part_not_read_is_refused(mi, args, parts, other):
+    import torch
+
+    out = torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match=other):
+        mi.kv_read_quant(*args, parts=parts, **{other: out})
+    with pytest.raises(ValueError, match=other):
+        mi.kv_read_quant(*args, parts=parts, k_out=out, v_out=torch.zeros_like(out))
