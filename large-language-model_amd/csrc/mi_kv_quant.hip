@@ -34,6 +34,23 @@ struct QuantView {
   int64_t scale_page, scale_head, scale_slot;
 };
 
+// The first sequence from s on that ends behind token t (n_seqs: none), each lane on its own: steps of 1, 1, 2, 4, .. until
+// one does, and halves of the last step; the next sequence is one load away, any number of empty ones a few (two prompts of
+// 2000 tokens side by side appended in 7.2 us, with 4000 empty sequences between them in 8.2; one by one 299).
+__device__ __forceinline__ int first_after(const PagedView& pv, int s, int t) {
+  int end = s;  // sequences before s end by t; `end` is looked at next
+  for (int64_t step = 1; end < pv.n_seqs && pv.q_start[end + 1] <= t; step *= 2) {
+    s = end + 1;
+    end = (int)min((int64_t)s + step - 1, (int64_t)pv.n_seqs);
+  }
+  while (s < end) {  // in [s, end]
+    const int mid = s + (end - s) / 2;
+    if (pv.q_start[mid + 1] <= t) s = mid + 1;
+    else end = mid;
+  }
+  return s;
+}
+
 // Tokens tok0 .. tok0 + n - 1 (n <= 64) looked up by the workgroup's first wave, one a lane: page (-1: none),
 // slot and position in its sequence; page -2: a row of no sequence.
 struct Tokens {
@@ -46,7 +63,7 @@ __device__ __forceinline__ void look_up_tokens(const PagedView& pv, int64_t tok0
   bool in = true;
   if (pv.q_start) {
     s = wave_first_false(pv.n_seqs, [&](int k) { return pv.q_start[k + 1] <= (int)tok0; });
-    while (s < pv.n_seqs && pv.q_start[s + 1] <= t) ++s;
+    s = first_after(pv, s, t);
     in = s < pv.n_seqs;
     if (in) {
       seq_rows(pv, s, q0, rows);
