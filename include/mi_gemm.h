@@ -497,11 +497,13 @@ typedef enum mi_kv_format {
  * half a step at most; the group's scale byte is e + 127 and each code is x / 2^e rounded to the
  * nearest number of the type, ties to even, at most 448 or 6.  A group with an infinity, a NaN or a
  * magnitude of 2^127 or more has scale byte 255, codes 0, and reads back as NaN.  Every value read
- * back is exact in bf16.  In a cache that something else has filled, any codes under byte 255 and the
- * e4m3 codes 0x7f and 0xff under any byte read back as NaN.  Pages as in mi_paged_cache: the codes of head h of slot i of page p are the
- * head_dim (e4m3) or head_dim / 2 (e2m1) bytes at k + p*page_stride + h*head_stride + i*slot_stride, their
- * scale bytes the head_dim / 32 at k_scale + p*scale_page_stride + h*scale_head_stride + i*scale_slot_stride,
- * and v alike.  head_dim is a multiple of 32; k and v are 16-byte aligned and the strides of codes
+ * back is exact in bf16.  The other bytes written are 27 to 246 (e4m3) or 252 (e2m1).  In a cache that
+ * something else has filled, any codes under byte 255 and the e4m3 codes 0x7f and 0xff under any byte read
+ * back as NaN, and codes of 0 under byte 0 (cleared memory) as zeros; what other bytes give is not defined.
+ * Pages as in mi_paged_cache: the codes of head h of slot i of page p are the head_dim (e4m3) or
+ * head_dim / 2 (e2m1) bytes at k + p*page_stride + h*head_stride + i*slot_stride, their scale bytes the
+ * head_dim / 32 at k_scale + p*scale_page_stride + h*scale_head_stride + i*scale_slot_stride, and v
+ * alike.  head_dim is a multiple of 32; k and v are 16-byte aligned and the strides of codes
  * multiples of 16 bytes; scale bytes may lie anywhere.
  */
 typedef struct mi_quant_cache {

@@ -10,7 +10,8 @@ namespace mig {
 
 constexpr int KV_GROUP = 32;  // components that share a scale byte
 
-// The power of two of a scale byte.  255 gives infinity, which the conversions below take for NaN, of any code.
+// The power of two of a scale byte.  255 gives infinity, which the conversions below take for NaN, of any code; 0 gives 0,
+// which leaves codes of 0 zeros and any others finite.
 __device__ __forceinline__ float kv_power(uint32_t scale_byte) { return __uint_as_float(scale_byte << 23); }
 
 // Codes 2i, 2i+1 of a dword of codes times s, as two bf16: exact for every scale byte that is written.

@@ -5,7 +5,9 @@
 // and multiplies on the way, both exactly, so scores and sums are those of a bf16 cache that holds the values
 // which the codes stand for.
 //
-// A quarter of a row (head_dim / 4 components, within one group) is what a lane loads and converts.
+// A quarter of a row of up to D = 64 or 128 components is what a lane loads and converts: D / 4 of them, within one
+// group.  Quarters past head_dim are zeros that are multiplied like the others: half of them in heads of 32, one of
+// four in heads of 96.
 //
 // Few rows are bound by HBM where the keys are many, else by a wave's chain for a block (0.6 us with one wave a SIMD);
 // many by their waves' chains of products and exponentials.  On an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with
@@ -69,7 +71,7 @@ struct Quarter {
   __device__ __forceinline__ bool nan(int c) const {
     return scale == 255 || (BITS == 8 && (nan_codes(c / 4) >> (8 * (c & 3) + 7)) & 1);
   }
-  // What reads back as NaN becomes zero (in a group of byte 255 the codes stay, times 2^-127); whether there was any.
+  // What reads back as NaN becomes zero, or under byte 0 at least finite, if it had byte 255; whether there was any.
   __device__ __forceinline__ bool hide() {
     bool any = scale == 255;
     scale = any ? 0 : scale;
@@ -128,7 +130,7 @@ struct PqNan {
   }
 };
 
-// Codes and scale bytes of keys that no row sees, and of components past head_dim: zeros times 2^-127.
+// Codes and scale bytes of keys that no row sees, and of components past head_dim: zeros under byte 0, which are zeros.
 __device__ __align__(16) uint32_t pq_zero[8];
 
 // Few rows: V of a 32-key block of a wave, converted, rows of D components whose 16-byte chunks are moved so that
