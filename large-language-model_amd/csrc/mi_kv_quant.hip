@@ -11,8 +11,8 @@
 // rounded to 32 bits on the way to the code is rounded to odd, so that the one rounding that counts is the last.
 //
 // Bound by HBM where there are many tokens, by the launch and a chain of tables, pages and rows where there are few.
-// On an MI355X: 64 tokens appended in 4.0 us, 2100 of twelve prompts in 9.7 (23 MB; the rotation in 64 bits is 0.2 of
-// them), 41000 read back in 21.0 (107 MB, 5.1 TB/s: a copy's rate).
+// On an MI355X: 64 tokens appended in 4.0 us, 2100 of twelve prompts in 9.5 (23 MB; the rotation in 64 bits is 0.2 of
+// them), 41000 read back in 21.2 (107 MB, 5.0 TB/s: a copy's rate).
 #include <hip/hip_runtime.h>
 #include <math.h>
 

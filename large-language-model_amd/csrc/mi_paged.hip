@@ -240,7 +240,8 @@ __device__ __forceinline__ void pf_segment(const AttnParams& p, PfShared<D>& lds
                                                       __builtin_bit_cast(bf16x8_t, hi), o[c], 0, 0, 0);
       }
     }
-  }  static_assert(PF_ROWS * PF_PITCH<D> * 4 <= 2 * L::BYTES, "a wave's sums fit its ring");
+  }
+  static_assert(PF_ROWS * PF_PITCH<D> * 4 <= 2 * L::BYTES, "a wave's sums fit its ring");
   wait_vmcnt<0>();  // nothing is on its way to the ring any more
   pf_join_waves<D>(p, lds.ring, 2 * L::BYTES, lds.waves, t, kvh, n_packed, o, m_run, l_run, whole, part_at,
                    [](int, int) { return 0u; });

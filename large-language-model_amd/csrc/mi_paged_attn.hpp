@@ -754,7 +754,8 @@ inline int pa_prepare(AttnParams& p, PaPlan& plan, bool& launch, const void* Q, 
     return host_fail(MI_ERR_LD, "a stride of O is shorter than a row of %lld", (long long)d);
   if (Q == O && ((rows > 1 && q_t != o_t) || (n_heads > 1 && q_h != o_h)))
     return host_fail(MI_ERR_UNSUPPORTED, "in place needs the same strides of Q and O");
-  if (!(scale > 0.0f) || !isfinite(scale * 1.4426950408889634f)) return host_fail(MI_ERR_UNSUPPORTED, "scale must be positive and finite");
+  if (!(scale > 0.0f) || !isfinite(scale * 1.4426950408889634f))
+    return host_fail(MI_ERR_UNSUPPORTED, "scale must be positive and finite");
   if (rows * n_heads > INT32_MAX) return host_fail(MI_ERR_SHAPE, "total_q * n_heads exceeds 2^31-1");
   const int st = host_device();
   if (st != MI_OK) return st;

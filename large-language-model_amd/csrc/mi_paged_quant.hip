@@ -10,10 +10,12 @@
 // four in heads of 96.
 //
 // Few rows are bound by HBM where the keys are many, else by a wave's chain for a block (0.6 us with one wave a SIMD);
-// many by their waves' chains of products and exponentials.  On an MI355X: 64 x 32768 keys at 5.2 TB/s in 4 bits (with
-// no arithmetic at all 5.5) and 5.7 to 5.9 in 8 bits; 64 sequences of 500 to 8000 keys in 4 bits 28.5 us (in bf16
-// 77.5), 16 in 8 bits 38.6 (69.5); four chunks of 1024 rows over 4095 keys 75 (69.5), of whose busy CUs' clocks the
-// matrix cores have 43 % and vector instructions 54 %.
+// many by their waves' chains of products and exponentials: a 64-key block of 128 rows takes 1.6 us alone in a CU, 2.3
+// beside a second workgroup and 4.2 beside two (heads of 64; of 128 in 4 bits 2.4 and 4.8), and with all pages in the
+// caches at most 4 % less, so its loads, one block ahead, are not what it waits for.  On an MI355X: 64 x 32768 keys at 5.2 TB/s
+// in 4 bits (with no arithmetic at all 5.5) and 5.7 to 5.9 in 8 bits; 64 sequences of 500 to 8000 keys in 4 bits 28.1
+// us (in bf16 77.5), 16 in 8 bits 39 (70); four chunks of 1024 rows over 4095 keys 75 (69.5), of whose busy CUs' clocks
+// the matrix cores have 44 % and vector instructions 56 %.
 //
 // The plan's borders are those of the cache in bf16 (pa_plan), and hold here (us, 16 / 4 heads of 128, 4 bits). One piece
 // / pieces of 128 keys: 512 keys 8.5 / 9.7, 1024 keys 11.5 / 9.8.  Pieces / even shares, which the
@@ -159,7 +161,7 @@ struct PqShared {
 // Keys [k_begin, k_end) of a tile of KV head kvh; whole: they are all its keys, and O and lse are written; else the
 // part, at part_at(row of the sequence, head).  Every wave takes 32-key blocks of its own, whose codes come into
 // registers DEPTH blocks ahead: with one more the steady rate is the same, and a segment starts and ends later (64
-// sequences of 500 to 8000 keys in 4 bits 28.5 us, so 29.9; 16 in 8 bits 38.6 and 39.9).  One load for all scale
+// sequences of 500 to 8000 keys in 4 bits 28.5 us, so 29.9 beside it; 16 in 8 bits 38.6 and 39.9).  One load for all scale
 // bytes of a block, given to the lanes by shuffles, was slower (30.6): it makes the chain longer.
 // ONE: the tile's rows are of one token.
 template <int D, int BITS, bool ONE, class PartAt>
@@ -512,7 +514,8 @@ __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per
 }
 
 // The first blocks of a sequence arrive 4 us after the last sum of the one before, in which a workgroup does 300 keys:
-// counted as 256, the workgroups end together (64 sequences of 500 to 8000 keys: 30.5 us, not counted 32.0; 512 as 256).
+// counted as 256, the workgroups end together (64 sequences of 500 to 8000 keys in 4 bits: 28.1 us, not counted 30.7, as 512
+// 28.5; 16 in 8 bits 39, 40.6 and 38.2).
 constexpr int PQ_EXTRA = 256 / PF_BLOCK;
 template <int D, int BITS>
 __global__ void __launch_bounds__(64 * PF_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
@@ -562,8 +565,9 @@ int mi_paged_attn_quant(void* stream, const void* Q, int64_t q_t, int64_t q_h, v
   p.ks = (const uint8_t*)cache->k_scale, p.vs = (const uint8_t*)cache->v_scale;
   p.scale_page = cache->scale_page_stride, p.scale_head = cache->scale_head_stride, p.scale_slot = cache->scale_slot_stride;
   hipStream_t hs = (hipStream_t)stream;
-  if (cache->format == MI_KV_E2M1) return cache->head_dim <= 64 ? pq_launch<64, 4>(p, plan, hs) : pq_launch<128, 4>(p, plan, hs);
-  return cache->head_dim <= 64 ? pq_launch<64, 8>(p, plan, hs) : pq_launch<128, 8>(p, plan, hs);
+  const bool narrow = cache->head_dim <= 64;
+  if (cache->format == MI_KV_E2M1) return narrow ? pq_launch<64, 4>(p, plan, hs) : pq_launch<128, 4>(p, plan, hs);
+  return narrow ? pq_launch<64, 8>(p, plan, hs) : pq_launch<128, 8>(p, plan, hs);
 }
 
 }  // extern "C"
