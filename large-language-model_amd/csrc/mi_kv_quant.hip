@@ -34,7 +34,7 @@ struct QuantView {
   int64_t scale_page, scale_head, scale_slot;
 };
 
-// The first sequence from s on that ends behind token t (n_seqs: none), each lane on its own: steps of 1, 1, 2, 4, .. until
+// The first sequence from s on that ends behind token t (n_seqs: none), each lane on its own: steps of 1, 2, 4, .. until
 // one does, and halves of the last step; the next sequence is one load away, any number of empty ones a few (two prompts of
 // 2000 tokens side by side appended in 7.2 us, with 4000 empty sequences between them in 8.2; one by one 299).
 __device__ __forceinline__ int first_after(const PagedView& pv, int s, int t) {
